@@ -19,6 +19,7 @@ GA_STATIC_SCRATCH_BYTES = 32 << 20
 GA_DEGREE_BUCKETS = 31
 GA_CLASSES_MIN_DEGREE = 16
 GA_ACT_NONE, GA_ACT_RELU, GA_ACT_ELU = 0, 1, 2
+GA_GATE_SILU, GA_GATE_GELU, GA_GATE_RELU = 0, 1, 2
 GA_F32, GA_BF16 = 0, 1
 GA_COPY_U, GA_COPY_E, GA_U_MUL_E, GA_U_ADD_E, GA_U_SUB_E, GA_U_DIV_E = 0, 1, 2, 3, 4, 5
 GA_SDDMM_ADD, GA_SDDMM_SUB, GA_SDDMM_MUL, GA_SDDMM_DIV = 0, 1, 2, 3
@@ -138,6 +139,21 @@ SIGNATURES = {
                                     ctypes.c_float, _int, _int, _vp, _sz, _vp]),
     "ga_gat_aggregate_from_z_act": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                            _i64, ctypes.c_float, _int, _int, _vp, _sz, _vp]),
+    "ga_rms_norm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _int, _vp]),
+    "ga_rms_norm_fp8": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _int, _vp]),
+    "ga_quantize_fp8": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp]),
+    "ga_quantize_weight_fp8": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp]),
+    "ga_rms_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "ga_rms_norm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_float, _int,
+                                    _vp, _sz, _vp]),
+    "ga_gated_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "ga_gated_linear": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _sz, _vp]),
+    "ga_gated_linear_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "ga_gated_linear_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int,
+                                        _int, _vp, _sz, _vp]),
+    "ga_linear_fp8": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "ga_gated_linear_fp8": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int,
+                                   _vp]),
 }
 
 _lib = None

@@ -1,0 +1,82 @@
+// Products of 8-bit rows (norm.hip): y = x w^T with x (rows, K) and w (M, K) in e4m3, a power-of-two
+// scale for every 128 values of a row of x and for every 128 x 128 values of w, and the gated form
+// act(x wg^T) * (x wu^T) of a feed-forward block.
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 takes 128 values of k at a time, exactly a block, and
+// multiplies by both scales itself: the products of all blocks add up in one fp32 accumulator with no
+// other instruction, at twice the rate of bf16.  Of every eight products that the instruction adds
+// first it keeps what lies within 2^-13 of the largest (measured); everything after that is fp32.
+#include "tile_mm.h"
+
+namespace ga {
+namespace {
+
+int check_fp8(int64_t rows, int64_t K, int64_t M, int dtype) {
+  if (rows < 0 || K <= 0 || M <= 0 || K % 128 != 0) return GA_EINVAL;
+  if (dtype != GA_F32 && dtype != GA_BF16) return GA_EUNSUPPORTED;
+  if (K > (1 << 22)) return GA_EUNSUPPORTED;               // 32-bit offsets inside a tile of 256 rows
+  return GA_OK;
+}
+
+TileMm fp8_product(const void *x8, const void *xs, const void *w0, const void *s0, const void *w1, const void *s1,
+                   int64_t rows, int64_t K, int64_t M) {
+  TileMm m{};
+  m.segments = 1;
+  m.a[0] = x8;
+  m.b0[0] = w0;
+  m.b1[0] = w1;
+  m.lda = m.ldb = K;
+  m.rows = rows;
+  m.cols = M;
+  m.K = K;
+  m.sa = (const uint8_t *)xs;
+  m.sb0 = (const uint8_t *)s0;
+  m.sb1 = (const uint8_t *)s1;
+  m.splits = 1;
+  return m;
+}
+
+template <typename T>
+int linear8(const TileMm &m, void *y, hipStream_t s) {
+  const bool whole = m.cols % 4 == 0 && aligned(y, 4 * sizeof(T));
+  return tile_mm_launch<true, false, false, false>(m, StoreEpi<T>{(T *)y, m.cols, whole}, s);
+}
+template <typename T>
+int gated8(const TileMm &m, void *h, int act, hipStream_t s) {
+  const bool whole = m.cols % 4 == 0 && aligned(h, 4 * sizeof(T));
+  return tile_mm_launch<true, false, false, true>(m, GateEpi<T>{(T *)h, m.cols, act, whole}, s);
+}
+
+}  // namespace
+}  // namespace ga
+
+extern "C" {
+
+int ga_linear_fp8(const void *x8, const void *x_scales, const void *w8, const void *w_scales, void *y, int64_t rows,
+                  int64_t K, int64_t M, int out_dtype, ga_stream_t stream) {
+  using namespace ga;
+  if (int rc = check_fp8(rows, K, M, out_dtype)) return rc;
+  if (rows == 0) return GA_OK;
+  if (!x8 || !x_scales || !w8 || !w_scales || !y) return GA_EINVAL;
+  if (!aligned(x8, 16) || !aligned(w8, 16) || !aligned(y, out_dtype == GA_F32 ? 4 : 2)) return GA_EALIGN;
+  const TileMm m = fp8_product(x8, x_scales, w8, w_scales, nullptr, nullptr, rows, K, M);
+  hipStream_t s = (hipStream_t)stream;
+  return out_dtype == GA_F32 ? linear8<float>(m, y, s) : linear8<bf16_t>(m, y, s);
+}
+
+int ga_gated_linear_fp8(const void *x8, const void *x_scales, const void *wg8, const void *wg_scales, const void *wu8,
+                        const void *wu_scales, void *h, int64_t rows, int64_t K, int64_t F, int activation,
+                        int out_dtype, ga_stream_t stream) {
+  using namespace ga;
+  if (int rc = check_fp8(rows, K, F, out_dtype)) return rc;
+  if (activation != GA_GATE_SILU && activation != GA_GATE_GELU && activation != GA_GATE_RELU) return GA_EUNSUPPORTED;
+  if (rows == 0) return GA_OK;
+  if (!x8 || !x_scales || !wg8 || !wg_scales || !wu8 || !wu_scales || !h) return GA_EINVAL;
+  if (!aligned(x8, 16) || !aligned(wg8, 16) || !aligned(wu8, 16) || !aligned(h, out_dtype == GA_F32 ? 4 : 2))
+    return GA_EALIGN;
+  const TileMm m = fp8_product(x8, x_scales, wg8, wg_scales, wu8, wu_scales, rows, K, F);
+  hipStream_t s = (hipStream_t)stream;
+  return out_dtype == GA_F32 ? gated8<float>(m, h, activation, s) : gated8<bf16_t>(m, h, activation, s);
+}
+
+}  // extern "C"

@@ -1403,3 +1403,295 @@ def linear_attn(x, weight, a_l=None, a_r=None):
         x.data_ptr(), weight.data_ptr(), a_l.data_ptr(), a_r.data_ptr(), z.data_ptr(),
         el.data_ptr(), er.data_ptr(), rows, K, M, heads, dt, _stream(x)), "ga_project_attn")
     return z, el, er
+
+
+# ------------------------------- rows of a residual stream: norm, 8 bits, feed-forward ----
+_GATES = {"silu": capi.GA_GATE_SILU, "gelu": capi.GA_GATE_GELU, "relu": capi.GA_GATE_RELU}
+FP8_BLOCK = 128          # values of a row, and rows and columns of a weight, that share a scale
+RMS_NORM_MAX_COLS = 16384
+
+
+def _gate(name) -> int:
+    if name not in _GATES:
+        raise RuntimeError("activation must be 'silu', 'gelu' or 'relu'")
+    return _GATES[name]
+
+
+def _check_rows(x, name: str) -> int:
+    """A (rows, cols) matrix of features; its dtype code."""
+    _check_input(x, name)
+    dt = _feat_dtype(x, name)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise RuntimeError(f"{name} must be (rows, columns)")
+    return dt
+
+
+def _check_like(x, name: str, shape, like) -> None:
+    _check_input(x, name)
+    if tuple(x.shape) != tuple(shape) or x.dtype != like.dtype or x.device != like.device:
+        raise RuntimeError(f"{name} must be {tuple(shape)}, of the dtype and on the device of the rows")
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _no_grad_form(what: str, *tensors) -> None:
+    if _wants_grad(*tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def _not_recorded(what: str) -> None:
+    """A backward pass in a recorded HIP graph and an eager one of the same leaves do not go
+    together in torch; the operators that return gradients can be recorded."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} with gradients cannot be recorded into a HIP graph: record it "
+                           f"under torch.no_grad() together with {what}_backward")
+
+
+def _launch(entry: str, device, *args) -> None:
+    """Call a C entry point on the current stream of ``device`` (its last argument)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        capi.check(getattr(capi.load(), entry)(*args, torch.cuda.current_stream(index).cuda_stream), entry)
+        return
+    with torch.cuda.device(index):
+        capi.check(getattr(capi.load(), entry)(*args, torch.cuda.current_stream(index).cuda_stream), entry)
+
+
+def _scratch(n_bytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(n_bytes, dtype=torch.uint8, device=device) if n_bytes else None
+
+
+def _norm_args(x, weight, residual, eps):
+    dt = _check_rows(x, "x")
+    rows, cols = int(x.shape[0]), int(x.shape[1])
+    if cols > RMS_NORM_MAX_COLS:
+        raise RuntimeError(f"x must have at most {RMS_NORM_MAX_COLS} columns")
+    if not eps >= 0:
+        raise RuntimeError("eps must not be negative")
+    _check_like(weight, "weight", (cols,), x)
+    if residual is not None:
+        _check_like(residual, "residual", x.shape, x)
+    return dt, rows, cols
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        _not_recorded("rms_norm")
+        got = _rms_norm(x, weight, residual, eps)
+        ctx.eps, ctx.residual = eps, residual is not None
+        ctx.save_for_backward(got[1] if ctx.residual else x, weight)
+        ctx.set_materialize_grads(False)
+        return got
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y, grad_sum=None):
+        _not_recorded("rms_norm")
+        total, weight = ctx.saved_tensors
+        if grad_y is None:
+            return grad_sum, None, grad_sum, None
+        gx, gw = rms_norm_backward(grad_y.contiguous(), total, weight, ctx.eps,
+                                   None if grad_sum is None else grad_sum.contiguous())
+        return gx, gw, gx if ctx.residual else None, None
+
+
+def _rms_norm(x, weight, residual, eps):
+    dt, rows, cols = _norm_args(x, weight, residual, eps)
+    y = torch.empty_like(x)
+    total = None if residual is None else torch.empty_like(x)
+    _launch("ga_rms_norm", x.device, x.data_ptr(), _ptr(residual), weight.data_ptr(), y.data_ptr(),
+            _ptr(total), rows, cols, float(eps), dt)
+    return y if residual is None else (y, total)
+
+
+def rms_norm(x, weight, residual=None, eps: float = 1e-6):
+    """Root-mean-square norm of rows, with the residual's addition: t = x + residual,
+    y = t / sqrt(mean(t^2) + eps) * weight for (rows, cols) features and a (cols,) weight of the
+    same dtype.  Returns y, or (y, t) with a residual: t is the stream that the next addition
+    takes.  t is summed and squared in fp32 and rounded only where it is stored.  Differentiable in x, weight
+    and residual."""
+    if _wants_grad(x, weight, residual):
+        return _RmsNorm.apply(x, weight, residual, eps)
+    return _rms_norm(x, weight, residual, eps)
+
+
+def rms_norm_backward(grad_y, total, weight, eps: float = 1e-6, grad_sum=None):
+    """Gradients of :func:`rms_norm`: ``total`` is the t it returned (x itself without a
+    residual), ``grad_sum`` what reaches t from elsewhere (None: nothing).  Returns
+    (gradient of x and of the residual alike, gradient of weight)."""
+    dt, rows, cols = _norm_args(total, weight, None, eps)
+    _check_like(grad_y, "grad_y", total.shape, total)
+    if grad_sum is not None:
+        _check_like(grad_sum, "grad_sum", total.shape, total)
+    gx, gw = torch.empty_like(total), torch.empty_like(weight)
+    ws = _scratch(capi.load().ga_rms_norm_backward_workspace_bytes(rows, cols), total.device)
+    _launch("ga_rms_norm_backward", total.device, grad_y.data_ptr(), total.data_ptr(),
+            weight.data_ptr(), _ptr(grad_sum), gx.data_ptr(), gw.data_ptr(), rows, cols, float(eps),
+            dt, ws.data_ptr(), ws.numel())
+    return gx, gw
+
+
+def _rows_8bit(rows: int, cols: int, device):
+    blocks = -(-cols // FP8_BLOCK)
+    return (torch.empty((rows, blocks * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=device),
+            torch.empty((rows, blocks), dtype=torch.float8_e8m0fnu, device=device))
+
+
+def rms_norm_fp8(x, weight, residual=None, eps: float = 1e-6):
+    """:func:`rms_norm` with y cut to 8 bits, as :func:`linear_fp8` takes rows.  Returns
+    (y8, scales), or (y8, scales, t) with a residual.  y8 is (rows, cols rounded up to 128) e4m3, zeros
+    behind cols; scales (rows, blocks of 128) e8m0: the smallest power of two that brings the
+    block's largest finite magnitude to at most 448.  Not differentiable."""
+    _no_grad_form("rms_norm_fp8", x, weight, residual)
+    dt, rows, cols = _norm_args(x, weight, residual, eps)
+    y8, scales = _rows_8bit(rows, cols, x.device)
+    total = None if residual is None else torch.empty_like(x)
+    _launch("ga_rms_norm_fp8", x.device, x.data_ptr(), _ptr(residual), weight.data_ptr(), y8.data_ptr(),
+            scales.data_ptr(), _ptr(total), rows, cols, float(eps), dt)
+    return (y8, scales) if residual is None else (y8, scales, total)
+
+
+def quantize_fp8(x):
+    """(rows, cols) features cut to 8 bits: (x8, scales) as :func:`rms_norm_fp8` returns them."""
+    _no_grad_form("quantize_fp8", x)
+    dt = _check_rows(x, "x")
+    rows, cols = int(x.shape[0]), int(x.shape[1])
+    if cols > RMS_NORM_MAX_COLS:
+        raise RuntimeError(f"x must have at most {RMS_NORM_MAX_COLS} columns")
+    x8, scales = _rows_8bit(rows, cols, x.device)
+    _launch("ga_quantize_fp8", x.device, x.data_ptr(), x8.data_ptr(), scales.data_ptr(), rows, cols, dt)
+    return x8, scales
+
+
+def quantize_weight_fp8(weight):
+    """A (K, M) weight as :func:`linear_fp8` takes it, done once per weight: (w8, scales) with w8
+    (M, K rounded up to 128) e4m3 and a power-of-two scale for every 128 x 128 values."""
+    _no_grad_form("quantize_weight_fp8", weight)
+    dt = _check_rows(weight, "weight")
+    k, m = int(weight.shape[0]), int(weight.shape[1])
+    if k == 0:
+        raise RuntimeError("weight must be (K, M)")
+    blocks = -(-k // FP8_BLOCK)
+    w8 = torch.empty((m, blocks * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=weight.device)
+    scales = torch.empty((-(-m // FP8_BLOCK), blocks), dtype=torch.float8_e8m0fnu, device=weight.device)
+    _launch("ga_quantize_weight_fp8", weight.device, weight.data_ptr(), w8.data_ptr(), scales.data_ptr(),
+            k, m, dt)
+    return w8, scales
+
+
+def _check_8bit(values, scales, name: str, device, rows_each: int, k=None) -> None:
+    _check_input(values, name)
+    _check_input(scales, name + "_scales")
+    if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float8_e8m0fnu:
+        raise RuntimeError(f"{name} must be float8_e4m3fn with float8_e8m0fnu scales")
+    if values.device != device or scales.device != device:
+        raise RuntimeError(f"{name} and its scales must be on the device of the rows")
+    if values.dim() != 2 or values.shape[1] == 0 or values.shape[1] % FP8_BLOCK or \
+            (k is not None and values.shape[1] != k):
+        raise RuntimeError(f"{name} must be (rows, K), K a multiple of {FP8_BLOCK} and the same for all")
+    if tuple(scales.shape) != (-(-int(values.shape[0]) // rows_each), values.shape[1] // FP8_BLOCK):
+        raise RuntimeError(f"{name}_scales must hold one scale per block of {name}")
+
+
+def _out_8bit(x8, m: int, out_dtype):
+    if out_dtype not in _DTYPES:
+        raise RuntimeError("out_dtype must be float32 or bfloat16")
+    return torch.empty((x8.shape[0], m), dtype=out_dtype, device=x8.device)
+
+
+def linear_fp8(x8, x_scales, w8, w_scales, out_dtype=torch.bfloat16):
+    """x @ weight for rows and a weight in 8 bits (:func:`quantize_fp8` or :func:`rms_norm_fp8`,
+    :func:`quantize_weight_fp8`): (rows, M) of ``out_dtype``, accumulated in fp32."""
+    _check_8bit(x8, x_scales, "x8", x8.device, 1)
+    k = int(x8.shape[1])
+    _check_8bit(w8, w_scales, "w8", x8.device, FP8_BLOCK, k)
+    y = _out_8bit(x8, int(w8.shape[0]), out_dtype)
+    if y.numel():
+        _launch("ga_linear_fp8", x8.device, x8.data_ptr(), x_scales.data_ptr(), w8.data_ptr(),
+                w_scales.data_ptr(), y.data_ptr(), int(x8.shape[0]), k, int(w8.shape[0]), _DTYPES[out_dtype])
+    return y
+
+
+def gated_linear_fp8(x8, x_scales, wg8, wg_scales, wu8, wu_scales, activation: str = "silu",
+                     out_dtype=torch.bfloat16):
+    """:func:`gated_linear` for rows and weights in 8 bits: act(x @ w_gate) * (x @ w_up) from one
+    kernel."""
+    act = _gate(activation)
+    _check_8bit(x8, x_scales, "x8", x8.device, 1)
+    k = int(x8.shape[1])
+    _check_8bit(wg8, wg_scales, "wg8", x8.device, FP8_BLOCK, k)
+    _check_8bit(wu8, wu_scales, "wu8", x8.device, FP8_BLOCK, k)
+    if wg8.shape != wu8.shape:
+        raise RuntimeError("wg8 and wu8 must share a shape")
+    h = _out_8bit(x8, int(wg8.shape[0]), out_dtype)
+    if h.numel():
+        _launch("ga_gated_linear_fp8", x8.device, x8.data_ptr(), x_scales.data_ptr(), wg8.data_ptr(),
+                wg_scales.data_ptr(), wu8.data_ptr(), wu_scales.data_ptr(), h.data_ptr(), int(x8.shape[0]), k,
+                int(wg8.shape[0]), act, _DTYPES[out_dtype])
+    return h
+
+
+def _gated_args(x, w_gate, w_up):
+    dt = _check_rows(x, "x")
+    rows, k = int(x.shape[0]), int(x.shape[1])
+    _check_input(w_gate, "w_gate")
+    if w_gate.dim() != 2 or w_gate.shape[0] != k or w_gate.shape[1] == 0:
+        raise RuntimeError("w_gate must be (K, F)")
+    f = int(w_gate.shape[1])
+    _check_like(w_gate, "w_gate", (k, f), x)
+    _check_like(w_up, "w_up", (k, f), x)
+    return dt, rows, k, f
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, activation):
+        _not_recorded("gated_linear")
+        h = _gated_linear(x, w_gate, w_up, activation)
+        ctx.activation = activation
+        ctx.save_for_backward(x, w_gate, w_up)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_h):
+        _not_recorded("gated_linear")
+        return (*gated_linear_backward(grad_h.contiguous(), *ctx.saved_tensors, ctx.activation), None)
+
+
+def _gated_linear(x, w_gate, w_up, activation):
+    act = _gate(activation)
+    dt, rows, k, f = _gated_args(x, w_gate, w_up)
+    h = torch.empty((rows, f), dtype=x.dtype, device=x.device)
+    n = capi.load().ga_gated_linear_workspace_bytes(rows, k, f, dt)
+    ws = _scratch(n, x.device)
+    _launch("ga_gated_linear", x.device, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(),
+            rows, k, f, act, dt, _ptr(ws), n)
+    return h
+
+
+def gated_linear(x, w_gate, w_up, activation: str = "silu"):
+    """act(x @ w_gate) * (x @ w_up) from one kernel: the first half of a feed-forward block
+    (:func:`linear` is the other).  x (rows, K), w_gate and w_up (K, F) of one dtype; activation
+    "silu" | "gelu" (with the error function) | "relu".  Sums in fp32, one rounding; fp32
+    products are those of :func:`linear_attn`.  Differentiable in all three."""
+    if _wants_grad(x, w_gate, w_up):
+        return _GatedLinear.apply(x, w_gate, w_up, activation)
+    return _gated_linear(x, w_gate, w_up, activation)
+
+
+def gated_linear_backward(grad_h, x, w_gate, w_up, activation: str = "silu"):
+    """Gradients of :func:`gated_linear`: (of x, of w_gate, of w_up).  Both products are formed
+    again; nothing but the operands is kept from the forward pass."""
+    act = _gate(activation)
+    dt, rows, k, f = _gated_args(x, w_gate, w_up)
+    _check_like(grad_h, "grad_h", (rows, f), x)
+    gx, gg, gu = torch.empty_like(x), torch.empty_like(w_gate), torch.empty_like(w_up)
+    n = capi.load().ga_gated_linear_backward_workspace_bytes(rows, k, f, dt)
+    ws = _scratch(n, x.device)
+    _launch("ga_gated_linear_backward", x.device, grad_h.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+            w_up.data_ptr(), gx.data_ptr(), gg.data_ptr(), gu.data_ptr(), rows, k, f, act, dt, _ptr(ws), n)
+    return gx, gg, gu

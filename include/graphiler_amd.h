@@ -758,6 +758,92 @@ int ga_project_attn_strided(const void *X, const void *W, const float *a_l, cons
                             void *Z, int64_t ldz, float *el, float *er, int64_t rows, int64_t K,
                             int64_t M, int64_t heads, int dtype, ga_stream_t stream);
 
+/* ---- rows of a residual stream: what a layer has after its attention ---------------- */
+
+/*
+ * Root-mean-square norm with the residual's addition:
+ *   t = x + residual (x alone where residual is NULL), y = t / sqrt(mean(t^2) + eps) * weight
+ * x, residual, y, sum (rows, cols), weight (cols), all of `dtype`; t is kept in fp32 and, where
+ * sum is not NULL (residual only), stored rounded there.  sum may be residual or x itself.
+ * GA_EUNSUPPORTED when cols > 16384.
+ */
+int ga_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *sum,
+                int64_t rows, int64_t cols, float eps, int dtype, ga_stream_t stream);
+
+/*
+ * The same with y cut to 8 bits (e4m3): y8 (rows, Kp) bytes with Kp = cols rounded up to 128,
+ * zeros behind cols, 16-byte aligned; scales (rows, Kp / 128) bytes e + 127: every block of 128
+ * values of a row is held as value / 2^e with the smallest e in [-126, 126] for which its
+ * largest finite magnitude is at most 448 * 2^e (zeros: e = 0).  Values that are not finite are NaN.
+ */
+int ga_rms_norm_fp8(const void *x, const void *residual, const void *weight, void *y8, void *scales,
+                    void *sum, int64_t rows, int64_t cols, float eps, int dtype, ga_stream_t stream);
+
+/* Rows x (rows, cols) of `dtype` cut to 8 bits: x8 and scales as ga_rms_norm_fp8 writes them. */
+int ga_quantize_fp8(const void *x, void *x8, void *scales, int64_t rows, int64_t cols, int dtype,
+                    ga_stream_t stream);
+
+/*
+ * A weight w (K, M) of `dtype` cut to 8 bits and laid out for ga_linear_fp8: w8 (M, Kp) bytes,
+ * Kp = K rounded up to 128, zeros behind K; scales (ceil(M / 128), Kp / 128) bytes, one for every
+ * 128 x 128 values.  Meant to be done once per weight.  GA_EUNSUPPORTED when M > 8388480.
+ */
+int ga_quantize_weight_fp8(const void *w, void *w8, void *scales, int64_t K, int64_t M, int dtype,
+                           ga_stream_t stream);
+
+/*
+ * Gradients of ga_rms_norm from t (`sum`; x itself where there was no residual):
+ *   grad_x = i (weight grad_y) - t i^3 mean(t weight grad_y) + grad_sum,  i = 1 / sqrt(mean(t^2) + eps)
+ *   grad_weight = sum over rows of grad_y t i
+ * grad_x is the gradient of x and of the residual alike; grad_sum (NULL: none) is what reaches t
+ * from elsewhere.  grad_x may be grad_y or grad_sum itself.  Every sum is fp32; its order depends
+ * on rows and cols only.
+ */
+size_t ga_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int ga_rms_norm_backward(const void *grad_y, const void *sum, const void *weight, const void *grad_sum,
+                         void *grad_x, void *grad_weight, int64_t rows, int64_t cols, float eps, int dtype,
+                         void *workspace, size_t workspace_bytes, ga_stream_t stream);
+
+/*
+ * The gated half of a feed-forward block: h = act(x @ w_gate) * (x @ w_up), x (rows, K), w_gate and
+ * w_up (K, F), h (rows, F), all of `dtype`, sums in fp32, h rounded once.  activation: ga_gate
+ * (silu: g / (1 + exp(-g)); gelu with the error function; relu).  fp32 products are formed from bf16
+ * pieces as in ga_linear_attn (less than 2^-22 of a product is left out; inputs that are not finite
+ * give NaN, operands below 2^-110 lose bits).  bf16 tensors whose rows are whole 16-byte pieces have to
+ * be 16-byte aligned.  GA_EUNSUPPORTED when K or F exceeds 2^21.
+ */
+enum ga_gate { GA_GATE_SILU = 0, GA_GATE_GELU = 1, GA_GATE_RELU = 2 };
+size_t ga_gated_linear_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype);
+int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h, int64_t rows, int64_t K,
+                    int64_t F, int activation, int dtype, void *workspace, size_t workspace_bytes,
+                    ga_stream_t stream);
+
+/*
+ * Its gradients: with gate = x @ w_gate, up = x @ w_up (formed again), du = grad_h act(gate),
+ * dg = grad_h up act'(gate) (both rounded to bf16 where the tensors are bf16):
+ *   grad_x = dg @ w_gate^T + du @ w_up^T, grad_gate = x^T @ dg, grad_up = x^T @ du.
+ * The slope of relu at 0 is 0.  No order of a sum depends on anything but the sizes.
+ */
+size_t ga_gated_linear_backward_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype);
+int ga_gated_linear_backward(const void *grad_h, const void *x, const void *w_gate, const void *w_up,
+                             void *grad_x, void *grad_gate, void *grad_up, int64_t rows, int64_t K,
+                             int64_t F, int activation, int dtype, void *workspace,
+                             size_t workspace_bytes, ga_stream_t stream);
+
+/*
+ * Products of 8-bit rows: y = x @ w^T, x8 (rows, K) and x_scales as ga_quantize_fp8 and
+ * ga_rms_norm_fp8 write them, w8 (M, K) and w_scales as ga_quantize_weight_fp8 does; K is the padded
+ * width, a multiple of 128.  y (rows, M) of `out_dtype`, accumulated in fp32 by the matrix
+ * instruction, which adds eight products at a time and drops of those what lies 2^-13 below the largest.
+ * A scale byte of 255 (NaN) makes its products NaN.  GA_EUNSUPPORTED when K exceeds 2^22.
+ */
+int ga_linear_fp8(const void *x8, const void *x_scales, const void *w8, const void *w_scales, void *y,
+                  int64_t rows, int64_t K, int64_t M, int out_dtype, ga_stream_t stream);
+/* h = act(x @ wg^T) * (x @ wu^T), h (rows, F) of `out_dtype`; wg8 and wu8 (F, K). */
+int ga_gated_linear_fp8(const void *x8, const void *x_scales, const void *wg8, const void *wg_scales,
+                        const void *wu8, const void *wu_scales, void *h, int64_t rows, int64_t K,
+                        int64_t F, int activation, int out_dtype, ga_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
