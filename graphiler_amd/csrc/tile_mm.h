@@ -3,15 +3,17 @@
 //
 //   C[i, j] = sum over k of A(i, k) B(j, k), accumulated in fp32
 //
-// An operand lies either with k adjacent ("by k": a row of 128 bytes is one step of k) or with
-// its rows adjacent ("across k": x^T in the gradient of a weight, a weight (K, M) in x W).  A step
-// is 64 values of k in bf16, 128 in 8 bits.  Both tiles of a step come straight from the memory into LDS
-// (16 bytes a lane, no registers), two steps deep: the next step's tiles are on their way while the matrix
-// instructions work on this one, one barrier a step.  The order of 16-byte pieces inside LDS is
-// chosen by what address a lane loads from, so that both the 16-byte reads of operands by k and
-// the transposing reads of operands across k (ds_read_b64_tr_b16) spread over all banks.
-// What lies outside the operands is not read: such a lane's offset is out of the buffer descriptor's range, for
-// which the load unit writes zeros.
+// An operand lies either with k adjacent ("by k") or with its rows adjacent ("across k": x^T in the
+// gradient of a weight, a weight (K, M) in x W).  A step is 64 bytes of k (32 values of bf16, 64 of
+// 8 bits).  Its tiles come straight from the memory into LDS (16 bytes a lane, no registers) and
+// four steps have a buffer: while one is multiplied, the next is there and two more are on their
+// way, so that a load has two steps' time and the operands of a step's first products are read
+// before the barrier in front of it.  One barrier a step: it says that the next step's tiles have landed and
+// that the last one's have been read.  The order of 16-byte pieces inside LDS is chosen by what address a
+// lane loads from, so that both the 16-byte reads of operands by k and the transposing reads of
+// operands across k (ds_read_b64_tr_b16) spread over all banks.  What lies outside the operands is not
+// read: such a lane's offset is out of the buffer descriptor's range, for which the load unit
+// writes zeros.
 //
 // The matrix instruction is given B as its first operand: a lane then holds four adjacent columns
 // of one row of C.
@@ -42,25 +44,25 @@ __device__ __forceinline__ rsrc_t tile_rsrc(const char *base) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
 }
 
-// One operand's tile of a step: R rows of C by 128 bytes of k, WAVES wavefronts move it.
+// One operand's tile of a step: R rows of C by 64 bytes of k, WAVES wavefronts move it.
 template <bool ACROSS, int R, int WAVES>
 struct Tile {
-  static constexpr int kBytes = R * 128;
+  static constexpr int kBytes = R * 64;
   static constexpr int kMoves = kBytes / 1024 / WAVES;       // of 1 KB by a wavefront
-  static constexpr int kRowPieces = ACROSS ? R / 8 : 8;      // 16-byte pieces of a tile row
+  static constexpr int kRowPieces = ACROSS ? R / 8 : 4;      // 16-byte pieces of a tile row
   static_assert(kMoves * 1024 * WAVES == kBytes, "whole moves");
 
-  // where piece c of tile row r lies in its row
+  // where piece c of tile row r lies in its row: at c ^ turn(r)
   static __device__ __forceinline__ int turn(int r) {
-    if constexpr (!ACROSS) return r & 7;
+    if constexpr (!ACROSS) return (r >> 2) & 3;
     else if constexpr (kRowPieces >= 16) return 2 * ((r & 3) | (((r >> 3) & 1) << 2));
     else return 2 * (((r >> 1) & 1) | (((r >> 3) & 1) << 1));
   }
 
   uint32_t off[kMoves];                  // from the step's base, or kOutside
-  int k[kMoves];                         // the value of k in the step a move's piece begins with
+  int k[kMoves];                         // across k: the value of k of the step that a move's piece is of; by k: its piece
 
-  // first: row of C the tile begins with; left: rows of C there are from there on
+  // left: rows of C there are from the tile's first on
   __device__ __forceinline__ void init(int64_t ld, int64_t left) {
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = threadIdx.x / kWave;
@@ -73,11 +75,11 @@ struct Tile {
         k[i] = r;
       } else {
         off[i] = r < left ? (uint32_t)(r * ld + c * 16) : kOutside;
-        k[i] = c * 8;
+        k[i] = (lane % kRowPieces) ^ ((lane >> 4) & 3);      // c: the same for all moves
       }
     }
   }
-  // `left`: values of k there are from this step on
+  // `left`: values of k (across) or 16-byte pieces of k there are from this step on
   __device__ __forceinline__ void load(const char *base, lds_char *to, int at, int left) const {
     const rsrc_t r = tile_rsrc(base);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -87,38 +89,48 @@ struct Tile {
                                                k[i] < left ? off[i] : kOutside, 0, 0, 0);
   }
 
-  // Where a lane's operands of the tile begin: of the 16 rows of C from row 0 on, of the first 32
-  // values of k.  Every read is one offset from an array of its own, which is how the compiler can
-  // tell that it is not of the tile on its way.
-  static __device__ __forceinline__ int at16(int r0, int s) {
-    const int lane = threadIdx.x & (kWave - 1), n = lane & 15, q = lane >> 4;
-    if constexpr (!ACROSS) {
-      return (r0 + n) * 128 + ((s * 4 + q) ^ (n & 7)) * 16;                // r0: a multiple of 16
+  // Where a lane's operand of the tile's rows from r0 (16 T times a whole number) on begins: 16 rows of bf16,
+  // k = 8 q ... + 7 (q: lane / 16), or 32 rows of 8 bits, of which lane / 32 takes pieces 0 and 1 or 2 and 3.
+  // The value is hidden from the compiler: a read's address then is one offset from an array of
+  // its own, by which it can tell that the read is not of a tile on its way.
+  template <bool FP8>
+  static __device__ __forceinline__ int lane_at(int r0) {
+    const int lane = threadIdx.x & (kWave - 1);
+    int at;
+    if constexpr (FP8) {
+      const int n = lane & 31, h = lane >> 5;
+      at = (r0 + n) * 64 + ((2 * h) ^ turn(n)) * 16;
+    } else if constexpr (!ACROSS) {
+      const int n = lane & 15, q = lane >> 4;
+      at = (r0 + n) * 64 + (q ^ turn(n)) * 16;
     } else {
       // lane n of 16 points at k = n / 4, rows 4 (n % 4) ... + 3 and receives row n, four k
-      const int kr = s * 32 + q * 8 + (n >> 2);
-      return kr * (kRowPieces * 16) + ((r0 / 8 + ((n & 3) >> 1)) ^ turn(kr)) * 16 + (n & 1) * 8;
+      const int n = lane & 15, q = lane >> 4, kr = q * 8 + (n >> 2);
+      at = kr * (kRowPieces * 16) + ((r0 / 8 + ((n & 3) >> 1)) ^ turn(kr)) * 16 + (n & 1) * 8;
     }
+    asm volatile("" : "+v"(at));
+    return at;
   }
-  // k = 32 s + 8 q ... + 7 (q: lane / 16) of the step, bf16
-  static __device__ __forceinline__ bf16x8 read16(const lds_char *t, int at) {
+  // tile i of 16 rows from r0 on; `base`: where the operand's tile lies in t
+  static __device__ __forceinline__ bf16x8 read16(const lds_char *t, int base, int at, int i) {
     if constexpr (!ACROSS) {
-      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8 *>(t + at);
+      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8 *>(t + (base + i * 1024) + at);
     } else {
       typedef __attribute__((address_space(3))) shortx4 lds_short4;
-      // k + 4 keeps its turn where 16 pieces make a row: bits 0, 1 and 3 of k; with 8, bits 1 and 3
-      const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(t + at));
-      const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(t + (at + 4 * kRowPieces * 16)));
+      // two pieces further on, before the turn; four k further on the turn is the same: it is made of bits 0, 1
+      // and 3 of k with 16 pieces, 1 and 3 with 8
+      const lds_char *p = t + base + (at ^ (i * 32));
+      const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)p);
+      const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(p + 4 * kRowPieces * 16));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
-  static constexpr int kReads16 = ACROSS ? 2 : 1;            // LDS instructions of read16
-  // 16 rows, 32 values of 8 bits: pieces q and q + 4 of the row
-  static __device__ __forceinline__ intx8 read8(const lds_char *t, int at) {
+  // tile i of 32 rows
+  static __device__ __forceinline__ intx8 read32(const lds_char *t, int base, int at, int i) {
     typedef int intx4 __attribute__((ext_vector_type(4)));
     typedef const __attribute__((address_space(3))) intx4 lds_int4;
-    const intx4 lo = *(lds_int4 *)(t + at);
-    const intx4 hi = *(lds_int4 *)(t + (at ^ 64));
+    const intx4 lo = *(lds_int4 *)(t + (base + i * 2048) + at);
+    const intx4 hi = *(lds_int4 *)(t + (base + i * 2048) + (at ^ 16));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
@@ -134,24 +146,53 @@ __device__ __forceinline__ void tile_of(int id, int n_tiles, int row_tiles, int 
   tc = in / high;
 }
 
-// Every wavefront's loads into LDS have arrived, and every wavefront has read the tiles before.
-__device__ __forceinline__ void tiles_landed() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+// All but the youngest n loads of this wavefront have arrived.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "six bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+}
+// ... of every wavefront, and every wavefront has read what it read before.
+template <int N>
+__device__ __forceinline__ void landed() {
+  asm volatile("" ::: "memory");
+  wait_loads<N>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
-// The kernel.  A workgroup of WM x WN wavefronts takes TM * WM * 16 rows and TN * WN * 16 rows of
-// B; PAIR: the first half of them in b0, the others (the same columns) in b1.  Epi gets a lane's
-// results: four adjacent columns of a row, of a PAIR both products'.
-template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int TM, int TN, typename Epi>
+// The operands and results of one matrix instruction: 16 x 16 x 32 of bf16, 32 x 32 x 64 of 8 bits.
+template <bool FP8> struct Mma;
+template <> struct Mma<false> {
+  static constexpr int kTile = 16, kQuads = 1;               // rows and columns; runs of four columns a lane holds
+  typedef bf16x8 operand;
+  typedef floatx4 result;
+};
+template <> struct Mma<true> {
+  static constexpr int kTile = 32, kQuads = 4;
+  typedef intx8 operand;
+  typedef float result __attribute__((ext_vector_type(16)));
+};
+
+constexpr int kSteps = 4;                // that have a buffer
+
+// The kernel.  A workgroup of WM x WN wavefronts takes TM * WM tiles of rows of A and TN * WN of B;
+// PAIR: the first half of them in b0, the others (the same columns) in b1.  Epi gets a lane's
+// results: four adjacent columns of a row, of a PAIR both products'.  BLOCKS: most blocks of 128 along k (8 bits).
+template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int TM, int TN, int BLOCKS, typename Epi>
 __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
-  constexpr int kWaves = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
+  typedef Mma<FP8> M;
+  constexpr int kT = M::kTile;
+  constexpr int kWaves = WM * WN, BM = WM * TM * kT, BN = WN * TN * kT;
   constexpr int kPair = PAIR ? 2 : 1, BC = BN / kPair, TC = TN / kPair;      // columns of C
-  constexpr int kStepK = FP8 ? 128 : 64, kElem = FP8 ? 1 : 2;
+  constexpr int kStepK = FP8 ? 64 : 32, kElem = FP8 ? 1 : 2;
   typedef Tile<A_ACROSS, BM, kWaves> TA;
   typedef Tile<B_ACROSS, BC, kWaves> TB;
-  __shared__ __attribute__((aligned(1024))) char la0[TA::kBytes], la1[TA::kBytes];
-  __shared__ __attribute__((aligned(1024))) char lb0[kPair * TB::kBytes], lb1[kPair * TB::kBytes];
+  constexpr int kStage = TA::kBytes + kPair * TB::kBytes;
+  constexpr int kLoads = TA::kMoves + kPair * TB::kMoves;    // of a wavefront a step
+  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage], stage2[kStage], stage3[kStage];
+  // 8 bits: scales of the tile's rows [block][wave row][row of the tile][tile], of the wavefronts' columns [block][..]
+  __shared__ __attribute__((aligned(16))) uint8_t row_scales[FP8 ? BLOCKS * BM : 16], col_scales[FP8 ? BLOCKS * 8 : 16];
 
   const int row_tiles = (int)((p.rows + BM - 1) / BM), col_tiles = (int)((p.cols + BC - 1) / BC);
   int tr, tc;
@@ -159,52 +200,43 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   const int64_t row0 = (int64_t)tr * BM, col0 = (int64_t)tc * BC;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / WN, wn = wave % WN;
-  const int lane = threadIdx.x & (kWave - 1), n = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & (kWave - 1), n = lane & (kT - 1), q = lane / kT;
 
   TA ta;
   TB tb;
   ta.init(p.lda, p.rows - row0);
   tb.init(p.ldb, p.cols - col0);
-  const int64_t a_step = A_ACROSS ? kStepK * p.lda : kStepK * kElem, b_step = B_ACROSS ? kStepK * p.ldb : kStepK * kElem;
+  const int64_t a_step = A_ACROSS ? kStepK * p.lda : 64, b_step = B_ACROSS ? kStepK * p.ldb : 64;
   const int64_t a_at = A_ACROSS ? row0 * kElem : row0 * p.lda, b_at = B_ACROSS ? col0 * kElem : col0 * p.ldb;
   const int per_segment = (int)((p.K + kStepK - 1) / kStepK);
   const int all = per_segment * p.segments, share = (all + p.splits - 1) / p.splits;
   const int first = (int)blockIdx.y * share, last = min(all, first + share);
 
-  floatx4 acc[TM][TN];
+  typename M::result acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0, 0, 0, 0};
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4 * M::kQuads; ++r) acc[i][j][r] = 0.0f;
 
-  // where the step to be fetched next begins
+  // where the step to be fetched next begins; `to_fetch` steps are left
+  int to_fetch = last - first;
   int seg = first / per_segment, in_seg = first - seg * per_segment;
   const char *a_ptr = nullptr, *b0_ptr = nullptr, *b1_ptr = nullptr;
-  // 8 bits: a scale for every row of A, one for a wavefront's columns, which lie in one block of 128
-  static_assert(!FP8 || (TC * 16 <= 128 && 128 % (TC * 16) == 0 && BC % (TC * 16) == 0), "columns of one scale");
-  const int kb = FP8 ? (int)(p.K / 128) : 0;
-  const rsrc_t sa_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t *>(FP8 ? p.sa + row0 * kb : nullptr), 0, (int)min((int64_t)BM, p.rows - row0) * kb, 0x00020000);
-  const int sa_at = ((wm * TM) * 16 + n) * kb;             // rows that are not there: out of range, 0
-  const int64_t sb_at = (min(col0 + wn * TC * 16, p.cols - 1) / 128) * kb;
   auto enter = [&]() {
     a_ptr = (const char *)p.a[seg] + a_at + in_seg * a_step;
     b0_ptr = (const char *)p.b0[seg] + b_at + in_seg * b_step;
     if constexpr (PAIR) b1_ptr = (const char *)p.b1[seg] + b_at + in_seg * b_step;
   };
-  auto stage = [&](lds_char *la, lds_char *lb, int (&scale_a)[TM], int (&scale_b)[2], bool live) {
-    const int left = live ? (int)min((int64_t)kStepK, p.K - (int64_t)in_seg * kStepK) : 0;
-    if constexpr (FP8) {                 // ahead of the tiles: loads return in order
-      if (live) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) scale_a[i] = __builtin_amdgcn_raw_buffer_load_b8(sa_rsrc, sa_at + i * 16 * kb + in_seg, 0, 0);
-        scale_b[0] = p.sb0[sb_at + in_seg];
-        if constexpr (PAIR) scale_b[1] = p.sb1[sb_at + in_seg];
-      }
-    }
-    ta.load(a_ptr, la, 0, left);
-    tb.load(b0_ptr, lb, 0, left);
-    if constexpr (PAIR) tb.load(b1_ptr, lb, TB::kBytes, left);
+  auto fetch = [&](lds_char *to) {
+    // what is left of k: values (across) and pieces of 16 bytes (by k, whose rows are whole pieces)
+    const int values = to_fetch > 0 ? (int)min((int64_t)kStepK, p.K - (int64_t)in_seg * kStepK) : 0;
+    const int pieces = (values * kElem + 15) / 16;
+    ta.load(a_ptr, to, 0, A_ACROSS ? values : pieces);
+    tb.load(b0_ptr, to, TA::kBytes, B_ACROSS ? values : pieces);
+    if constexpr (PAIR) tb.load(b1_ptr, to, TA::kBytes + TB::kBytes, B_ACROSS ? values : pieces);
+    --to_fetch;
     a_ptr += a_step;
     b0_ptr += b_step;
     b1_ptr += b_step;
@@ -213,98 +245,157 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
       if (++seg < p.segments) enter();
     }
   };
-  auto b_row = [&](int j) { return (wn * TC + (PAIR && j >= TC ? j - TC : j)) * 16; };
-  auto b_base = [&](int j) { return PAIR && j >= TC ? TB::kBytes : 0; };
-  auto multiply = [&](const lds_char *la, const lds_char *lb, const int (&scale_a)[TM], const int (&scale_b)[2]) {
-    if constexpr (FP8) {
-      intx8 b[TN], a[TM];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = TB::read8(lb, b_base(j) + TB::at16(b_row(j), 0));
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        a[i] = TA::read8(la, TA::at16((wm * TM + i) * 16, 0));
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              b[j], a[i], acc[i][j], 0, 0, 0, scale_b[PAIR && j >= TC], 0, scale_a[i]);
-      }
-      constexpr int kRead = 0x100, kMfma = 0x8;
-      __builtin_amdgcn_sched_group_barrier(kRead, TN * 2 + 4, 0);
-#pragma unroll
-      for (int g = 0; g < TM; ++g) {
-        __builtin_amdgcn_sched_group_barrier(kMfma, TN, 0);
-        __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
-      }
-    } else {
-      bf16x8 b[2][TN], a[2][TM];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j) b[s][j] = TB::read16(lb, b_base(j) + TB::at16(b_row(j), s));
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          a[s][i] = TA::read16(la, TA::at16((wm * TM + i) * 16, s));
-#pragma unroll
-          for (int j = 0; j < TN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[s][j], a[s][i], acc[i][j], 0, 0, 0);
-        }
-      }
-      // Operands are read two sets of TN products before they are multiplied, no earlier: all of
-      // them at once do not fit the registers.
-      constexpr int kRead = 0x100, kMfma = 0x8;
-      constexpr int kSpread = (TN * TB::kReads16 + TM - 1) / TM;
-      __builtin_amdgcn_sched_group_barrier(kRead, TN * TB::kReads16 + 2 * TA::kReads16, 0);
-#pragma unroll
-      for (int g = 0; g < TM; ++g) {
-        __builtin_amdgcn_sched_group_barrier(kMfma, TN, 0);
-        __builtin_amdgcn_sched_group_barrier(kRead, TA::kReads16 + kSpread, 0);
-      }
-#pragma unroll
-      for (int g = 0; g < TM; ++g) {
-        __builtin_amdgcn_sched_group_barrier(kMfma, TN, 0);
-        __builtin_amdgcn_sched_group_barrier(kRead, TA::kReads16, 0);
-      }
-    }
+  const int lane_a = TA::template lane_at<FP8>(wm * TM * kT), lane_b = TB::template lane_at<FP8>(wn * TC * kT);
+  auto read_a = [&](const lds_char *t, int i) {
+    if constexpr (FP8) return TA::read32(t, 0, lane_a, i);
+    else return TA::read16(t, 0, lane_a, i);
+  };
+  auto read_b = [&](const lds_char *t, int j) {
+    const bool second = PAIR && j >= TC;
+    const int base = TA::kBytes + (second ? TB::kBytes : 0), i = second ? j - TC : j;
+    if constexpr (FP8) return TB::read32(t, base, lane_b, i);
+    else return TB::read16(t, base, lane_b, i);
   };
 
-  lds_char *const A0 = (lds_char *)la0, *const A1 = (lds_char *)la1;
-  lds_char *const B0 = (lds_char *)lb0, *const B1 = (lds_char *)lb1;
-  int sa0[TM], sa1[TM], sb0[2], sb1[2];
+  if constexpr (FP8) {
+    static_assert(TC * kT <= 128 && 128 % (TC * kT) == 0 && BC % (TC * kT) == 0, "columns of one scale");
+    static_assert((TM == 2 || TM == 4) && WN * kPair <= 8, "scales of a step are a word and two bytes");
+    const int kb = (int)(p.K / 128);
+    for (int r = threadIdx.x; r < BM; r += kWaves * kWave) {
+      if (row0 + r >= p.rows) break;
+      const uint8_t *src = p.sa + (row0 + r) * kb;
+      const int at = r / (TM * kT) * (TM * kT) + r % kT * TM + r / kT % TM;
+      for (int b = 0; b < kb; ++b) row_scales[b * BM + at] = src[b];
+    }
+    for (int id = threadIdx.x; id < kb * 8; id += kWaves * kWave) {
+      const int b = id / 8, w = id % 8 % WN, second = id % 8 / WN;
+      const int64_t c = min(col0 + w * TC * kT, p.cols - 1) / 128 * kb + b;
+      if (second < kPair) col_scales[id] = second ? p.sb1[c] : p.sb0[c];
+    }
+  }
+
+  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1, *const L2 = (lds_char *)stage2,
+                 *const L3 = (lds_char *)stage3;
+  if (first < last) enter();
+  fetch(L0);
+  fetch(L1);
+  fetch(L2);
+
+  typename M::operand a[TM], b[2][TN];
+  int scale_a = 0, scale_b[2] = {0, 0};
+  auto read_scales = [&](int block, int &sa, int (&sb)[2]) {
+    if constexpr (FP8) {
+      const int at = block * BM + wm * TM * kT + n * TM;
+      if constexpr (TM == 4) sa = *reinterpret_cast<const int *>(row_scales + at);
+      else sa = *reinterpret_cast<const uint16_t *>(row_scales + at);
+      sb[0] = col_scales[block * 8 + wn];
+      if constexpr (PAIR) sb[1] = col_scales[block * 8 + WN + wn];
+    }
+  };
+  auto products = [&](int i, int which) {
+    if constexpr (FP8) {
+      const int sa = __builtin_amdgcn_ubfe(scale_a, 8 * i, 8);
 #pragma unroll
-  for (int i = 0; i < TM; ++i) sa0[i] = sa1[i] = 0;
-  sb0[0] = sb0[1] = sb1[0] = sb1[1] = 0;
-  if (first < last) {
-    enter();
-    stage(A0, B0, sa0, sb0, true);
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[which][j], a[i], acc[i][j], 0, 0, 0,
+                                                                   scale_b[PAIR && j >= TC], 0, sa);
+    } else {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[which][j], a[i], acc[i][j], 0, 0, 0);
+    }
+  };
+  // A step, whose tiles are in `here` and whose first operands have been read; `next` holds the step after and
+  // `freed` had the one before.  `which`: its number's last bit; 8 bits: two steps are a block of scales.
+  constexpr int kHalf = TM / 2;
+  // The products of half a step stay where they are: without this the compiler moves the long ones of 8 bits
+  // behind the barriers of the steps after, and keeps all their operands.
+  auto hold = [&](int i0) {
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[i0 + i][j]));
+    }
+  };
+  const int blocks = FP8 ? (int)(p.K / 128) : 0;
+  int block = 0;
+  auto step = [&](const lds_char *here, const lds_char *next, lds_char *freed, int which) {
+    landed<kLoads>();
+    fetch(freed);
+#pragma unroll
+    for (int i = kHalf; i < TM; ++i) a[i] = read_a(here, i);
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) products(i, which);
+    hold(0);
+    __builtin_amdgcn_sched_barrier(0);   // the reads below take registers that the products above free
+    int sa = scale_a, sb[2] = {scale_b[0], scale_b[1]};
+    if (FP8 && which == 1) {
+      block = min(block + 1, blocks - 1);
+      read_scales(block, sa, sb);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) b[which ^ 1][j] = read_b(next, j);
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) a[i] = read_a(next, i);
+#pragma unroll
+    for (int i = kHalf; i < TM; ++i) products(i, which);
+    hold(kHalf);
+    scale_a = sa;
+    scale_b[0] = sb[0];
+    scale_b[1] = sb[1];
+  };
+
+  wait_loads<2 * kLoads>();
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  landed<2 * kLoads>();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  read_scales(0, scale_a, scale_b);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) b[0][j] = read_b(L0, j);
+#pragma unroll
+  for (int i = 0; i < kHalf; ++i) a[i] = read_a(L0, i);
+  int left = last - first;
+  // in 8 bits the last turn may multiply zeros: a whole turn is one place where accumulators change
+  for (; FP8 ? left > 0 : left >= 4; left -= 4) {
+    step(L0, L1, L3, 0);
+    step(L1, L2, L0, 1);
+    step(L2, L3, L1, 0);
+    step(L3, L0, L2, 1);
   }
-  // Two steps a turn, so that each names its own arrays; where their number is odd the last turn
-  // multiplies zeros (no value of k is left, and nothing is read).
-  for (int step = first; step < last; step += 2) {
-    tiles_landed();
-    stage(A1, B1, sa1, sb1, step + 1 < last);
-    multiply(A0, B0, sa0, sb0);
-    tiles_landed();
-    if (step + 2 < last) stage(A0, B0, sa0, sb0, true);      // none is on its way when the kernel ends
-    multiply(A1, B1, sa1, sb1);
+  if (!FP8 && left > 0) {
+    step(L0, L1, L3, 0);
+    if (left > 1) {
+      step(L1, L2, L0, 1);
+      if (left > 2) step(L2, L3, L1, 0);
+    }
   }
+  wait_loads<0>();                       // nothing may arrive in LDS that another workgroup has by then
 
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int64_t row = row0 + (wm * TM + i) * 16 + n;
+    const int64_t row = row0 + (wm * TM + i) * kT + n;
     if (row >= p.rows) continue;
 #pragma unroll
-    for (int j = 0; j < TC; ++j) {
-      const int64_t col = col0 + (wn * TC + j) * 16 + q * 4;
-      if (col >= p.cols) continue;
-      const floatx4 second = acc[i][PAIR ? j + TC : j];
-      epi(p, row, col, acc[i][j], second);
-    }
+    for (int j = 0; j < TC; ++j)
+#pragma unroll
+      for (int g = 0; g < M::kQuads; ++g) {
+        const int64_t col = col0 + (wn * TC + j) * kT + g * 8 + q * 4;
+        if (col >= p.cols) continue;
+        floatx4 u, v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          u[r] = acc[i][j][4 * g + r];
+          v[r] = acc[i][PAIR ? j + TC : j][4 * g + r];
+        }
+        epi(p, row, col, u, v);
+      }
   }
 }
 
-template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int TM, int TN, typename Epi>
-__global__ __launch_bounds__(WM *WN *kWave, 2) void tile_mm_kernel(TileMm p, Epi epi) {
-  tile_mm<FP8, A_ACROSS, B_ACROSS, PAIR, WM, WN, TM, TN>(p, epi);
+template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int TM, int TN, int BLOCKS, typename Epi>
+__global__ __launch_bounds__(WM *WN *kWave, BLOCKS > 64 ? 1 : 2) void tile_mm_kernel(TileMm p, Epi epi) {
+  tile_mm<FP8, A_ACROSS, B_ACROSS, PAIR, WM, WN, TM, TN, BLOCKS>(p, epi);
 }
 
 // Four adjacent values of a row, of which `n` exist; `whole`: rows are 4-value aligned.
@@ -384,17 +475,27 @@ inline int64_t tiles_of(int64_t rows, int64_t cols, int bm, int bc) {
 // Launches the tile size that suits the grid: 256 x 256 rows of A and B (one workgroup of eight
 // wavefronts a compute unit) where there is one for most of the compute units, 128 x 128 otherwise.
 constexpr int64_t kLargeTilesFrom = 192;
+constexpr int kFewBlocks = 64, kMostBlocks = 256;        // of 128 along k, whose scales have room in LDS
 template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, typename Epi>
 int tile_mm_launch(const TileMm &p, const Epi &epi, hipStream_t s) {
-  const int64_t large = tiles_of(p.rows, p.cols, 256, PAIR ? 128 : 256) * p.splits;
+  const int64_t large = tiles_of(p.rows, p.cols, 256, PAIR ? 128 : 256);
   const int64_t small = tiles_of(p.rows, p.cols, 128, PAIR ? 64 : 128);
   if (small > 0x7fffffff || p.splits > 65535) return GA_EUNSUPPORTED;
-  if (large >= kLargeTilesFrom) {
-    const dim3 grid((unsigned)tiles_of(p.rows, p.cols, 256, PAIR ? 128 : 256), (unsigned)p.splits);
-    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, 8, 4, Epi>), grid, dim3(512), 0, s, p, epi);
-  } else {
-    const dim3 grid((unsigned)small, (unsigned)p.splits);
-    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, 4, 4, Epi>), grid, dim3(256), 0, s, p, epi);
+  if (FP8 && p.K > 128 * kMostBlocks) return GA_EUNSUPPORTED;
+  constexpr int kTall = FP8 ? 4 : 8, kWide = FP8 ? 2 : 4;  // tiles of a wavefront: 128 x 64
+  const bool few = !FP8 || p.K <= 128 * kFewBlocks;
+  if (large * p.splits >= kLargeTilesFrom && few) {
+    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kTall, kWide, kFewBlocks, Epi>),
+                       dim3((unsigned)large, (unsigned)p.splits), dim3(512), 0, s, p, epi);
+    return launch_status();
+  }
+  const dim3 grid((unsigned)small, (unsigned)p.splits);
+  if (few) {
+    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kTall / 2, kWide, kFewBlocks, Epi>), grid,
+                       dim3(256), 0, s, p, epi);
+  } else if constexpr (FP8) {
+    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kTall / 2, kWide, kMostBlocks, Epi>), grid,
+                       dim3(256), 0, s, p, epi);
   }
   return launch_status();
 }
