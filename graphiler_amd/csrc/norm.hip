@@ -206,21 +206,26 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(
   }
 }
 
-// The workgroups' sums of grad_w, folded in the order of the workgroups: 64 columns by four runs of them.
+// The workgroups' sums of grad_w: 16 columns by 64 runs of workgroups, the runs added in pairs.
+constexpr int kFoldCols = 16, kFoldRuns = 64;
 template <typename T>
-__global__ __launch_bounds__(kBlock) void norm_fold_kernel(const float *__restrict__ parts, T *__restrict__ gw,
+__global__ __launch_bounds__(kFoldCols *kFoldRuns) void norm_fold_kernel(const float *__restrict__ parts, T *__restrict__ gw,
                                                            int n_parts, int cols) {
-  __shared__ float some[kBlock];
-  const int c = blockIdx.x * kWave + (threadIdx.x & (kWave - 1)), run = threadIdx.x / kWave;
-  const int per = (n_parts + 3) / 4, end = min(n_parts, (run + 1) * per);
+  __shared__ float some[kFoldCols * kFoldRuns];
+  const int c = blockIdx.x * kFoldCols + (threadIdx.x & (kFoldCols - 1)), run = threadIdx.x / kFoldCols;
+  const int per = (n_parts + kFoldRuns - 1) / kFoldRuns, end = min(n_parts, (run + 1) * per);
   float s = 0.0f;
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 8
     for (int p = run * per; p < end; ++p) s += parts[(int64_t)p * cols + c];
+  }
   some[threadIdx.x] = s;
   __syncthreads();
-  if (run == 0 && c < cols)
-    f32_to_elem((some[threadIdx.x] + some[threadIdx.x + 64]) + (some[threadIdx.x + 128] + some[threadIdx.x + 192]),
-                gw[c]);
+  for (int half = kFoldRuns / 2; half > 0; half /= 2) {
+    if (run < half) some[threadIdx.x] += some[threadIdx.x + half * kFoldCols];
+    __syncthreads();
+  }
+  if (run == 0 && c < cols) f32_to_elem(some[threadIdx.x], gw[c]);
 }
 
 // A weight (K, M) as 8-bit rows of its columns: (M, padded K), a scale for every 128 x 128 values.
@@ -326,7 +331,8 @@ int grad_launch(const void *gy, const void *t, const void *w, const void *gt, vo
 #undef GA_GRAD
   const int rc = launch_status();
   if (rc != GA_OK) return rc;
-  hipLaunchKernelGGL((norm_fold_kernel<T>), dim3((unsigned)((cols + kWave - 1) / kWave)), dim3(kBlock), 0, s, parts,
+  hipLaunchKernelGGL((norm_fold_kernel<T>), dim3((unsigned)((cols + kFoldCols - 1) / kFoldCols)),
+                     dim3(kFoldCols * kFoldRuns), 0, s, parts,
                      (T *)gw, (int)grid, (int)cols);
   return launch_status();
 }

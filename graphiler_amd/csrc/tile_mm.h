@@ -4,16 +4,16 @@
 //   C[i, j] = sum over k of A(i, k) B(j, k), accumulated in fp32
 //
 // An operand lies either with k adjacent ("by k") or with its rows adjacent ("across k": x^T in the
-// gradient of a weight, a weight (K, M) in x W).  A step is 64 bytes of k (32 values of bf16, 64 of
-// 8 bits).  Its tiles come straight from the memory into LDS (16 bytes a lane, no registers) and
-// four steps have a buffer: while one is multiplied, the next is there and two more are on their
-// way, so that a load has two steps' time and the operands of a step's first products are read
-// before the barrier in front of it.  One barrier a step: it says that the next step's tiles have landed and
-// that the last one's have been read.  The order of 16-byte pieces inside LDS is chosen by what address a
-// lane loads from, so that both the 16-byte reads of operands by k and the transposing reads of
-// operands across k (ds_read_b64_tr_b16) spread over all banks.  What lies outside the operands is not
-// read: such a lane's offset is out of the buffer descriptor's range, for which the load unit
-// writes zeros.
+// gradient of a weight, a weight (K, M) in x W).  A step is 128 bytes of k, a whole cache line of a row (64
+// values of bf16, 128 of 8 bits).  Its tiles come straight from the memory into LDS (16 bytes a lane, no
+// registers), and two steps have a buffer.  A step is multiplied in four phases, two halves of k by two
+// halves of the wavefront's rows; the operands of a phase are read from LDS while the phase before
+// multiplies.  After the third a step's buffer has been read by all (the one barrier of a step): the tiles two
+// steps further on are sent for into it, with a whole step's time to arrive, and the first operands
+// of the next step are read.  The order of 16-byte pieces inside LDS is chosen by what address a lane loads
+// from, so that both the 16-byte reads of operands by k and the transposing reads of operands across k
+// (ds_read_b64_tr_b16) spread over all banks.  What lies outside the operands is not read: such a
+// lane's offset is out of the buffer descriptor's range, for which the load unit writes zeros.
 //
 // The matrix instruction is given B as its first operand: a lane then holds four adjacent columns
 // of one row of C.
@@ -44,17 +44,17 @@ __device__ __forceinline__ rsrc_t tile_rsrc(const char *base) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
 }
 
-// One operand's tile of a step: R rows of C by 64 bytes of k, WAVES wavefronts move it.
+// One operand's tile of a step: R rows of C by 128 bytes of k, WAVES wavefronts move it.
 template <bool ACROSS, int R, int WAVES>
 struct Tile {
-  static constexpr int kBytes = R * 64;
+  static constexpr int kBytes = R * 128;
   static constexpr int kMoves = kBytes / 1024 / WAVES;       // of 1 KB by a wavefront
-  static constexpr int kRowPieces = ACROSS ? R / 8 : 4;      // 16-byte pieces of a tile row
+  static constexpr int kRowPieces = ACROSS ? R / 8 : 8;      // 16-byte pieces of a tile row
   static_assert(kMoves * 1024 * WAVES == kBytes, "whole moves");
 
   // where piece c of tile row r lies in its row: at c ^ turn(r)
   static __device__ __forceinline__ int turn(int r) {
-    if constexpr (!ACROSS) return (r >> 2) & 3;
+    if constexpr (!ACROSS) return (r >> 1) & 7;
     else if constexpr (kRowPieces >= 16) return 2 * ((r & 3) | (((r >> 3) & 1) << 2));
     else return 2 * (((r >> 1) & 1) | (((r >> 3) & 1) << 1));
   }
@@ -75,7 +75,7 @@ struct Tile {
         k[i] = r;
       } else {
         off[i] = r < left ? (uint32_t)(r * ld + c * 16) : kOutside;
-        k[i] = (lane % kRowPieces) ^ ((lane >> 4) & 3);      // c: the same for all moves
+        k[i] = c;
       }
     }
   }
@@ -99,10 +99,10 @@ struct Tile {
     int at;
     if constexpr (FP8) {
       const int n = lane & 31, h = lane >> 5;
-      at = (r0 + n) * 64 + ((2 * h) ^ turn(n)) * 16;
+      at = (r0 + n) * 128 + ((2 * h) ^ turn(n)) * 16;
     } else if constexpr (!ACROSS) {
       const int n = lane & 15, q = lane >> 4;
-      at = (r0 + n) * 64 + (q ^ turn(n)) * 16;
+      at = (r0 + n) * 128 + (q ^ turn(n)) * 16;
     } else {
       // lane n of 16 points at k = n / 4, rows 4 (n % 4) ... + 3 and receives row n, four k
       const int n = lane & 15, q = lane >> 4, kr = q * 8 + (n >> 2);
@@ -111,26 +111,26 @@ struct Tile {
     asm volatile("" : "+v"(at));
     return at;
   }
-  // tile i of 16 rows from r0 on; `base`: where the operand's tile lies in t
-  static __device__ __forceinline__ bf16x8 read16(const lds_char *t, int base, int at, int i) {
+  // tile i of 16 rows from r0 on, half s of k; `base`: where the operand's tile lies in t
+  static __device__ __forceinline__ bf16x8 read16(const lds_char *t, int base, int at, int i, int s) {
     if constexpr (!ACROSS) {
-      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8 *>(t + (base + i * 1024) + at);
+      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8 *>(t + (base + i * 2048) + (at ^ (s * 64)));
     } else {
       typedef __attribute__((address_space(3))) shortx4 lds_short4;
-      // two pieces further on, before the turn; four k further on the turn is the same: it is made of bits 0, 1
+      // two pieces further on, before the turn; four or 32 k further on the turn is the same: it is made of bits 0, 1
       // and 3 of k with 16 pieces, 1 and 3 with 8
-      const lds_char *p = t + base + (at ^ (i * 32));
+      const lds_char *p = t + (base + s * 32 * kRowPieces * 16) + (at ^ (i * 32));
       const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)p);
       const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(p + 4 * kRowPieces * 16));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
-  // tile i of 32 rows
-  static __device__ __forceinline__ intx8 read32(const lds_char *t, int base, int at, int i) {
+  // tile i of 32 rows, half s of k
+  static __device__ __forceinline__ intx8 read32(const lds_char *t, int base, int at, int i, int s) {
     typedef int intx4 __attribute__((ext_vector_type(4)));
     typedef const __attribute__((address_space(3))) intx4 lds_int4;
-    const intx4 lo = *(lds_int4 *)(t + (base + i * 2048) + at);
-    const intx4 hi = *(lds_int4 *)(t + (base + i * 2048) + (at ^ 16));
+    const intx4 lo = *(lds_int4 *)(t + (base + i * 4096) + (at ^ (s * 64)));
+    const intx4 hi = *(lds_int4 *)(t + (base + i * 4096) + (at ^ (s * 64 + 16)));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
@@ -146,17 +146,17 @@ __device__ __forceinline__ void tile_of(int id, int n_tiles, int row_tiles, int 
   tc = in / high;
 }
 
-// All but the youngest n loads of this wavefront have arrived.
+// All but the youngest N loads of this wavefront have arrived.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   static_assert(N < 64, "six bits");
   __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
 }
-// ... of every wavefront, and every wavefront has read what it read before.
+// ... of every wavefront, and every wavefront has what it read or written in LDS behind it.
 template <int N>
 __device__ __forceinline__ void landed() {
   asm volatile("" ::: "memory");
-  wait_loads<N>();
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -174,8 +174,6 @@ template <> struct Mma<true> {
   typedef float result __attribute__((ext_vector_type(16)));
 };
 
-constexpr int kSteps = 4;                // that have a buffer
-
 // The kernel.  A workgroup of WM x WN wavefronts takes TM * WM tiles of rows of A and TN * WN of B;
 // PAIR: the first half of them in b0, the others (the same columns) in b1.  Epi gets a lane's
 // results: four adjacent columns of a row, of a PAIR both products'.  BLOCKS: most blocks of 128 along k (8 bits).
@@ -185,12 +183,12 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   constexpr int kT = M::kTile;
   constexpr int kWaves = WM * WN, BM = WM * TM * kT, BN = WN * TN * kT;
   constexpr int kPair = PAIR ? 2 : 1, BC = BN / kPair, TC = TN / kPair;      // columns of C
-  constexpr int kStepK = FP8 ? 64 : 32, kElem = FP8 ? 1 : 2;
+  constexpr int kStepK = FP8 ? 128 : 64, kElem = FP8 ? 1 : 2;
   typedef Tile<A_ACROSS, BM, kWaves> TA;
   typedef Tile<B_ACROSS, BC, kWaves> TB;
   constexpr int kStage = TA::kBytes + kPair * TB::kBytes;
   constexpr int kLoads = TA::kMoves + kPair * TB::kMoves;    // of a wavefront a step
-  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage], stage2[kStage], stage3[kStage];
+  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage];
   // 8 bits: scales of the tile's rows [block][wave row][row of the tile][tile], of the wavefronts' columns [block][..]
   __shared__ __attribute__((aligned(16))) uint8_t row_scales[FP8 ? BLOCKS * BM : 16], col_scales[FP8 ? BLOCKS * 8 : 16];
 
@@ -206,7 +204,7 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   TB tb;
   ta.init(p.lda, p.rows - row0);
   tb.init(p.ldb, p.cols - col0);
-  const int64_t a_step = A_ACROSS ? kStepK * p.lda : 64, b_step = B_ACROSS ? kStepK * p.ldb : 64;
+  const int64_t a_step = A_ACROSS ? kStepK * p.lda : 128, b_step = B_ACROSS ? kStepK * p.ldb : 128;
   const int64_t a_at = A_ACROSS ? row0 * kElem : row0 * p.lda, b_at = B_ACROSS ? col0 * kElem : col0 * p.ldb;
   const int per_segment = (int)((p.K + kStepK - 1) / kStepK);
   const int all = per_segment * p.segments, share = (all + p.splits - 1) / p.splits;
@@ -246,15 +244,15 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     }
   };
   const int lane_a = TA::template lane_at<FP8>(wm * TM * kT), lane_b = TB::template lane_at<FP8>(wn * TC * kT);
-  auto read_a = [&](const lds_char *t, int i) {
-    if constexpr (FP8) return TA::read32(t, 0, lane_a, i);
-    else return TA::read16(t, 0, lane_a, i);
+  auto read_a = [&](const lds_char *t, int i, int half) {
+    if constexpr (FP8) return TA::read32(t, 0, lane_a, i, half);
+    else return TA::read16(t, 0, lane_a, i, half);
   };
-  auto read_b = [&](const lds_char *t, int j) {
+  auto read_b = [&](const lds_char *t, int j, int half) {
     const bool second = PAIR && j >= TC;
     const int base = TA::kBytes + (second ? TB::kBytes : 0), i = second ? j - TC : j;
-    if constexpr (FP8) return TB::read32(t, base, lane_b, i);
-    else return TB::read16(t, base, lane_b, i);
+    if constexpr (FP8) return TB::read32(t, base, lane_b, i, half);
+    else return TB::read16(t, base, lane_b, i, half);
   };
 
   if constexpr (FP8) {
@@ -274,12 +272,10 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     }
   }
 
-  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1, *const L2 = (lds_char *)stage2,
-                 *const L3 = (lds_char *)stage3;
+  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1;
   if (first < last) enter();
   fetch(L0);
   fetch(L1);
-  fetch(L2);
 
   typename M::operand a[TM], b[2][TN];
   int scale_a = 0, scale_b[2] = {0, 0};
@@ -305,71 +301,70 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[which][j], a[i], acc[i][j], 0, 0, 0);
     }
   };
-  // A step, whose tiles are in `here` and whose first operands have been read; `next` holds the step after and
-  // `freed` had the one before.  `which`: its number's last bit; 8 bits: two steps are a block of scales.
+  // A step, whose tiles are in `here` and whose first operands have been read; `next` holds the step after.
   constexpr int kHalf = TM / 2;
   // The products of half a step stay where they are: without this the compiler moves the long ones of 8 bits
   // behind the barriers of the steps after, and keeps all their operands.
   auto hold = [&](int i0) {
-    if constexpr (FP8) {
 #pragma unroll
-      for (int i = 0; i < kHalf; ++i)
+    for (int i = 0; i < kHalf; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[i0 + i][j]));
-    }
+      for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[i0 + i][j]));
   };
   const int blocks = FP8 ? (int)(p.K / 128) : 0;
   int block = 0;
-  auto step = [&](const lds_char *here, const lds_char *next, lds_char *freed, int which) {
-    landed<kLoads>();
-    fetch(freed);
+  auto first_operands = [&](const lds_char *t, int half) {
 #pragma unroll
-    for (int i = kHalf; i < TM; ++i) a[i] = read_a(here, i);
+    for (int j = 0; j < TN; ++j) b[half][j] = read_b(t, j, half);
 #pragma unroll
-    for (int i = 0; i < kHalf; ++i) products(i, which);
+    for (int i = 0; i < kHalf; ++i) a[i] = read_a(t, i, half);
+  };
+  auto second_operands = [&](const lds_char *t, int half) {
+#pragma unroll
+    for (int i = kHalf; i < TM; ++i) a[i] = read_a(t, i, half);
+  };
+  auto first_products = [&](int half) {
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) products(i, half);
     hold(0);
-    __builtin_amdgcn_sched_barrier(0);   // the reads below take registers that the products above free
+  };
+  auto second_products = [&](int half) {
+#pragma unroll
+    for (int i = kHalf; i < TM; ++i) products(i, half);
+    hold(kHalf);
+  };
+  auto step = [&](lds_char *here, const lds_char *next) {
+    second_operands(here, 0);
+    first_products(0);
+    __builtin_amdgcn_sched_barrier(0);   // a phase's reads take registers that the phase before frees
+    first_operands(here, 1);
+    second_products(0);
+    __builtin_amdgcn_sched_barrier(0);
+    second_operands(here, 1);
+    first_products(1);
+    landed<0>();
+    fetch(here);
     int sa = scale_a, sb[2] = {scale_b[0], scale_b[1]};
-    if (FP8 && which == 1) {
+    if constexpr (FP8) {
       block = min(block + 1, blocks - 1);
       read_scales(block, sa, sb);
     }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) b[which ^ 1][j] = read_b(next, j);
-#pragma unroll
-    for (int i = 0; i < kHalf; ++i) a[i] = read_a(next, i);
-#pragma unroll
-    for (int i = kHalf; i < TM; ++i) products(i, which);
-    hold(kHalf);
+    first_operands(next, 0);
+    second_products(1);
     scale_a = sa;
     scale_b[0] = sb[0];
     scale_b[1] = sb[1];
   };
 
-  wait_loads<2 * kLoads>();
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  landed<2 * kLoads>();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  landed<kLoads>();
   read_scales(0, scale_a, scale_b);
-#pragma unroll
-  for (int j = 0; j < TN; ++j) b[0][j] = read_b(L0, j);
-#pragma unroll
-  for (int i = 0; i < kHalf; ++i) a[i] = read_a(L0, i);
+  first_operands(L0, 0);
   int left = last - first;
-  // in 8 bits the last turn may multiply zeros: a whole turn is one place where accumulators change
-  for (; FP8 ? left > 0 : left >= 4; left -= 4) {
-    step(L0, L1, L3, 0);
-    step(L1, L2, L0, 1);
-    step(L2, L3, L1, 0);
-    step(L3, L0, L2, 1);
+  for (; left >= 2; left -= 2) {         // two steps a turn, so that each names its own arrays
+    step(L0, L1);
+    step(L1, L0);
   }
-  if (!FP8 && left > 0) {
-    step(L0, L1, L3, 0);
-    if (left > 1) {
-      step(L1, L2, L0, 1);
-      if (left > 2) step(L2, L3, L1, 0);
-    }
-  }
+  if (left > 0) step(L0, L1);
   wait_loads<0>();                       // nothing may arrive in LDS that another workgroup has by then
 
 #pragma unroll
@@ -472,32 +467,38 @@ inline int64_t tiles_of(int64_t rows, int64_t cols, int bm, int bc) {
   return ((rows + bm - 1) / bm) * ((cols + bc - 1) / bc);
 }
 
-// Launches the tile size that suits the grid: 256 x 256 rows of A and B (one workgroup of eight
-// wavefronts a compute unit) where there is one for most of the compute units, 128 x 128 otherwise.
+// The tiles a product may be cut into, rows by rows of B (of a PAIR: of both): 128 x 128 by four
+// wavefronts, two such workgroups a compute unit, of which one multiplies while the other begins or
+// stores, or 256 x 256 by eight.
+enum { kTile128, kTile256 };
 constexpr int64_t kLargeTilesFrom = 192;
-constexpr int kFewBlocks = 64, kMostBlocks = 256;        // of 128 along k, whose scales have room in LDS
+inline int tile_for(const TileMm &p, bool fp8, bool pair) {
+  const int64_t large = tiles_of(p.rows, p.cols, 256, pair ? 128 : 256) * p.splits;
+  return large >= kLargeTilesFrom ? kTile256 : kTile128;
+}
+
+template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int TM, int TN, int BLOCKS, typename Epi>
+int tile_mm_launch_as(const TileMm &p, const Epi &epi, hipStream_t s) {
+  constexpr int kT = Mma<FP8>::kTile;
+  const int64_t tiles = tiles_of(p.rows, p.cols, WM * TM * kT, WN * TN * kT / (PAIR ? 2 : 1));
+  if (tiles > 0x7fffffff || p.splits > 65535) return GA_EUNSUPPORTED;
+  hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, WM, WN, TM, TN, BLOCKS, Epi>),
+                     dim3((unsigned)tiles, (unsigned)p.splits), dim3(WM * WN * kWave), 0, s, p, epi);
+  return launch_status();
+}
+
+constexpr int kMostBlocks = 256;         // of 128 along k, whose scales have room in LDS
 template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, typename Epi>
 int tile_mm_launch(const TileMm &p, const Epi &epi, hipStream_t s) {
-  const int64_t large = tiles_of(p.rows, p.cols, 256, PAIR ? 128 : 256);
-  const int64_t small = tiles_of(p.rows, p.cols, 128, PAIR ? 64 : 128);
-  if (small > 0x7fffffff || p.splits > 65535) return GA_EUNSUPPORTED;
-  if (FP8 && p.K > 128 * kMostBlocks) return GA_EUNSUPPORTED;
-  constexpr int kTall = FP8 ? 4 : 8, kWide = FP8 ? 2 : 4;  // tiles of a wavefront: 128 x 64
-  const bool few = !FP8 || p.K <= 128 * kFewBlocks;
-  if (large * p.splits >= kLargeTilesFrom && few) {
-    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kTall, kWide, kFewBlocks, Epi>),
-                       dim3((unsigned)large, (unsigned)p.splits), dim3(512), 0, s, p, epi);
-    return launch_status();
-  }
-  const dim3 grid((unsigned)small, (unsigned)p.splits);
-  if (few) {
-    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kTall / 2, kWide, kFewBlocks, Epi>), grid,
-                       dim3(256), 0, s, p, epi);
-  } else if constexpr (FP8) {
-    hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kTall / 2, kWide, kMostBlocks, Epi>), grid,
-                       dim3(256), 0, s, p, epi);
-  }
-  return launch_status();
+  constexpr int kHigh = FP8 ? 4 : 8, kLow = kHigh / 2, kWide = FP8 ? 2 : 4;    // tiles of a wavefront
+  const int blocks = FP8 ? (int)((p.K + 127) / 128) : 0;
+  if (blocks > kMostBlocks) return GA_EUNSUPPORTED;
+  const int tile = tile_for(p, FP8, PAIR);
+  if (tile == kTile256 && blocks <= 64)
+    return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, 64>(p, epi, s);
+  if (blocks <= 32) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 32>(p, epi, s);
+  if constexpr (FP8) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, kMostBlocks>(p, epi, s);
+  return GA_EUNSUPPORTED;
 }
 
 }  // namespace ga
