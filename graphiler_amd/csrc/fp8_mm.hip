@@ -38,13 +38,11 @@ TileMm fp8_product(const void *x8, const void *xs, const void *w0, const void *s
 
 template <typename T>
 int linear8(const TileMm &m, void *y, hipStream_t s) {
-  const bool whole = m.cols % 4 == 0 && aligned(y, 4 * sizeof(T));
-  return tile_mm_launch<true, false, false, false>(m, StoreEpi<T>{(T *)y, m.cols, whole}, s);
+  return tile_mm_launch<true, false, false, false>(m, StoreEpi<T>((T *)y, m.cols), s);
 }
 template <typename T>
 int gated8(const TileMm &m, void *h, int act, hipStream_t s) {
-  const bool whole = m.cols % 4 == 0 && aligned(h, 4 * sizeof(T));
-  return tile_mm_launch<true, false, false, true>(m, GateEpi<T>{(T *)h, m.cols, act, whole}, s);
+  return tile_mm_launch<true, false, false, true>(m, GateEpi<T>((T *)h, m.cols, act), s);
 }
 
 }  // namespace

@@ -59,30 +59,45 @@ __global__ __launch_bounds__(kBlock) void lay_out_kernel(LayOut p) {
   }
 }
 
-// dg and du of a tile, as operands of the products after: bf16 rows of `ld` values, or three planes of pieces
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// dg and du of a tile, as operands of the products after: bf16 rows of `ld` values, of fp32 three planes of pieces.
 template <typename T>
-struct GradEpi {
+struct GradEpi : Stored<bf16_t> {
+  static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1, kOut = 2 * kPieces;
   const T *gh;
   int64_t gh_cols;
   bf16_t *dg, *du;
   int64_t ld, plane;
   int act;
   bool whole;                            // rows of gh are whole groups of four
-  __device__ __forceinline__ void operator()(const TileMm &, int64_t row, int64_t col, const floatx4 &g,
-                                             const floatx4 &u) const {
-    floatx4 t = {0, 0, 0, 0};
-    const T *src = gh + row * gh_cols + col;
+  __device__ __forceinline__ void make(const TileMm &p, int64_t row, int64_t col, const floatx4 &g, const floatx4 &u,
+                                       uintx2 (&o)[kOut]) const {
+    // no branch around a load, so that many are on their way: what is not there is out of range, 0
+    const int64_t row0 = row & ~(int64_t)255;                // the same for a tile's rows
+    const rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T *>(gh + uniform(row0) * gh_cols), 0,
+        (int)(min((int64_t)256, max(p.rows - uniform(row0), (int64_t)0)) * gh_cols * (int)sizeof(T)), 0x00020000);
+    const uint32_t at = ((uint32_t)(row - row0) * (uint32_t)gh_cols + (uint32_t)col) * sizeof(T);
+    floatx4 t;
     if (whole) {
+      const uint32_t o = col < gh_cols ? at : kOutside;
       if constexpr (sizeof(T) == 4) {
-        t = *reinterpret_cast<const floatx4 *>(src);
+        t = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(src, o, 0, 0));
       } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(src);
-        t = floatx4{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
+        const uintx2 w = __builtin_bit_cast(uintx2, __builtin_amdgcn_raw_buffer_load_b64(src, o, 0, 0));
+        t = floatx4{bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
       }
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (col + r < gh_cols) t[r] = elem_to_f32(src[r]);
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t o = col + r < gh_cols ? at + r * sizeof(T) : kOutside;
+        if constexpr (sizeof(T) == 4) t[r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src, o, 0, 0));
+        else t[r] = bf16_lo((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(src, o, 0, 0));
+      }
     }
     floatx4 a, b;
 #pragma unroll
@@ -90,37 +105,29 @@ struct GradEpi {
       a[r] = t[r] * u[r] * gate_slope(act, g[r]);
       b[r] = t[r] * gate_of(act, g[r]);
     }
-    const int64_t at = row * ld + col;
-    if constexpr (sizeof(T) == 2) {
-      store4(dg + at, a, 4, true);
-      store4(du + at, b, 4, true);
+    if constexpr (kPieces == 1) {
+      o[0] = pack(a);
+      o[1] = pack(b);
     } else {
-      put(dg + at, a);
-      put(du + at, b);
+      cut(a, o[0], o[1], o[2]);
+      cut(b, o[3], o[4], o[5]);
     }
   }
-  __device__ __forceinline__ void put(bf16_t *to, const floatx4 &v) const {
+  static __device__ __forceinline__ void cut(const floatx4 &v, uintx2 &o0, uintx2 &o1, uintx2 &o2) {
     uint32_t p[3][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) pieces(v[r], p[0][r], p[1][r], p[2][r]);
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      *reinterpret_cast<uint2 *>(to + i * plane) = uint2{p[i][0] | (p[i][1] << 16), p[i][2] | (p[i][3] << 16)};
+    o0 = uintx2{p[0][0] | (p[0][1] << 16), p[0][2] | (p[0][3] << 16)};
+    o1 = uintx2{p[1][0] | (p[1][1] << 16), p[1][2] | (p[1][3] << 16)};
+    o2 = uintx2{p[2][0] | (p[2][1] << 16), p[2][2] | (p[2][3] << 16)};
+  }
+  __device__ __forceinline__ void store(const TileMm &p, int k, int64_t row, int64_t col, const uintx4 &w) const {
+    bf16_t *to = (k < kPieces ? dg : du) + k % kPieces * plane;
+    store_chunk(to + row * ld + col, w, p.cols - col);
   }
 };
 
-// Both products of one part of the contraction, in fp32: part 2 s of the first product, 2 s + 1 of the second.
-struct PartEpi {
-  float *parts;
-  int64_t ld, plane;
-  bool whole;
-  __device__ __forceinline__ void operator()(const TileMm &p, int64_t row, int64_t col, const floatx4 &u,
-                                             const floatx4 &v) const {
-    float *to = parts + 2 * (int64_t)blockIdx.y * plane + row * ld + col;
-    store4(to, u, p.cols - col, whole);
-    store4(to + plane, v, p.cols - col, whole);
-  }
-};
+// Sums of the parts of a contraction; a part is the first product's values and then the second's.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void join_parts_kernel(const float *__restrict__ parts, T *__restrict__ out0,
                                                             T *__restrict__ out1, int64_t n, int splits) {
@@ -247,8 +254,7 @@ int forward(const void *x, const void *wg, const void *wu, void *h, int64_t rows
   Operands o;
   if (int rc = lay_operands<T>(p, x, wg, wu, rows, K, F, ws, o, s)) return rc;
   const TileMm m = both_products(p, o, rows, K, F);
-  const bool whole = F % 4 == 0 && aligned(h, 4 * sizeof(T));
-  return tile_mm_launch<false, false, true, true>(m, GateEpi<T>{(T *)h, F, act, whole}, s);
+  return tile_mm_launch<false, false, true, true>(m, GateEpi<T>((T *)h, F, act), s);
 }
 
 template <typename T>
@@ -261,7 +267,7 @@ int backward(const void *gh, const void *x, const void *wg, const void *wu, void
   {
     // the columns behind F, zeros of the laid out weights, are stored too: they are operands below
     const TileMm m = both_products(p, o, rows, K, p.Fp);
-    const GradEpi<T> e{(const T *)gh, F, dg, du, p.Fp, d_plane, act, F % 4 == 0 && p.Fp == F && aligned(gh, 4 * sizeof(T))};
+    const GradEpi<T> e{{}, (const T *)gh, F, dg, du, p.Fp, d_plane, act, F % 4 == 0 && aligned(gh, 4 * sizeof(T))};
     if (int rc = tile_mm_launch<false, false, true, true>(m, e, s)) return rc;
   }
   {
@@ -273,8 +279,7 @@ int backward(const void *gh, const void *x, const void *wg, const void *wu, void
     m.splits = 1;
     add_segments(m, p.pieces, dg, d_plane, o.wg, nullptr, w_plane);
     add_segments(m, p.pieces, du, d_plane, o.wu, nullptr, w_plane);
-    const StoreEpi<T> e{(T *)gx, K, K % 4 == 0 && aligned(gx, 4 * sizeof(T))};
-    if (int rc = tile_mm_launch<false, false, false, false>(m, e, s)) return rc;
+    if (int rc = tile_mm_launch<false, false, false, false>(m, StoreEpi<T>((T *)gx, K), s)) return rc;
   }
   TileMm m{};
   m.lda = 2 * p.Kp;
@@ -284,12 +289,11 @@ int backward(const void *gh, const void *x, const void *wg, const void *wu, void
   m.K = rows;
   m.splits = p.splits;
   add_segments(m, p.pieces, o.x, x_plane, dg, du, d_plane);
-  if (p.splits == 1) {
-    const bool whole = F % 4 == 0 && aligned(gwg, 4 * sizeof(T)) && aligned(gwu, 4 * sizeof(T));
-    return tile_mm_launch<false, true, true, true>(m, StorePairEpi<T>{(T *)gwg, (T *)gwu, F, whole}, s);
-  }
+  if (p.splits == 1)
+    return tile_mm_launch<false, true, true, true>(m, StorePairEpi<T>((T *)gwg, (T *)gwu, F, 0), s);
   float *parts = (float *)(ws + p.parts);
-  if (int rc = tile_mm_launch<false, true, true, true>(m, PartEpi{parts, F, K * F, F % 4 == 0}, s)) return rc;
+  const StorePairEpi<float> e(parts, parts + K * F, F, 2 * K * F);
+  if (int rc = tile_mm_launch<false, true, true, true>(m, e, s)) return rc;
   hipLaunchKernelGGL((join_parts_kernel<T>), dim3(stream_grid(2 * K * F)), dim3(kBlock), 0, s, parts, (T *)gwg,
                      (T *)gwu, K * F, p.splits);
   return launch_status();
@@ -300,7 +304,7 @@ int check_gated(int64_t rows, int64_t K, int64_t F, int act, int dtype) {
   if (dtype != GA_F32 && dtype != GA_BF16) return GA_EUNSUPPORTED;
   if (act != GA_GATE_SILU && act != GA_GATE_GELU && act != GA_GATE_RELU) return GA_EUNSUPPORTED;
   // 32-bit offsets inside a tile of 256 rows
-  if (K > (1 << 21) || F > (1 << 21)) return GA_EUNSUPPORTED;
+  if (K > (1 << 20) || F > (1 << 20)) return GA_EUNSUPPORTED;
   return GA_OK;
 }
 // bf16 operands that are not laid out anew are read 16 bytes at a time; fp32 ones by element

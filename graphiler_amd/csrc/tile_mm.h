@@ -26,6 +26,8 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef int intx8 __attribute__((ext_vector_type(8)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int kMmSegments = 12;          // pairs of operands whose products are added
@@ -39,10 +41,6 @@ struct TileMm {
   const uint8_t *sa, *sb0, *sb1;         // 8 bits: scales of the rows of A (rows, K / 128), of B (cols / 128, K / 128)
   int splits;                            // parts of the contraction, each its own fp32 result
 };
-
-__device__ __forceinline__ rsrc_t tile_rsrc(const char *base) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
-}
 
 // One operand's tile of a step: R rows of C by 128 bytes of k, WAVES wavefronts move it.
 template <bool ACROSS, int R, int WAVES>
@@ -59,34 +57,40 @@ struct Tile {
     else return 2 * (((r >> 1) & 1) | (((r >> 3) & 1) << 1));
   }
 
-  uint32_t off[kMoves];                  // from the step's base, or kOutside
-  int k[kMoves];                         // across k: the value of k of the step that a move's piece is of; by k: its piece
+  // Where a move's piece begins, from the step's base (or kOutside), and where on k: across, for every
+  // move, the value of k; by k, for even and odd moves (8 rows each), the piece of the row.
+  static constexpr int kKept = ACROSS ? kMoves : 2;
+  uint32_t off[kKept];
+  int k[kKept];
+  uint32_t ld8, range;                   // by k: bytes from a move to the next, of the rows there are
 
   // left: rows of C there are from the tile's first on
   __device__ __forceinline__ void init(int64_t ld, int64_t left) {
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = threadIdx.x / kWave;
+    ld8 = (uint32_t)(8 * ld);
+    range = ACROSS ? 0x7fffffffu : (uint32_t)(min(left, (int64_t)R) * ld);
 #pragma unroll
-    for (int i = 0; i < kMoves; ++i) {
+    for (int i = 0; i < kKept; ++i) {
       const int id = (wave * kMoves + i) * kWave + lane;
       const int r = id / kRowPieces, c = (id % kRowPieces) ^ turn(r);
       if constexpr (ACROSS) {
         off[i] = c * 8 < left ? (uint32_t)(r * ld + c * 16) : kOutside;
         k[i] = r;
       } else {
-        off[i] = r < left ? (uint32_t)(r * ld + c * 16) : kOutside;
+        off[i] = (uint32_t)((r - 8 * i) * ld + c * 16);
         k[i] = c;
       }
     }
   }
-  // `left`: values of k (across) or 16-byte pieces of k there are from this step on
-  __device__ __forceinline__ void load(const char *base, lds_char *to, int at, int left) const {
-    const rsrc_t r = tile_rsrc(base);
+  // Move i of a step.  `left`: values of k (across) or 16-byte pieces of k there are from this step on
+  __device__ __forceinline__ void move(const char *base, lds_char *to, int at, int left, int i) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-#pragma unroll
-    for (int i = 0; i < kMoves; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (at + (wave * kMoves + i) * 1024), 16,
-                                               k[i] < left ? off[i] : kOutside, 0, 0, 0);
+    const int kept = ACROSS ? i : i & 1;
+    const uint32_t o = ACROSS ? off[kept] : off[kept] + i * ld8;
+    const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)range, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (at + (wave * kMoves + i) * 1024), 16,
+                                             k[kept] < left ? o : kOutside, 0, 0, 0);
   }
 
   // Where a lane's operand of the tile's rows from r0 (16 T times a whole number) on begins: 16 rows of bf16,
@@ -161,6 +165,31 @@ __device__ __forceinline__ void landed() {
   asm volatile("" ::: "memory");
 }
 
+// Deals R LDS reads and L loads out between P matrix instructions.
+template <int P, int R, int L>
+__device__ __forceinline__ void weave() {
+  constexpr int kGroups = 4, kRead = 0x100, kLoad = 0x10, kMma = 0x8;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    __builtin_amdgcn_sched_group_barrier(kRead, (R + kGroups - 1) / kGroups, 0);
+    __builtin_amdgcn_sched_group_barrier(kLoad, (L + kGroups - 1) / kGroups, 0);
+    __builtin_amdgcn_sched_group_barrier(kMma, P / kGroups, 0);
+  }
+}
+
+// Of `tiles` tiles of results, as many (a divisor) as `room` bytes hold.
+constexpr int tiles_a_pass(int tiles, int bytes, int room) {
+  for (int n = tiles; n > 0; n /= 2)
+    if (n * bytes <= room) return n;
+  return 0;
+}
+// Where chunk c of row r of the results lies in its row of LDS: at c ^ turn, which spreads the rows of a write and the
+// chunks of a read over the banks.
+template <int CHUNKS>
+__device__ __forceinline__ int out_turn(int r) {
+  return CHUNKS == 4 ? (r >> 2) & 3 : CHUNKS == 8 ? (r >> 1) & 7 : r & 15;
+}
+
 // The operands and results of one matrix instruction: 16 x 16 x 32 of bf16, 32 x 32 x 64 of 8 bits.
 template <bool FP8> struct Mma;
 template <> struct Mma<false> {
@@ -227,13 +256,26 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     b0_ptr = (const char *)p.b0[seg] + b_at + in_seg * b_step;
     if constexpr (PAIR) b1_ptr = (const char *)p.b1[seg] + b_at + in_seg * b_step;
   };
-  auto fetch = [&](lds_char *to) {
-    // what is left of k: values (across) and pieces of 16 bytes (by k, whose rows are whole pieces)
+  // What is left of k for the step to be fetched: values (across) and pieces of 16 bytes (by k, whose rows are
+  // whole pieces).
+  int a_left = 0, b_left = 0;
+  auto measure = [&]() {
     const int values = to_fetch > 0 ? (int)min((int64_t)kStepK, p.K - (int64_t)in_seg * kStepK) : 0;
     const int pieces = (values * kElem + 15) / 16;
-    ta.load(a_ptr, to, 0, A_ACROSS ? values : pieces);
-    tb.load(b0_ptr, to, TA::kBytes, B_ACROSS ? values : pieces);
-    if constexpr (PAIR) tb.load(b1_ptr, to, TA::kBytes + TB::kBytes, B_ACROSS ? values : pieces);
+    a_left = A_ACROSS ? values : pieces;
+    b_left = B_ACROSS ? values : pieces;
+  };
+  // Half of the step's moves at a time: all in a row would hold up the products behind them.
+  auto fetch = [&](lds_char *to, int part) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if (i % 2 != part) continue;
+      if (i < TA::kMoves) ta.move(a_ptr, to, 0, a_left, i);
+      else if (i < TA::kMoves + TB::kMoves) tb.move(b0_ptr, to, TA::kBytes, b_left, i - TA::kMoves);
+      else tb.move(b1_ptr, to, TA::kBytes + TB::kBytes, b_left, i - TA::kMoves - TB::kMoves);
+    }
+  };
+  auto advance = [&]() {
     --to_fetch;
     a_ptr += a_step;
     b0_ptr += b_step;
@@ -242,6 +284,7 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
       in_seg = 0;
       if (++seg < p.segments) enter();
     }
+    measure();
   };
   const int lane_a = TA::template lane_at<FP8>(wm * TM * kT), lane_b = TB::template lane_at<FP8>(wn * TC * kT);
   auto read_a = [&](const lds_char *t, int i, int half) {
@@ -259,11 +302,19 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     static_assert(TC * kT <= 128 && 128 % (TC * kT) == 0 && BC % (TC * kT) == 0, "columns of one scale");
     static_assert((TM == 2 || TM == 4) && WN * kPair <= 8, "scales of a step are a word and two bytes");
     const int kb = (int)(p.K / 128);
-    for (int r = threadIdx.x; r < BM; r += kWaves * kWave) {
-      if (row0 + r >= p.rows) break;
-      const uint8_t *src = p.sa + (row0 + r) * kb;
-      const int at = r / (TM * kT) * (TM * kT) + r % kT * TM + r / kT % TM;
-      for (int b = 0; b < kb; ++b) row_scales[b * BM + at] = src[b];
+    for (int id = threadIdx.x; id < (kb + 3) / 4 * BM; id += kWaves * kWave) {
+      const int r = id % BM, b = id / BM * 4;
+      if (row0 + r >= p.rows) continue;
+      const uint8_t *src = p.sa + (row0 + r) * kb + b;
+      uint8_t *to = row_scales + b * BM + r / (TM * kT) * (TM * kT) + r % kT * TM + r / kT % TM;
+      if (b + 4 <= kb) {
+        struct __attribute__((packed, aligned(1))) Four { uint32_t w; };
+        const uint32_t w = reinterpret_cast<const Four *>(src)->w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i * BM] = (uint8_t)(w >> (8 * i));
+      } else {
+        for (int i = 0; b + i < kb; ++i) to[i * BM] = src[i];
+      }
     }
     for (int id = threadIdx.x; id < kb * 8; id += kWaves * kWave) {
       const int b = id / 8, w = id % 8 % WN, second = id % 8 / WN;
@@ -274,8 +325,11 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
 
   lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1;
   if (first < last) enter();
-  fetch(L0);
-  fetch(L1);
+  measure();
+  fetch(L0, 0);
+  fetch(L0, 1);
+  advance();
+  fetch(L1, 0);
 
   typename M::operand a[TM], b[2][TN];
   int scale_a = 0, scale_b[2] = {0, 0};
@@ -333,30 +387,40 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     for (int i = kHalf; i < TM; ++i) products(i, half);
     hold(kHalf);
   };
-  auto step = [&](lds_char *here, const lds_char *next) {
+  // A phase's LDS reads and moves are dealt out between its products.
+  constexpr int kReadA = FP8 || A_ACROSS ? 2 : 1, kReadB = FP8 || B_ACROSS ? 2 : 1;
+  constexpr int kReadsSecond = kHalf * kReadA, kReadsFirst = kHalf * kReadA + TN * kReadB, kProducts = kHalf * TN;
+  auto step = [&](lds_char *here, lds_char *next) {
     second_operands(here, 0);
+    fetch(next, 1);
     first_products(0);
+    weave<kProducts, kReadsSecond, kLoads / 2>();
     __builtin_amdgcn_sched_barrier(0);   // a phase's reads take registers that the phase before frees
+    advance();
     first_operands(here, 1);
     second_products(0);
+    weave<kProducts, kReadsFirst, 0>();
     __builtin_amdgcn_sched_barrier(0);
     second_operands(here, 1);
     first_products(1);
+    weave<kProducts, kReadsSecond, 0>();
     landed<0>();
-    fetch(here);
     int sa = scale_a, sb[2] = {scale_b[0], scale_b[1]};
     if constexpr (FP8) {
       block = min(block + 1, blocks - 1);
       read_scales(block, sa, sb);
     }
     first_operands(next, 0);
+    fetch(here, 0);
     second_products(1);
+    weave<kProducts, kReadsFirst + (FP8 ? 1 + kPair : 0), (kLoads + 1) / 2>();
+    __builtin_amdgcn_sched_barrier(0);
     scale_a = sa;
     scale_b[0] = sb[0];
     scale_b[1] = sb[1];
   };
 
-  landed<kLoads>();
+  landed<(kLoads + 1) / 2>();
   read_scales(0, scale_a, scale_b);
   first_operands(L0, 0);
   int left = last - first;
@@ -365,26 +429,49 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     step(L1, L0);
   }
   if (left > 0) step(L0, L1);
-  wait_loads<0>();                       // nothing may arrive in LDS that another workgroup has by then
 
+  // The results go through LDS, a part of it for each wavefront, so that whole pieces of rows leave
+  // with 16 bytes a lane: stored from where the products are, 16 rows would get 32 bytes each.
+  constexpr int kSize = Epi::kSize, kOut = Epi::kOut, kCols = TC * kT;
+  constexpr int kShare = 2 * kStage / kWaves, kRowBytes = kCols * kSize, kRowChunks = kRowBytes / 16;
+  constexpr int kPass = tiles_a_pass(TM, kT * kRowBytes * kOut, kShare), kRegion = kPass * kT * kRowBytes;
+  static_assert(kPass > 0 && kShare * (kWaves / 2) == kStage, "a wavefront's part holds a pass");
+  landed<0>();                           // every wavefront is done with the tiles
+  lds_char *const mine = (wave < kWaves / 2 ? L0 : L1) + wave % (kWaves / 2) * kShare;
+  const int64_t wave_row = row0 + wm * TM * kT, wave_col = col0 + wn * kCols;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int64_t row = row0 + (wm * TM + i) * kT + n;
-    if (row >= p.rows) continue;
+  for (int i0 = 0; i0 < TM; i0 += kPass) {
 #pragma unroll
-    for (int j = 0; j < TC; ++j)
+    for (int i = i0; i < i0 + kPass; ++i)
 #pragma unroll
-      for (int g = 0; g < M::kQuads; ++g) {
-        const int64_t col = col0 + (wn * TC + j) * kT + g * 8 + q * 4;
-        if (col >= p.cols) continue;
-        floatx4 u, v;
+      for (int j = 0; j < TC; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          u[r] = acc[i][j][4 * g + r];
-          v[r] = acc[i][PAIR ? j + TC : j][4 * g + r];
+        for (int g = 0; g < M::kQuads; ++g) {
+          floatx4 u, v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            u[r] = acc[i][j][4 * g + r];
+            v[r] = acc[i][PAIR ? j + TC : j][4 * g + r];
+          }
+          typename Epi::bits o[kOut];
+          const int col = j * kT + g * 8 + q * 4, row = (i - i0) * kT + n;
+          epi.make(p, wave_row + i * kT + n, wave_col + col, u, v, o);
+          const int at = row * kRowBytes + (col * kSize / 16 ^ out_turn<kRowChunks>(row)) * 16 + col * kSize % 16;
+#pragma unroll
+          for (int k = 0; k < kOut; ++k)
+            *reinterpret_cast<__attribute__((address_space(3))) typename Epi::bits *>(mine + k * kRegion + at) = o[k];
         }
-        epi(p, row, col, u, v);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < kOut; ++k)
+#pragma unroll
+      for (int it = 0; it < kRegion / 1024; ++it) {
+        const int id = it * kWave + lane, row = id / kRowChunks, c = (id % kRowChunks) ^ out_turn<kRowChunks>(row);
+        const uintx4 w = *reinterpret_cast<const __attribute__((address_space(3))) uintx4 *>(mine + k * kRegion + id * 16);
+        const int64_t r = wave_row + i0 * kT + row, col = wave_col + c * (16 / kSize);
+        if (r < p.rows && col < p.cols) epi.store(p, k, r, col, w);
       }
+    asm volatile("" ::: "memory");
   }
 }
 
@@ -393,34 +480,48 @@ __global__ __launch_bounds__(WM *WN *kWave, BLOCKS > 64 ? 1 : 2) void tile_mm_ke
   tile_mm<FP8, A_ACROSS, B_ACROSS, PAIR, WM, WN, TM, TN, BLOCKS>(p, epi);
 }
 
-// Four adjacent values of a row, of which `n` exist; `whole`: rows are 4-value aligned.
-__device__ __forceinline__ void store4(float *o, const floatx4 &v, int64_t n, bool whole) {
-  if (whole) {
-    *reinterpret_cast<floatx4 *>(o) = v;
-  } else {
-    for (int r = 0; r < 4; ++r)
-      if (r < n) o[r] = v[r];
+// Results as they are stored: `bits` holds four adjacent values, a 16-byte chunk kChunk of them.
+template <typename T> struct Stored;
+template <> struct Stored<float> {
+  typedef floatx4 bits;
+  static constexpr int kSize = 4, kChunk = 4;
+  static __device__ __forceinline__ bits pack(const floatx4 &v) { return v; }
+};
+template <> struct Stored<bf16_t> {
+  typedef uintx2 bits;
+  static constexpr int kSize = 2, kChunk = 8;
+  static __device__ __forceinline__ bits pack(const floatx4 &v) {
+    return uintx2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
   }
-}
-__device__ __forceinline__ void store4(bf16_t *o, const floatx4 &v, int64_t n, bool whole) {
-  if (whole) {
-    *reinterpret_cast<uint2 *>(o) = uint2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+};
+// A chunk of a row that may begin at any value and end inside the chunk.
+template <typename T>
+__device__ __forceinline__ void store_chunk(T *o, const uintx4 &w, int64_t n) {
+  constexpr int kChunk = Stored<T>::kChunk;
+  if (n >= kChunk) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { uintx4 w; };
+    reinterpret_cast<Any *>(o)->w = w;
   } else {
-    for (int r = 0; r < 4; ++r)
-      if (r < n) o[r] = (bf16_t)f32_to_bf16_bits(v[r]);
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < kChunk - 1; ++j) {
+      if (j >= n) break;
+      if constexpr (sizeof(T) == 4) o[j] = __uint_as_float(words[j]);
+      else o[j] = (T)(words[j / 2] >> (16 * (j & 1)));
+    }
   }
 }
 
 // What a gated block multiplies its second product by, and that function's slope.
 enum { kSilu = 0, kGelu = 1, kReluGate = 2 };
 __device__ __forceinline__ float gate_of(int act, float g) {
-  if (act == kSilu) return g / (1.0f + __expf(-g));
+  if (act == kSilu) return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g));    // one step of fp32 off
   if (act == kGelu) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
   return relu_keep_nan(g);
 }
 __device__ __forceinline__ float gate_slope(int act, float g) {
   if (act == kSilu) {
-    const float s = 1.0f / (1.0f + __expf(-g));
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
     return s * (1.0f + g * (1.0f - s));
   }
   if (act == kGelu) return 0.5f * (1.0f + erff(g * 0.70710678f)) + g * 0.39894228f * __expf(-0.5f * g * g);
@@ -428,38 +529,50 @@ __device__ __forceinline__ float gate_slope(int act, float g) {
 }
 
 template <typename T>
-struct StoreEpi {                        // C as it is
+struct StoreEpi : Stored<T> {            // C as it is
+  static constexpr int kOut = 1;
   T *out;
   int64_t ld;
-  bool whole;
-  __device__ __forceinline__ void operator()(const TileMm &p, int64_t row, int64_t col, const floatx4 &v,
-                                             const floatx4 &) const {
-    store4(out + row * ld + col, v, p.cols - col, whole);
+  StoreEpi(T *o, int64_t l) : out(o), ld(l) {}
+  __device__ __forceinline__ void make(const TileMm &, int64_t, int64_t, const floatx4 &u, const floatx4 &,
+                                       typename Stored<T>::bits (&o)[1]) const {
+    o[0] = Stored<T>::pack(u);
+  }
+  __device__ __forceinline__ void store(const TileMm &p, int, int64_t row, int64_t col, const uintx4 &w) const {
+    store_chunk(out + row * ld + col, w, p.cols - col);
   }
 };
 template <typename T>
-struct StorePairEpi {                    // both products of a pair
+struct StorePairEpi : Stored<T> {        // both products of a pair; of part z of the contraction `part` values further on
+  static constexpr int kOut = 2;
   T *out0, *out1;
-  int64_t ld;
-  bool whole;
-  __device__ __forceinline__ void operator()(const TileMm &p, int64_t row, int64_t col, const floatx4 &u,
-                                             const floatx4 &v) const {
-    store4(out0 + row * ld + col, u, p.cols - col, whole);
-    store4(out1 + row * ld + col, v, p.cols - col, whole);
+  int64_t ld, part;
+  StorePairEpi(T *o0, T *o1, int64_t l, int64_t n) : out0(o0), out1(o1), ld(l), part(n) {}
+  __device__ __forceinline__ void make(const TileMm &, int64_t, int64_t, const floatx4 &u, const floatx4 &v,
+                                       typename Stored<T>::bits (&o)[2]) const {
+    o[0] = Stored<T>::pack(u);
+    o[1] = Stored<T>::pack(v);
+  }
+  __device__ __forceinline__ void store(const TileMm &p, int k, int64_t row, int64_t col, const uintx4 &w) const {
+    store_chunk((k ? out1 : out0) + (int64_t)blockIdx.y * part + row * ld + col, w, p.cols - col);
   }
 };
 template <typename T>
-struct GateEpi {                         // act(first) * second
+struct GateEpi : Stored<T> {             // act(first) * second
+  static constexpr int kOut = 1;
   T *out;
   int64_t ld;
   int act;
-  bool whole;
-  __device__ __forceinline__ void operator()(const TileMm &p, int64_t row, int64_t col, const floatx4 &g,
-                                             const floatx4 &u) const {
+  GateEpi(T *o, int64_t l, int a) : out(o), ld(l), act(a) {}
+  __device__ __forceinline__ void make(const TileMm &, int64_t, int64_t, const floatx4 &g, const floatx4 &u,
+                                       typename Stored<T>::bits (&o)[1]) const {
     floatx4 h;
 #pragma unroll
     for (int r = 0; r < 4; ++r) h[r] = gate_of(act, g[r]) * u[r];
-    store4(out + row * ld + col, h, p.cols - col, whole);
+    o[0] = Stored<T>::pack(h);
+  }
+  __device__ __forceinline__ void store(const TileMm &p, int, int64_t row, int64_t col, const uintx4 &w) const {
+    store_chunk(out + row * ld + col, w, p.cols - col);
   }
 };
 
@@ -471,10 +584,13 @@ inline int64_t tiles_of(int64_t rows, int64_t cols, int bm, int bc) {
 // wavefronts, two such workgroups a compute unit, of which one multiplies while the other begins or
 // stores, or 256 x 256 by eight.
 enum { kTile128, kTile256 };
-constexpr int64_t kLargeTilesFrom = 192;
-inline int tile_for(const TileMm &p, bool fp8, bool pair) {
+inline int tile_for(const TileMm &p, bool pair) {
+  // what share of the workgroups that run at once (256 large ones, 512 small ones) has a tile, over all rounds;
+  // large tiles take 13 % less time where both fill theirs
   const int64_t large = tiles_of(p.rows, p.cols, 256, pair ? 128 : 256) * p.splits;
-  return large >= kLargeTilesFrom ? kTile256 : kTile128;
+  const int64_t small = tiles_of(p.rows, p.cols, 128, pair ? 64 : 128) * p.splits;
+  const int64_t large_slots = (large + 255) / 256 * 256, small_slots = (small + 511) / 512 * 512;
+  return 115 * large * small_slots >= 100 * small * large_slots ? kTile256 : kTile128;
 }
 
 template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int TM, int TN, int BLOCKS, typename Epi>
@@ -493,7 +609,7 @@ int tile_mm_launch(const TileMm &p, const Epi &epi, hipStream_t s) {
   constexpr int kHigh = FP8 ? 4 : 8, kLow = kHigh / 2, kWide = FP8 ? 2 : 4;    // tiles of a wavefront
   const int blocks = FP8 ? (int)((p.K + 127) / 128) : 0;
   if (blocks > kMostBlocks) return GA_EUNSUPPORTED;
-  const int tile = tile_for(p, FP8, PAIR);
+  const int tile = tile_for(p, PAIR);
   if (tile == kTile256 && blocks <= 64)
     return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, 64>(p, epi, s);
   if (blocks <= 32) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 32>(p, epi, s);

@@ -810,7 +810,7 @@ int ga_rms_norm_backward(const void *grad_y, const void *sum, const void *weight
  * (silu: g / (1 + exp(-g)); gelu with the error function; relu).  fp32 products are formed from bf16
  * pieces as in ga_linear_attn (less than 2^-22 of a product is left out; inputs that are not finite
  * give NaN, operands below 2^-110 lose bits).  bf16 tensors whose rows are whole 16-byte pieces have to
- * be 16-byte aligned.  GA_EUNSUPPORTED when K or F exceeds 2^21.
+ * be 16-byte aligned.  GA_EUNSUPPORTED when K or F exceeds 2^20.
  */
 enum ga_gate { GA_GATE_SILU = 0, GA_GATE_GELU = 1, GA_GATE_RELU = 2 };
 size_t ga_gated_linear_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype);
