@@ -11,6 +11,97 @@
 namespace ga {
 namespace {
 
+// Few rows: a workgroup takes 16 rows of w, its eight wavefronts take turns along K and add up what they have in
+// LDS; each reads 32 bytes a lane of w and of x for an instruction of 16 x 16 x 128, several ahead.  What counts is
+// how much of w is on its way.
+constexpr int kFewWaves = 8;
+template <int RT, bool PAIR, typename T>
+__global__ __launch_bounds__(kFewWaves *kWave) void few_fp8_kernel(
+    const uint8_t *__restrict__ x, const uint8_t *__restrict__ xs, const uint8_t *__restrict__ w0,
+    const uint8_t *__restrict__ s0, const uint8_t *__restrict__ w1, const uint8_t *__restrict__ s1, T *__restrict__ y,
+    int rows, int64_t K, int64_t M, int act) {
+  constexpr int kPair = PAIR ? 2 : 1, kDeep = RT > 2 ? 2 : 4;          // steps on their way
+  __shared__ float sums[kFewWaves][kPair][RT * 16][17];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n = lane & 15, q = lane >> 4;
+  const int64_t m0 = (int64_t)blockIdx.x * 16, kb = K / 128;
+  const int64_t m = min(m0 + n, M - 1);                                // rows behind the last: not stored
+  floatx4 acc[kPair][RT];
+#pragma unroll
+  for (int p = 0; p < kPair; ++p)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[p][t] = floatx4{0, 0, 0, 0};
+  auto take = [&](const uint8_t *base, int64_t row, int64_t b) {
+    const uintx4 lo = *reinterpret_cast<const uintx4 *>(base + row * K + b * 128 + q * 32);
+    const uintx4 hi = *reinterpret_cast<const uintx4 *>(base + row * K + b * 128 + q * 32 + 16);
+    return __builtin_bit_cast(intx8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  for (int64_t b0 = wave; b0 < kb; b0 += kFewWaves * kDeep) {
+    intx8 w[kDeep][kPair], v[kDeep][RT];
+    int ws[kDeep][kPair], vs[kDeep][RT];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const bool live = b0 + d * kFewWaves < kb;                       // behind the last: zeros, without a branch
+      const int64_t b = live ? b0 + d * kFewWaves : kb - 1;            // around what is read ahead
+#pragma unroll
+      for (int p = 0; p < kPair; ++p) {
+        w[d][p] = take(p ? w1 : w0, m, b);
+        ws[d][p] = (p ? s1 : s0)[m0 / 128 * kb + b];
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int64_t row = min(t * 16 + n, rows - 1);
+        v[d][t] = take(x, row, b);
+        if (!live) v[d][t] = intx8{0, 0, 0, 0, 0, 0, 0, 0};
+        vs[d][t] = xs[row * kb + b];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);                                 // all are asked for before the first is used
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+#pragma unroll
+      for (int p = 0; p < kPair; ++p)
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          acc[p][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[d][p], v[d][t], acc[p][t], 0, 0, 0, ws[d][p], 0,
+                                                                      vs[d][t]);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < kPair; ++p)
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sums[wave][p][t * 16 + n][4 * q + r] = acc[p][t][r];
+  __syncthreads();
+  for (int id = threadIdx.x; id < RT * 256; id += kFewWaves * kWave) {
+    const int row = id / 16, c = id % 16;
+    if (row >= rows || m0 + c >= M) continue;
+    float a[kPair];
+#pragma unroll
+    for (int p = 0; p < kPair; ++p) {
+      a[p] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kFewWaves; ++v) a[p] += sums[v][p][row][c];
+    }
+    f32_to_elem(PAIR ? gate_of(act, a[0]) * a[kPair - 1] : a[0], y[row * M + m0 + c]);
+  }
+}
+constexpr int64_t kFewRows = 64;
+template <bool PAIR, typename T>
+int few_fp8_launch(const TileMm &m, void *y, int act, hipStream_t s) {
+  const int64_t grid = (m.cols + 15) / 16;
+  if (grid > 0x7fffffff) return GA_EUNSUPPORTED;
+#define GA_FEW(R)                                                                                                \
+  hipLaunchKernelGGL((few_fp8_kernel<R, PAIR, T>), dim3((unsigned)grid), dim3(kFewWaves * kWave), 0, s,          \
+                     (const uint8_t *)m.a[0], m.sa, (const uint8_t *)m.b0[0], m.sb0, (const uint8_t *)m.b1[0],   \
+                     m.sb1, (T *)y, (int)m.rows, m.K, m.cols, act)
+  if (m.rows <= 16) GA_FEW(1);
+  else if (m.rows <= 32) GA_FEW(2);
+  else GA_FEW(4);
+#undef GA_FEW
+  return launch_status();
+}
+
 int check_fp8(int64_t rows, int64_t K, int64_t M, int dtype) {
   if (rows < 0 || K <= 0 || M <= 0 || K % 128 != 0) return GA_EINVAL;
   if (dtype != GA_F32 && dtype != GA_BF16) return GA_EUNSUPPORTED;
@@ -38,10 +129,12 @@ TileMm fp8_product(const void *x8, const void *xs, const void *w0, const void *s
 
 template <typename T>
 int linear8(const TileMm &m, void *y, hipStream_t s) {
+  if (m.rows <= kFewRows) return few_fp8_launch<false, T>(m, y, 0, s);
   return tile_mm_launch<true, false, false, false>(m, StoreEpi<T>((T *)y, m.cols), s);
 }
 template <typename T>
 int gated8(const TileMm &m, void *h, int act, hipStream_t s) {
+  if (m.rows <= kFewRows) return few_fp8_launch<true, T>(m, h, act, s);
   return tile_mm_launch<true, false, false, true>(m, GateEpi<T>((T *)h, m.cols, act), s);
 }
 

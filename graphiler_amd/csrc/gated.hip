@@ -13,7 +13,7 @@
 // product of two is six products of pieces (the three left out stay below 2^-22 of it; values
 // that are not finite give NaN, operands below 2^-110 lose bits).  The pieces are laid out once a
 // call, as are operands whose rows are not whole 16-byte pieces.
-#include "tile_mm.h"
+#include "gated_few.h"
 #include "vec8.h"
 
 namespace ga {
@@ -319,7 +319,7 @@ extern "C" {
 
 size_t ga_gated_linear_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype) {
   if (ga::check_gated(rows, K, F, GA_GATE_SILU, dtype) != GA_OK) return 0;
-  return ga::plan_of(rows, K, F, dtype, false).bytes;
+  return rows <= ga::kGatedFewRows ? 0 : ga::plan_of(rows, K, F, dtype, false).bytes;
 }
 
 int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h, int64_t rows, int64_t K, int64_t F,
@@ -331,6 +331,8 @@ int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h
   if (!operand_aligned(x, K, dtype) || !operand_aligned(w_gate, F, dtype) || !operand_aligned(w_up, F, dtype) ||
       !aligned(h, dtype == GA_F32 ? 4 : 2))
     return GA_EALIGN;
+  if (rows <= kGatedFewRows)
+    return gated_few_launch(x, w_gate, w_up, h, rows, K, F, activation, dtype, (hipStream_t)stream);
   const Plan p = plan_of(rows, K, F, dtype, false);
   if (p.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return GA_EWORKSPACE;
   hipStream_t s = (hipStream_t)stream;

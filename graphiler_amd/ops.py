@@ -1428,7 +1428,7 @@ def _check_rows(x, name: str) -> int:
 
 def _check_like(x, name: str, shape, like) -> None:
     _check_input(x, name)
-    if tuple(x.shape) != tuple(shape) or x.dtype != like.dtype or x.device != like.device:
+    if x.shape != shape or x.dtype != like.dtype or x.get_device() != like.get_device():
         raise RuntimeError(f"{name} must be {tuple(shape)}, of the dtype and on the device of the rows")
 
 
@@ -1449,14 +1449,20 @@ def _not_recorded(what: str) -> None:
                            f"under torch.no_grad() together with {what}_backward")
 
 
-def _launch(entry: str, device, *args) -> None:
-    """Call a C entry point on the current stream of ``device`` (its last argument)."""
-    index = device.index
+# The handle of a device's current stream: without building a Stream object where torch has a way.
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(entry: str, index: int, *args) -> None:
+    """Call a C entry point on the current stream of device ``index`` (its last argument)."""
     if index == torch.cuda.current_device():
-        capi.check(getattr(capi.load(), entry)(*args, torch.cuda.current_stream(index).cuda_stream), entry)
-        return
-    with torch.cuda.device(index):
-        capi.check(getattr(capi.load(), entry)(*args, torch.cuda.current_stream(index).cuda_stream), entry)
+        code = getattr(capi.load(), entry)(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            code = getattr(capi.load(), entry)(*args, _stream_of(index))
+    if code:
+        capi.check(code, entry)
 
 
 def _scratch(n_bytes: int, device) -> Optional[torch.Tensor]:
@@ -1502,7 +1508,7 @@ def _rms_norm(x, weight, residual, eps):
     dt, rows, cols = _norm_args(x, weight, residual, eps)
     y = torch.empty_like(x)
     total = None if residual is None else torch.empty_like(x)
-    _launch("ga_rms_norm", x.device, x.data_ptr(), _ptr(residual), weight.data_ptr(), y.data_ptr(),
+    _launch("ga_rms_norm", x.get_device(), x.data_ptr(), _ptr(residual), weight.data_ptr(), y.data_ptr(),
             _ptr(total), rows, cols, float(eps), dt)
     return y if residual is None else (y, total)
 
@@ -1528,7 +1534,7 @@ def rms_norm_backward(grad_y, total, weight, eps: float = 1e-6, grad_sum=None):
         _check_like(grad_sum, "grad_sum", total.shape, total)
     gx, gw = torch.empty_like(total), torch.empty_like(weight)
     ws = _scratch(capi.load().ga_rms_norm_backward_workspace_bytes(rows, cols), total.device)
-    _launch("ga_rms_norm_backward", total.device, grad_y.data_ptr(), total.data_ptr(),
+    _launch("ga_rms_norm_backward", total.get_device(), grad_y.data_ptr(), total.data_ptr(),
             weight.data_ptr(), _ptr(grad_sum), gx.data_ptr(), gw.data_ptr(), rows, cols, float(eps),
             dt, ws.data_ptr(), ws.numel())
     return gx, gw
@@ -1549,7 +1555,7 @@ def rms_norm_fp8(x, weight, residual=None, eps: float = 1e-6):
     dt, rows, cols = _norm_args(x, weight, residual, eps)
     y8, scales = _rows_8bit(rows, cols, x.device)
     total = None if residual is None else torch.empty_like(x)
-    _launch("ga_rms_norm_fp8", x.device, x.data_ptr(), _ptr(residual), weight.data_ptr(), y8.data_ptr(),
+    _launch("ga_rms_norm_fp8", x.get_device(), x.data_ptr(), _ptr(residual), weight.data_ptr(), y8.data_ptr(),
             scales.data_ptr(), _ptr(total), rows, cols, float(eps), dt)
     return (y8, scales) if residual is None else (y8, scales, total)
 
@@ -1562,7 +1568,7 @@ def quantize_fp8(x):
     if cols > RMS_NORM_MAX_COLS:
         raise RuntimeError(f"x must have at most {RMS_NORM_MAX_COLS} columns")
     x8, scales = _rows_8bit(rows, cols, x.device)
-    _launch("ga_quantize_fp8", x.device, x.data_ptr(), x8.data_ptr(), scales.data_ptr(), rows, cols, dt)
+    _launch("ga_quantize_fp8", x.get_device(), x.data_ptr(), x8.data_ptr(), scales.data_ptr(), rows, cols, dt)
     return x8, scales
 
 
@@ -1577,7 +1583,7 @@ def quantize_weight_fp8(weight):
     blocks = -(-k // FP8_BLOCK)
     w8 = torch.empty((m, blocks * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=weight.device)
     scales = torch.empty((-(-m // FP8_BLOCK), blocks), dtype=torch.float8_e8m0fnu, device=weight.device)
-    _launch("ga_quantize_weight_fp8", weight.device, weight.data_ptr(), w8.data_ptr(), scales.data_ptr(),
+    _launch("ga_quantize_weight_fp8", weight.get_device(), weight.data_ptr(), w8.data_ptr(), scales.data_ptr(),
             k, m, dt)
     return w8, scales
 
@@ -1587,7 +1593,7 @@ def _check_8bit(values, scales, name: str, device, rows_each: int, k=None) -> No
     _check_input(scales, name + "_scales")
     if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float8_e8m0fnu:
         raise RuntimeError(f"{name} must be float8_e4m3fn with float8_e8m0fnu scales")
-    if values.device != device or scales.device != device:
+    if values.get_device() != device or scales.get_device() != device:
         raise RuntimeError(f"{name} and its scales must be on the device of the rows")
     if values.dim() != 2 or values.shape[1] == 0 or values.shape[1] % FP8_BLOCK or \
             (k is not None and values.shape[1] != k):
@@ -1605,12 +1611,12 @@ def _out_8bit(x8, m: int, out_dtype):
 def linear_fp8(x8, x_scales, w8, w_scales, out_dtype=torch.bfloat16):
     """x @ weight for rows and a weight in 8 bits (:func:`quantize_fp8` or :func:`rms_norm_fp8`,
     :func:`quantize_weight_fp8`): (rows, M) of ``out_dtype``, accumulated in fp32."""
-    _check_8bit(x8, x_scales, "x8", x8.device, 1)
+    _check_8bit(x8, x_scales, "x8", x8.get_device(), 1)
     k = int(x8.shape[1])
-    _check_8bit(w8, w_scales, "w8", x8.device, FP8_BLOCK, k)
+    _check_8bit(w8, w_scales, "w8", x8.get_device(), FP8_BLOCK, k)
     y = _out_8bit(x8, int(w8.shape[0]), out_dtype)
     if y.numel():
-        _launch("ga_linear_fp8", x8.device, x8.data_ptr(), x_scales.data_ptr(), w8.data_ptr(),
+        _launch("ga_linear_fp8", x8.get_device(), x8.data_ptr(), x_scales.data_ptr(), w8.data_ptr(),
                 w_scales.data_ptr(), y.data_ptr(), int(x8.shape[0]), k, int(w8.shape[0]), _DTYPES[out_dtype])
     return y
 
@@ -1620,15 +1626,15 @@ def gated_linear_fp8(x8, x_scales, wg8, wg_scales, wu8, wu_scales, activation: s
     """:func:`gated_linear` for rows and weights in 8 bits: act(x @ w_gate) * (x @ w_up) from one
     kernel."""
     act = _gate(activation)
-    _check_8bit(x8, x_scales, "x8", x8.device, 1)
+    _check_8bit(x8, x_scales, "x8", x8.get_device(), 1)
     k = int(x8.shape[1])
-    _check_8bit(wg8, wg_scales, "wg8", x8.device, FP8_BLOCK, k)
-    _check_8bit(wu8, wu_scales, "wu8", x8.device, FP8_BLOCK, k)
+    _check_8bit(wg8, wg_scales, "wg8", x8.get_device(), FP8_BLOCK, k)
+    _check_8bit(wu8, wu_scales, "wu8", x8.get_device(), FP8_BLOCK, k)
     if wg8.shape != wu8.shape:
         raise RuntimeError("wg8 and wu8 must share a shape")
     h = _out_8bit(x8, int(wg8.shape[0]), out_dtype)
     if h.numel():
-        _launch("ga_gated_linear_fp8", x8.device, x8.data_ptr(), x_scales.data_ptr(), wg8.data_ptr(),
+        _launch("ga_gated_linear_fp8", x8.get_device(), x8.data_ptr(), x_scales.data_ptr(), wg8.data_ptr(),
                 wg_scales.data_ptr(), wu8.data_ptr(), wu_scales.data_ptr(), h.data_ptr(), int(x8.shape[0]), k,
                 int(wg8.shape[0]), act, _DTYPES[out_dtype])
     return h
@@ -1668,7 +1674,7 @@ def _gated_linear(x, w_gate, w_up, activation):
     h = torch.empty((rows, f), dtype=x.dtype, device=x.device)
     n = capi.load().ga_gated_linear_workspace_bytes(rows, k, f, dt)
     ws = _scratch(n, x.device)
-    _launch("ga_gated_linear", x.device, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(),
+    _launch("ga_gated_linear", x.get_device(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(),
             rows, k, f, act, dt, _ptr(ws), n)
     return h
 
@@ -1692,6 +1698,6 @@ def gated_linear_backward(grad_h, x, w_gate, w_up, activation: str = "silu"):
     gx, gg, gu = torch.empty_like(x), torch.empty_like(w_gate), torch.empty_like(w_up)
     n = capi.load().ga_gated_linear_backward_workspace_bytes(rows, k, f, dt)
     ws = _scratch(n, x.device)
-    _launch("ga_gated_linear_backward", x.device, grad_h.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+    _launch("ga_gated_linear_backward", x.get_device(), grad_h.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
             w_up.data_ptr(), gx.data_ptr(), gg.data_ptr(), gu.data_ptr(), rows, k, f, act, dt, _ptr(ws), n)
     return gx, gg, gu
