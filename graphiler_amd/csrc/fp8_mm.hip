@@ -112,7 +112,7 @@ int check_fp8(int64_t rows, int64_t K, int64_t M, int dtype) {
 TileMm fp8_product(const void *x8, const void *xs, const void *w0, const void *s0, const void *w1, const void *s1,
                    int64_t rows, int64_t K, int64_t M) {
   TileMm m{};
-  m.segments = 1;
+  m.terms = m.pieces = 1;
   m.a[0] = x8;
   m.b0[0] = w0;
   m.b1[0] = w1;
@@ -130,7 +130,7 @@ TileMm fp8_product(const void *x8, const void *xs, const void *w0, const void *s
 template <typename T>
 int linear8(const TileMm &m, void *y, hipStream_t s) {
   if (m.rows <= kFewRows) return few_fp8_launch<false, T>(m, y, 0, s);
-  return tile_mm_launch<true, false, false, false>(m, StoreEpi<T>((T *)y, m.cols), s);
+  return tile_mm_launch<true, false, false, false>(m, StoreEpi<T>((T *)y, m.cols, 0), s);
 }
 template <typename T>
 int gated8(const TileMm &m, void *h, int act, hipStream_t s) {

@@ -127,16 +127,16 @@ struct GradEpi : Stored<bf16_t> {
   }
 };
 
-// Sums of the parts of a contraction; a part is the first product's values and then the second's.
+// Sums of the parts of a contraction, `all` values each: n of the first result, then the second's.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void join_parts_kernel(const float *__restrict__ parts, T *__restrict__ out0,
-                                                            T *__restrict__ out1, int64_t n, int splits) {
-  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < 2 * n; i += (int64_t)gridDim.x * kBlock) {
-    const bool second = i >= n;
-    const float *src = parts + i;
+                                                            T *__restrict__ out1, int64_t n, int64_t all,
+                                                            int splits) {
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < all; i += (int64_t)gridDim.x * kBlock) {
     float s = 0.0f;
-    for (int k = 0; k < splits; ++k) s += src[2 * (int64_t)k * n];
-    f32_to_elem(s, second ? out1[i - n] : out0[i]);
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += parts[k * all + i];
+    f32_to_elem(s, i >= n ? out1[i - n] : out0[i]);
   }
 }
 template <typename T>
@@ -159,9 +159,16 @@ struct Plan {
   int pieces;                            // 1 of bf16, 3 of fp32
   int64_t x, wg, wu, dg, du;             // bytes from the workspace's start
   int64_t parts;
-  int splits;
+  int splits, x_splits;                  // parts of the sums of the weights' gradients and of x's
   size_t bytes;
 };
+// Into how many parts a contraction of `steps` steps is cut for `tiles` tiles: as many as give the
+// chip's 512 places a workgroup each, none of fewer than eight steps (a part writes and reads its results once more).
+int parts_of(int64_t tiles, int64_t steps) {
+  int64_t n = 512 / (tiles > 0 ? tiles : 1);
+  if (n > steps / 8) n = steps / 8;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
 Plan plan_of(int64_t rows, int64_t K, int64_t F, int dtype, bool grad) {
   Plan p;
   p.Kp = round8(K);
@@ -178,35 +185,21 @@ Plan plan_of(int64_t rows, int64_t K, int64_t F, int dtype, bool grad) {
   p.wg = own_w ? take(2 * p.pieces * K * p.Fp) : -1;
   p.wu = own_w ? take(2 * p.pieces * K * p.Fp) : -1;
   p.dg = p.du = p.parts = -1;
-  p.splits = 1;
+  p.splits = p.x_splits = 1;
   if (grad) {
     p.dg = take(2 * p.pieces * rows * p.Fp);
     p.du = take(2 * p.pieces * rows * p.Fp);
-    // the gradients of the weights sum over all rows: cut where their tiles do not fill the chip
-    const int64_t tiles = tiles_of(K, F, 128, 64), steps = (rows + 63) / 64 * (p.pieces == 3 ? 6 : 1);
-    if (tiles < 256) {
-      int64_t n = (512 + tiles - 1) / tiles;
-      if (n > steps / 4) n = steps / 4;
-      p.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-    }
-    if (p.splits > 1) p.parts = take((int64_t)p.splits * 2 * K * F * 4);
+    // Sums over all rows, and over both weights' columns, are cut where their tiles do not fill the chip.
+    const int six = p.pieces == 3 ? 6 : 1;
+    p.splits = parts_of(tiles_of(K, F, 128, 64), (rows + 63) / 64 * six);
+    p.x_splits = parts_of(tiles_of(rows, K, 128, 128), (F + 63) / 64 * 2 * six);
+    int64_t most = 0;
+    if (p.splits > 1) most = (int64_t)p.splits * 2 * K * F;
+    if (p.x_splits > 1 && p.x_splits * rows * K > most) most = p.x_splits * rows * K;
+    if (most) p.parts = take(4 * most);
   }
   p.bytes = (size_t)at;
   return p;
-}
-
-// The pairs of pieces whose products are added, small ones first.
-constexpr int kPairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-
-// The segments of C = A B of one or two pairs of operands of `pieces` planes each.
-void add_segments(TileMm &m, int pieces, const bf16_t *a, int64_t a_plane, const bf16_t *b0, const bf16_t *b1,
-                  int64_t b_plane) {
-  for (int i = pieces == 1 ? 5 : 0; i < 6; ++i) {
-    const int s = m.segments++;
-    m.a[s] = a + kPairs[i][0] * a_plane;
-    m.b0[s] = b0 + kPairs[i][1] * b_plane;
-    m.b1[s] = b1 ? b1 + kPairs[i][1] * b_plane : nullptr;
-  }
 }
 
 struct Operands { const bf16_t *x, *wg, *wu; };
@@ -244,7 +237,13 @@ TileMm both_products(const Plan &p, const Operands &o, int64_t rows, int64_t K, 
   m.cols = cols;
   m.K = K;
   m.splits = 1;
-  add_segments(m, p.pieces, o.x, rows * p.Kp, o.wg, o.wu, K * p.Fp);
+  m.terms = 1;
+  m.pieces = p.pieces;
+  m.a[0] = o.x;
+  m.b0[0] = o.wg;
+  m.b1[0] = o.wu;
+  m.a_plane = 2 * rows * p.Kp;
+  m.b_plane = 2 * K * p.Fp;
   return m;
 }
 
@@ -276,10 +275,24 @@ int backward(const void *gh, const void *x, const void *wg, const void *wu, void
     m.rows = rows;
     m.cols = K;
     m.K = p.Fp;
-    m.splits = 1;
-    add_segments(m, p.pieces, dg, d_plane, o.wg, nullptr, w_plane);
-    add_segments(m, p.pieces, du, d_plane, o.wu, nullptr, w_plane);
-    if (int rc = tile_mm_launch<false, false, false, false>(m, StoreEpi<T>((T *)gx, K), s)) return rc;
+    m.splits = p.x_splits;
+    m.terms = 2;
+    m.pieces = p.pieces;
+    m.a[0] = dg;
+    m.a[1] = du;
+    m.b0[0] = o.wg;
+    m.b0[1] = o.wu;
+    m.a_plane = 2 * d_plane;
+    m.b_plane = 2 * w_plane;
+    if (p.x_splits == 1) {
+      if (int rc = tile_mm_launch<false, false, false, false>(m, StoreEpi<T>((T *)gx, K, 0), s)) return rc;
+    } else {
+      float *parts = (float *)(ws + p.parts);
+      if (int rc = tile_mm_launch<false, false, false, false>(m, StoreEpi<float>(parts, K, rows * K), s)) return rc;
+      hipLaunchKernelGGL((join_parts_kernel<T>), dim3(stream_grid(rows * K)), dim3(kBlock), 0, s, parts, (T *)gx,
+                         (T *)nullptr, rows * K, rows * K, p.x_splits);
+      if (int rc = launch_status()) return rc;
+    }
   }
   TileMm m{};
   m.lda = 2 * p.Kp;
@@ -288,14 +301,20 @@ int backward(const void *gh, const void *x, const void *wg, const void *wu, void
   m.cols = F;
   m.K = rows;
   m.splits = p.splits;
-  add_segments(m, p.pieces, o.x, x_plane, dg, du, d_plane);
+  m.terms = 1;
+  m.pieces = p.pieces;
+  m.a[0] = o.x;
+  m.b0[0] = dg;
+  m.b1[0] = du;
+  m.a_plane = 2 * x_plane;
+  m.b_plane = 2 * d_plane;
   if (p.splits == 1)
     return tile_mm_launch<false, true, true, true>(m, StorePairEpi<T>((T *)gwg, (T *)gwu, F, 0), s);
   float *parts = (float *)(ws + p.parts);
   const StorePairEpi<float> e(parts, parts + K * F, F, 2 * K * F);
   if (int rc = tile_mm_launch<false, true, true, true>(m, e, s)) return rc;
   hipLaunchKernelGGL((join_parts_kernel<T>), dim3(stream_grid(2 * K * F)), dim3(kBlock), 0, s, parts, (T *)gwg,
-                     (T *)gwu, K * F, p.splits);
+                     (T *)gwu, K * F, 2 * K * F, p.splits);
   return launch_status();
 }
 

@@ -30,17 +30,24 @@ typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
-constexpr int kMmSegments = 12;          // pairs of operands whose products are added
 constexpr uint32_t kOutside = 0x80000000u;   // an offset that no descriptor below has in range
 
+// C = sum over `terms` pairs of operands.  fp32 operands lie as three planes of bf16 pieces, and a pair is six
+// segments, the products of two pieces each; of bf16 and 8 bits it is one.  The addresses of a segment are reckoned
+// from what fits the registers: a table of them would be fetched from the arguments at every segment.
 struct TileMm {
-  int segments;
-  const void *a[kMmSegments], *b0[kMmSegments], *b1[kMmSegments];   // b1: the second product of a pair
+  int terms, pieces;
+  const void *a[2], *b0[2], *b1[2];      // b1: the second product of a PAIR
+  int64_t a_plane, b_plane;              // bytes from piece to piece
   int64_t lda, ldb;                      // bytes between rows of an operand by k, between k across it
-  int64_t rows, cols, K;                 // of C (of each product of a pair) and of one segment
+  int64_t rows, cols, K;                 // of C (of each product of a PAIR) and of one segment
   const uint8_t *sa, *sb0, *sb1;         // 8 bits: scales of the rows of A (rows, K / 128), of B (cols / 128, K / 128)
   int splits;                            // parts of the contraction, each its own fp32 result
+  __host__ __device__ int segments() const { return terms * (pieces == 3 ? 6 : 1); }
 };
+// Pieces of segment s of a pair, small products first: (2, 0) (0, 2) (1, 1) (1, 0) (0, 1) (0, 0).
+__device__ __forceinline__ int piece_a(int s) { return 0x052 >> (2 * s) & 3; }
+__device__ __forceinline__ int piece_b(int s) { return 0x118 >> (2 * s) & 3; }
 
 // One operand's tile of a step: R rows of C by 128 bytes of k, WAVES wavefronts move it.
 template <bool ACROSS, int R, int WAVES>
@@ -236,7 +243,7 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   const int64_t a_step = A_ACROSS ? kStepK * p.lda : 128, b_step = B_ACROSS ? kStepK * p.ldb : 128;
   const int64_t a_at = A_ACROSS ? row0 * kElem : row0 * p.lda, b_at = B_ACROSS ? col0 * kElem : col0 * p.ldb;
   const int per_segment = (int)((p.K + kStepK - 1) / kStepK);
-  const int all = per_segment * p.segments, share = (all + p.splits - 1) / p.splits;
+  const int segments = p.segments(), all = per_segment * segments, share = (all + p.splits - 1) / p.splits;
   const int first = (int)blockIdx.y * share, last = min(all, first + share);
 
   typename M::result acc[TM][TN];
@@ -252,9 +259,12 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   int seg = first / per_segment, in_seg = first - seg * per_segment;
   const char *a_ptr = nullptr, *b0_ptr = nullptr, *b1_ptr = nullptr;
   auto enter = [&]() {
-    a_ptr = (const char *)p.a[seg] + a_at + in_seg * a_step;
-    b0_ptr = (const char *)p.b0[seg] + b_at + in_seg * b_step;
-    if constexpr (PAIR) b1_ptr = (const char *)p.b1[seg] + b_at + in_seg * b_step;
+    const int term = p.pieces == 3 ? seg / 6 : seg, s = p.pieces == 3 ? seg % 6 : 5;
+    const int64_t a_off = piece_a(s) * p.a_plane + a_at + in_seg * a_step;
+    const int64_t b_off = piece_b(s) * p.b_plane + b_at + in_seg * b_step;
+    a_ptr = (const char *)(term ? p.a[1] : p.a[0]) + a_off;
+    b0_ptr = (const char *)(term ? p.b0[1] : p.b0[0]) + b_off;
+    if constexpr (PAIR) b1_ptr = (const char *)p.b1[0] + b_off;
   };
   // What is left of k for the step to be fetched: values (across) and pieces of 16 bytes (by k, whose rows are
   // whole pieces).
@@ -282,7 +292,7 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     b1_ptr += b_step;
     if (++in_seg == per_segment) {
       in_seg = 0;
-      if (++seg < p.segments) enter();
+      if (++seg < segments) enter();
     }
     measure();
   };
@@ -514,9 +524,26 @@ __device__ __forceinline__ void store_chunk(T *o, const uintx4 &w, int64_t n) {
 
 // What a gated block multiplies its second product by, and that function's slope.
 enum { kSilu = 0, kGelu = 1, kReluGate = 2 };
+// The normal distribution's integral up to g and its density, without a branch: erfc(x) = exp(-x^2) P(1 / (1 + p x)) for
+// x >= 0, formula 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions (off by at most 1.5e-7);
+// exp(-x^2) with x = |g| / sqrt(2) is the density's too.
+__device__ __forceinline__ void normal(float g, float &integral, float &density) {
+  const float e = __expf(-0.5f * g * g), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(g), 1.0f));
+  float q = fmaf(1.061405429f, t, -1.453152027f);
+  q = fmaf(q, t, 1.421413741f);
+  q = fmaf(q, t, -0.284496736f);
+  q = fmaf(q, t, 0.254829592f);
+  const float tail = 0.5f * q * t * e;
+  integral = g > 0.0f ? 1.0f - tail : tail;      // NaN: e is
+  density = 0.39894228f * e;
+}
 __device__ __forceinline__ float gate_of(int act, float g) {
   if (act == kSilu) return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g));    // one step of fp32 off
-  if (act == kGelu) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
+  if (act == kGelu) {
+    float integral, density;
+    normal(g, integral, density);
+    return integral > 0.0f || g != g ? g * integral : 0.0f;    // -inf: 0
+  }
   return relu_keep_nan(g);
 }
 __device__ __forceinline__ float gate_slope(int act, float g) {
@@ -524,26 +551,30 @@ __device__ __forceinline__ float gate_slope(int act, float g) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
     return s * (1.0f + g * (1.0f - s));
   }
-  if (act == kGelu) return 0.5f * (1.0f + erff(g * 0.70710678f)) + g * 0.39894228f * __expf(-0.5f * g * g);
+  if (act == kGelu) {
+    float integral, density;
+    normal(g, integral, density);
+    return density > 0.0f || g != g ? fmaf(g, density, integral) : integral;
+  }
   return g > 0.0f ? 1.0f : (g != g ? g : 0.0f);
 }
 
 template <typename T>
-struct StoreEpi : Stored<T> {            // C as it is
+struct StoreEpi : Stored<T> {            // C as it is; of part z of the contraction `part` values further on
   static constexpr int kOut = 1;
   T *out;
-  int64_t ld;
-  StoreEpi(T *o, int64_t l) : out(o), ld(l) {}
+  int64_t ld, part;
+  StoreEpi(T *o, int64_t l, int64_t n) : out(o), ld(l), part(n) {}
   __device__ __forceinline__ void make(const TileMm &, int64_t, int64_t, const floatx4 &u, const floatx4 &,
                                        typename Stored<T>::bits (&o)[1]) const {
     o[0] = Stored<T>::pack(u);
   }
   __device__ __forceinline__ void store(const TileMm &p, int, int64_t row, int64_t col, const uintx4 &w) const {
-    store_chunk(out + row * ld + col, w, p.cols - col);
+    store_chunk(out + (int64_t)blockIdx.y * part + row * ld + col, w, p.cols - col);
   }
 };
 template <typename T>
-struct StorePairEpi : Stored<T> {        // both products of a pair; of part z of the contraction `part` values further on
+struct StorePairEpi : Stored<T> {        // both products of a PAIR, likewise
   static constexpr int kOut = 2;
   T *out0, *out1;
   int64_t ld, part;
@@ -580,15 +611,17 @@ inline int64_t tiles_of(int64_t rows, int64_t cols, int bm, int bc) {
   return ((rows + bm - 1) / bm) * ((cols + bc - 1) / bc);
 }
 
-// The tiles a product may be cut into, rows by rows of B (of a PAIR: of both): 128 x 128 by four
-// wavefronts, two such workgroups a compute unit, of which one multiplies while the other begins or
-// stores, or 256 x 256 by eight.
-enum { kTile128, kTile256 };
+// The tiles a product may be cut into, rows by rows of B (of a PAIR: of both): 256 x 256 by eight
+// wavefronts, 128 x 128 by four, two such workgroups a compute unit, of which one multiplies while the other
+// begins or stores, 64 x 128 for grids that would leave compute units without one.
+enum { kTile128, kTile256, kTile64 };
 inline int tile_for(const TileMm &p, bool pair) {
-  // what share of the workgroups that run at once (256 large ones, 512 small ones) has a tile, over all rounds;
-  // large tiles take 13 % less time where both fill theirs
   const int64_t large = tiles_of(p.rows, p.cols, 256, pair ? 128 : 256) * p.splits;
   const int64_t small = tiles_of(p.rows, p.cols, 128, pair ? 64 : 128) * p.splits;
+  if (small <= 256) return kTile64;
+  if (small <= 512) return kTile128;
+  // what share of the workgroups that run at once (256 large ones, 512 small ones) has a tile, over all rounds;
+  // large tiles take 13 % less time where both fill theirs
   const int64_t large_slots = (large + 255) / 256 * 256, small_slots = (small + 511) / 512 * 512;
   return 115 * large * small_slots >= 100 * small * large_slots ? kTile256 : kTile128;
 }
@@ -612,6 +645,11 @@ int tile_mm_launch(const TileMm &p, const Epi &epi, hipStream_t s) {
   const int tile = tile_for(p, PAIR);
   if (tile == kTile256 && blocks <= 64)
     return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, 64>(p, epi, s);
+  if (tile == kTile64 && blocks <= 32) {
+    if constexpr (!FP8) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, 2, 4, 32>(p, epi, s);
+    else if constexpr (PAIR) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 1, 2, 2, 2, 32>(p, epi, s);
+    else return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 1, 4, 2, 1, 32>(p, epi, s);
+  }
   if (blocks <= 32) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 32>(p, epi, s);
   if constexpr (FP8) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, kMostBlocks>(p, epi, s);
   return GA_EUNSUPPORTED;
