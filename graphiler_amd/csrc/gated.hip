@@ -65,7 +65,7 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 }
 
 // dg and du of a tile, as operands of the products after: bf16 rows of `ld` values, of fp32 three planes of pieces.
-template <typename T>
+template <typename T, int ACT = -1>
 struct GradEpi : Stored<bf16_t> {
   static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1, kOut = 2 * kPieces;
   const T *gh;
@@ -74,6 +74,14 @@ struct GradEpi : Stored<bf16_t> {
   int64_t ld, plane;
   int act;
   bool whole;                            // rows of gh are whole groups of four
+  template <int A> __device__ __forceinline__ GradEpi<T, A> as() const {
+    return GradEpi<T, A>{{}, gh, gh_cols, dg, du, ld, plane, A, whole};
+  }
+  template <typename F> __device__ __forceinline__ void visit(F f) const {
+    if (act == kSilu) f(as<kSilu>());
+    else if (act == kGelu) f(as<kGelu>());
+    else f(as<kReluGate>());
+  }
   __device__ __forceinline__ void make(const TileMm &p, int64_t row, int64_t col, const floatx4 &g, const floatx4 &u,
                                        uintx2 (&o)[kOut]) const {
     // no branch around a load, so that many are on their way: what is not there is out of range, 0
@@ -102,8 +110,8 @@ struct GradEpi : Stored<bf16_t> {
     floatx4 a, b;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      a[r] = t[r] * u[r] * gate_slope(act, g[r]);
-      b[r] = t[r] * gate_of(act, g[r]);
+      a[r] = t[r] * u[r] * gate_slope(ACT, g[r]);
+      b[r] = t[r] * gate_of(ACT, g[r]);
     }
     if constexpr (kPieces == 1) {
       o[0] = pack(a);
@@ -121,9 +129,9 @@ struct GradEpi : Stored<bf16_t> {
     o1 = uintx2{p[1][0] | (p[1][1] << 16), p[1][2] | (p[1][3] << 16)};
     o2 = uintx2{p[2][0] | (p[2][1] << 16), p[2][2] | (p[2][3] << 16)};
   }
-  __device__ __forceinline__ void store(const TileMm &p, int k, int64_t row, int64_t col, const uintx4 &w) const {
+  __device__ __forceinline__ void store(const TileMm &, int k, int64_t row, int64_t col, const uintx4 &w, int64_t n) const {
     bf16_t *to = (k < kPieces ? dg : du) + k % kPieces * plane;
-    store_chunk(to + row * ld + col, w, p.cols - col);
+    store_chunk(to + row * ld + col, w, n);
   }
 };
 

@@ -64,11 +64,11 @@ struct Tile {
     else return 2 * (((r >> 1) & 1) | (((r >> 3) & 1) << 1));
   }
 
-  // Where a move's piece begins, from the step's base (or kOutside), and where on k: across, for every
-  // move, the value of k; by k, for even and odd moves (8 rows each), the piece of the row.
-  static constexpr int kKept = ACROSS ? kMoves : 2;
+  // Where a move's piece begins, from the step's base (or kOutside), and where on k: across, the value of k of the
+  // first move; by k, for even and odd moves (8 rows each), the piece of the row.
+  static constexpr int kKept = ACROSS ? kMoves : 2, kRowsMove = kWave / kRowPieces;
   uint32_t off[kKept];
-  int k[kKept];
+  int k[ACROSS ? 1 : 2];
   uint32_t ld8, range;                   // by k: bytes from a move to the next, of the rows there are
 
   // left: rows of C there are from the tile's first on
@@ -83,7 +83,7 @@ struct Tile {
       const int r = id / kRowPieces, c = (id % kRowPieces) ^ turn(r);
       if constexpr (ACROSS) {
         off[i] = c * 8 < left ? (uint32_t)(r * ld + c * 16) : kOutside;
-        k[i] = r;
+        if (i == 0) k[0] = r;
       } else {
         off[i] = (uint32_t)((r - 8 * i) * ld + c * 16);
         k[i] = c;
@@ -97,7 +97,7 @@ struct Tile {
     const uint32_t o = ACROSS ? off[kept] : off[kept] + i * ld8;
     const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)range, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (at + (wave * kMoves + i) * 1024), 16,
-                                             k[kept] < left ? o : kOutside, 0, 0, 0);
+                                             (ACROSS ? k[0] < left - i * kRowsMove : k[kept] < left) ? o : kOutside, 0, 0, 0);
   }
 
   // Where a lane's operand of the tile's rows from r0 (16 T times a whole number) on begins: 16 rows of bf16,
@@ -234,7 +234,7 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   const int64_t row0 = (int64_t)tr * BM, col0 = (int64_t)tc * BC;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / WN, wn = wave % WN;
-  const int lane = threadIdx.x & (kWave - 1), n = lane & (kT - 1), q = lane / kT;
+  const int n = threadIdx.x & (kT - 1);
 
   TA ta;
   TB tb;
@@ -449,40 +449,58 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   landed<0>();                           // every wavefront is done with the tiles
   lds_char *const mine = (wave < kWaves / 2 ? L0 : L1) + wave % (kWaves / 2) * kShare;
   const int64_t wave_row = row0 + wm * TM * kT, wave_col = col0 + wn * kCols;
+  const bool inside = wave_row + TM * kT <= p.rows && wave_col + kCols <= p.cols;
+  epi.visit([&](const auto &e) {
+    // hidden here, so that addresses are reckoned where they are used and not for all forms at once before the choice
+    int lane = threadIdx.x & (kWave - 1);
+    asm volatile("" : "+v"(lane));
+    const int n = lane & (kT - 1), q = lane / kT;
 #pragma unroll
-  for (int i0 = 0; i0 < TM; i0 += kPass) {
+    for (int i0 = 0; i0 < TM; i0 += kPass) {
 #pragma unroll
-    for (int i = i0; i < i0 + kPass; ++i)
+      for (int i = i0; i < i0 + kPass; ++i)
 #pragma unroll
-      for (int j = 0; j < TC; ++j)
+        for (int j = 0; j < TC; ++j)
 #pragma unroll
-        for (int g = 0; g < M::kQuads; ++g) {
-          floatx4 u, v;
+          for (int g = 0; g < M::kQuads; ++g) {
+            floatx4 u, v;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            u[r] = acc[i][j][4 * g + r];
-            v[r] = acc[i][PAIR ? j + TC : j][4 * g + r];
+            for (int r = 0; r < 4; ++r) {
+              u[r] = acc[i][j][4 * g + r];
+              v[r] = acc[i][PAIR ? j + TC : j][4 * g + r];
+            }
+            typename Epi::bits o[kOut];
+            const int col = j * kT + g * 8 + q * 4, row = (i - i0) * kT + n;
+            e.make(p, wave_row + i * kT + n, wave_col + col, u, v, o);
+            const int at = row * kRowBytes + (col * kSize / 16 ^ out_turn<kRowChunks>(row)) * 16 + col * kSize % 16;
+#pragma unroll
+            for (int k = 0; k < kOut; ++k)
+              *reinterpret_cast<__attribute__((address_space(3))) typename Epi::bits *>(mine + k * kRegion + at) = o[k];
           }
-          typename Epi::bits o[kOut];
-          const int col = j * kT + g * 8 + q * 4, row = (i - i0) * kT + n;
-          epi.make(p, wave_row + i * kT + n, wave_col + col, u, v, o);
-          const int at = row * kRowBytes + (col * kSize / 16 ^ out_turn<kRowChunks>(row)) * 16 + col * kSize % 16;
+      asm volatile("" ::: "memory");
 #pragma unroll
-          for (int k = 0; k < kOut; ++k)
-            *reinterpret_cast<__attribute__((address_space(3))) typename Epi::bits *>(mine + k * kRegion + at) = o[k];
+      for (int k = 0; k < kOut; ++k) {
+        constexpr int kBatch = kRegion / 1024 < 4 ? kRegion / 1024 : 4;      // chunks read before the first is stored
+#pragma unroll
+        for (int i1 = 0; i1 < kRegion / 1024; i1 += kBatch) {
+          uintx4 w[kBatch];
+#pragma unroll
+          for (int it = 0; it < kBatch; ++it)
+            w[it] = *reinterpret_cast<const __attribute__((address_space(3))) uintx4 *>(
+                mine + k * kRegion + ((i1 + it) * kWave + lane) * 16);
+#pragma unroll
+          for (int it = 0; it < kBatch; ++it) {
+            const int id = (i1 + it) * kWave + lane, row = id / kRowChunks;
+            const int c = (id % kRowChunks) ^ out_turn<kRowChunks>(row);
+            const int64_t r = wave_row + i0 * kT + row, col = wave_col + c * (16 / kSize);
+            if (inside) e.store(p, k, r, col, w[it], 16 / kSize);
+            else if (r < p.rows && col < p.cols) e.store(p, k, r, col, w[it], p.cols - col);
+          }
         }
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int k = 0; k < kOut; ++k)
-#pragma unroll
-      for (int it = 0; it < kRegion / 1024; ++it) {
-        const int id = it * kWave + lane, row = id / kRowChunks, c = (id % kRowChunks) ^ out_turn<kRowChunks>(row);
-        const uintx4 w = *reinterpret_cast<const __attribute__((address_space(3))) uintx4 *>(mine + k * kRegion + id * 16);
-        const int64_t r = wave_row + i0 * kT + row, col = wave_col + c * (16 / kSize);
-        if (r < p.rows && col < p.cols) epi.store(p, k, r, col, w);
       }
-    asm volatile("" ::: "memory");
-  }
+      asm volatile("" ::: "memory");
+    }
+  });
 }
 
 template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int TM, int TN, int BLOCKS, typename Epi>
@@ -559,18 +577,22 @@ __device__ __forceinline__ float gate_slope(int act, float g) {
   return g > 0.0f ? 1.0f : (g != g ? g : 0.0f);
 }
 
+// What becomes of a tile's results: make() forms what is stored of four adjacent columns, store() takes n values of a
+// row in a 16-byte chunk, visit() passes on a form of itself whose choices are made: a branch between the values
+// would have each wait for the one before.
 template <typename T>
 struct StoreEpi : Stored<T> {            // C as it is; of part z of the contraction `part` values further on
   static constexpr int kOut = 1;
   T *out;
   int64_t ld, part;
   StoreEpi(T *o, int64_t l, int64_t n) : out(o), ld(l), part(n) {}
+  template <typename F> __device__ __forceinline__ void visit(F f) const { f(*this); }
   __device__ __forceinline__ void make(const TileMm &, int64_t, int64_t, const floatx4 &u, const floatx4 &,
                                        typename Stored<T>::bits (&o)[1]) const {
     o[0] = Stored<T>::pack(u);
   }
-  __device__ __forceinline__ void store(const TileMm &p, int, int64_t row, int64_t col, const uintx4 &w) const {
-    store_chunk(out + (int64_t)blockIdx.y * part + row * ld + col, w, p.cols - col);
+  __device__ __forceinline__ void store(const TileMm &, int, int64_t row, int64_t col, const uintx4 &w, int64_t n) const {
+    store_chunk(out + (int64_t)blockIdx.y * part + row * ld + col, w, n);
   }
 };
 template <typename T>
@@ -579,31 +601,37 @@ struct StorePairEpi : Stored<T> {        // both products of a PAIR, likewise
   T *out0, *out1;
   int64_t ld, part;
   StorePairEpi(T *o0, T *o1, int64_t l, int64_t n) : out0(o0), out1(o1), ld(l), part(n) {}
+  template <typename F> __device__ __forceinline__ void visit(F f) const { f(*this); }
   __device__ __forceinline__ void make(const TileMm &, int64_t, int64_t, const floatx4 &u, const floatx4 &v,
                                        typename Stored<T>::bits (&o)[2]) const {
     o[0] = Stored<T>::pack(u);
     o[1] = Stored<T>::pack(v);
   }
-  __device__ __forceinline__ void store(const TileMm &p, int k, int64_t row, int64_t col, const uintx4 &w) const {
-    store_chunk((k ? out1 : out0) + (int64_t)blockIdx.y * part + row * ld + col, w, p.cols - col);
+  __device__ __forceinline__ void store(const TileMm &, int k, int64_t row, int64_t col, const uintx4 &w, int64_t n) const {
+    store_chunk((k ? out1 : out0) + (int64_t)blockIdx.y * part + row * ld + col, w, n);
   }
 };
-template <typename T>
+template <typename T, int ACT = -1>
 struct GateEpi : Stored<T> {             // act(first) * second
   static constexpr int kOut = 1;
   T *out;
   int64_t ld;
   int act;
-  GateEpi(T *o, int64_t l, int a) : out(o), ld(l), act(a) {}
+  __host__ __device__ GateEpi(T *o, int64_t l, int a) : out(o), ld(l), act(a) {}
+  template <typename F> __device__ __forceinline__ void visit(F f) const {
+    if (act == kSilu) f(GateEpi<T, kSilu>(out, ld, act));
+    else if (act == kGelu) f(GateEpi<T, kGelu>(out, ld, act));
+    else f(GateEpi<T, kReluGate>(out, ld, act));
+  }
   __device__ __forceinline__ void make(const TileMm &, int64_t, int64_t, const floatx4 &g, const floatx4 &u,
                                        typename Stored<T>::bits (&o)[1]) const {
     floatx4 h;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) h[r] = gate_of(act, g[r]) * u[r];
+    for (int r = 0; r < 4; ++r) h[r] = gate_of(ACT, g[r]) * u[r];
     o[0] = Stored<T>::pack(h);
   }
-  __device__ __forceinline__ void store(const TileMm &p, int, int64_t row, int64_t col, const uintx4 &w) const {
-    store_chunk(out + row * ld + col, w, p.cols - col);
+  __device__ __forceinline__ void store(const TileMm &, int, int64_t row, int64_t col, const uintx4 &w, int64_t n) const {
+    store_chunk(out + row * ld + col, w, n);
   }
 };
 

@@ -241,3 +241,39 @@ def hgt_layer(g: DGLGraph, h, k_weight, q_weight, v_weight, a_weight,
     alpha = ops.BroadcastNodeType(torch.sigmoid(skip.float()).unsqueeze(1), g)
     out = ops.SegmentMMNode(t, a_weight, g)
     return (out.float() * alpha).to(h.dtype)
+
+
+def feed_forward(x, w_gate, w_up, w_down, activation: str = "silu"):
+    """A gated feed-forward block, (act(x @ w_gate) * (x @ w_up)) @ w_down.  The weights are
+    (K, F), (K, F) and (F, M) tensors of the rows' dtype, or all three the pairs that
+    ``ops.quantize_weight_fp8`` makes of them; then the rows are cut to 8 bits in front of both
+    products (``x``: features, or the pair that ``ops.rms_norm_fp8`` returned)."""
+    if not isinstance(w_gate, tuple):
+        return ops.linear(ops.gated_linear(x, w_gate, w_up, activation), w_down)
+    out_dtype = torch.bfloat16 if isinstance(x, tuple) else x.dtype
+    return _feed_forward_fp8(x if isinstance(x, tuple) else ops.quantize_fp8(x), w_gate, w_up,
+                             w_down, activation, out_dtype)
+
+
+def _feed_forward_fp8(rows, w_gate, w_up, w_down, activation, out_dtype):
+    hidden = ops.gated_linear_fp8(*rows, *w_gate, *w_up, activation=activation, out_dtype=out_dtype)
+    return ops.linear_fp8(*ops.quantize_fp8(hidden), *w_down, out_dtype=out_dtype)
+
+
+def hgt_block(g: DGLGraph, h, norm_attention, attention, norm_ff, ff, heads: int = 1,
+              activation: str = "silu", eps: float = 1e-6, fused=True):
+    """An HGT layer as a block of a deep network, with norms in front of both halves and a residual
+    stream behind them:
+
+      t   = h + hgt_layer(g, rms_norm(h, norm_attention), *attention)
+      out = t + feed_forward(rms_norm(t, norm_ff), *ff)
+
+    ``attention``: the eight weights that :func:`hgt_layer` takes after h, in its order; ``ff``: the
+    three of :func:`feed_forward`, as tensors or in 8 bits.  The addition in front of the second
+    norm is the norm kernel's, and with weights in 8 bits it writes the rows in 8 bits too."""
+    a = hgt_layer(g, ops.rms_norm(h, norm_attention, eps=eps), *attention, heads=heads, fused=fused)
+    if isinstance(ff[0], tuple):
+        x8, scales, t = ops.rms_norm_fp8(a, norm_ff, residual=h, eps=eps)
+        return t + _feed_forward_fp8((x8, scales), *ff, activation, h.dtype)
+    x, t = ops.rms_norm(a, norm_ff, residual=h, eps=eps)
+    return t + feed_forward(x, *ff, activation)
