@@ -156,6 +156,11 @@ def test_gradients_with_large_tiles_and_long_sums(rows, k, f, dtype):
     check_backward(rows, k, f, dtype, "silu")
 
 
+@pytest.mark.parametrize("rows,k,f", [(8192, 1280, 40), (70, 2048, 2600)])
+def test_gradients_of_rows_and_of_weights_with_large_tiles(rows, k, f):
+    check_backward(rows, k, f, torch.bfloat16, "silu")
+
+
 def test_gradients_against_differences():
     x, wg, wu, gh = make(2, 9, 40, 24, torch.float32)
     leaves = [t.requires_grad_() for t in (x, wg, wu)]

@@ -24,5 +24,6 @@ def test_nothing_is_spilled(tmp_path, source):
     assert "failed to meet occupancy" not in r.stderr
     spilled = [int(x) for x in re.findall(r"VGPRs Spill: (\d+)", r.stderr)]
     scratch = [int(x) for x in re.findall(r"ScratchSize \[bytes/lane\]: (\d+)", r.stderr)]
-    assert spilled and len(spilled) == len(scratch)
+    scalars = [int(x) for x in re.findall(r"SGPRs Spill: (\d+)", r.stderr)]
+    assert spilled and len(spilled) == len(scratch) == len(scalars) and not any(scalars)
     assert not any(spilled) and not any(scratch), (spilled, scratch)
