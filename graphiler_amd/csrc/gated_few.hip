@@ -1,7 +1,8 @@
 // act(x Wg) * (x Wu) for few rows of x: a query that is answered by itself.  All there is to do is
 // to read both weights once, with enough of them on their way: 64 columns a workgroup (128 or 256
 // bytes of a weight's row), its wavefronts take turns along k and add up what they have in
-// LDS, in their order.
+// LDS, in their order.  Three rows, 1024 to 4096, bf16 (16.8 MB): 5.7 us, 2.9 TB/s; a wavefront that
+// read 64 of k of both weights and then multiplied took 10.2.
 //
 // bf16 on v_mfma_f32_16x16x32_bf16.  A lane reads 16 bytes of eight rows of W, k = 8 (lane / 8) ... + 7 of 64,
 // columns 8 (lane % 8) ... + 7, and turns that 8 x 8 block in registers: for every column of it one
@@ -53,66 +54,69 @@ __device__ __forceinline__ void few_products(const uintx4 (&w)[8], const bf16x8 
   }
 }
 
-template <int RT, int WAVES>
-__global__ __launch_bounds__(WAVES *kWave) void gated_few_bf16_kernel(
+// Eight wavefronts, four for each weight, with CHUNKS times 64 of k on their way each: what the
+// registers hold beside RT times 32 sums.
+constexpr int kTurns = 4;
+template <int RT, int CHUNKS>
+__global__ __launch_bounds__(2 * kTurns *kWave) void gated_few_bf16_kernel(
     const bf16_t *__restrict__ x, const bf16_t *__restrict__ wg, const bf16_t *__restrict__ wu, bf16_t *__restrict__ h,
     int rows, int64_t K, int64_t F, int act) {
-  constexpr int kRows = 8 * RT;
-  __shared__ float sums[WAVES][2][kRows][kFewCols];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  constexpr int kRows = 8 * RT, kLd = kFewCols + 4;                    // rows of sums four banks apart
+  __shared__ float sums[kTurns][2][2][kRows][kLd];                     // turn, half of k, weight
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int turn = wave >> 1, which = wave & 1;
+  const bf16_t *__restrict__ w = which ? wu : wg;
   const int64_t c = (int64_t)blockIdx.x * kFewCols + (lane & 7) * 8;
   const int half = (lane >> 3) & 1, q = lane >> 4;                     // of operand x: rows lane % 8, k 8 (2 q + half) ...
-  floatx4 gate[RT][8], up[RT][8];
+  floatx4 acc[RT][8];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) gate[t][j] = up[t][j] = floatx4{0, 0, 0, 0};
-  for (int64_t k0 = (int64_t)wave * 64; k0 < K; k0 += WAVES * 64) {
-    uintx4 g[8], u[8];
-    bf16x8 xv[RT];
-    const int64_t kr = k0 + (lane >> 3) * 8;
-    auto take = [&](auto whole) {
+    for (int j = 0; j < 8; ++j) acc[t][j] = floatx4{0, 0, 0, 0};
+  for (int64_t k0 = (int64_t)turn * 64; k0 < K; k0 += kTurns * CHUNKS * 64) {
+    uintx4 v[CHUNKS][8];
+    bf16x8 xv[CHUNKS][RT];
+    auto take = [&](auto whole, int d, int64_t k1) {
       constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         const int row = t * 8 + (lane & 7);
-        xv[t] = __builtin_bit_cast(bf16x8, weight8<kWhole>(x, kWhole ? min(row, rows - 1) : row, rows,
-                                                           k0 + 8 * (2 * q + half), K));
+        xv[d][t] = __builtin_bit_cast(bf16x8, weight8<kWhole>(x, kWhole ? min(row, rows - 1) : row, rows,
+                                                              k1 + 8 * (2 * q + half), K));
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = weight8<kWhole>(wg, kr + i, K, c, F);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = weight8<kWhole>(wu, kr + i, K, c, F);
+      for (int i = 0; i < 8; ++i) v[d][i] = weight8<kWhole>(w, k1 + (lane >> 3) * 8 + i, K, c, F);
     };
-    if (k0 + 64 <= K && (int64_t)(blockIdx.x + 1) * kFewCols <= F) take(std::true_type());
-    else take(std::false_type());
-    few_products<RT>(g, xv, gate);
-    few_products<RT>(u, xv, up);
+    const int64_t behind = k0 + (CHUNKS - 1) * kTurns * 64 + 64;       // of the last of them
+    if (behind <= K && (int64_t)(blockIdx.x + 1) * kFewCols <= F) {
+#pragma unroll
+      for (int d = 0; d < CHUNKS; ++d) take(std::true_type(), d, k0 + d * kTurns * 64);
+    } else {
+#pragma unroll
+      for (int d = 0; d < CHUNKS; ++d) take(std::false_type(), d, k0 + d * kTurns * 64);
+    }
+#pragma unroll
+    for (int d = 0; d < CHUNKS; ++d) few_products<RT>(v[d], xv[d], acc);
   }
   // lane: row lane % 8 (of half lane / 8 % 2), results 4 q + r: of half q / 2, column 8 ((4 q + r) % 8) + j
+  if (half == q / 2) {
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float g = gate[t][j][r] + __shfl_xor(gate[t][j][r], 40), u = up[t][j][r] + __shfl_xor(up[t][j][r], 40);
-        if ((lane & 40) == 0) {
-          const int col = ((4 * q + r) & 7) * 8 + j;
-          sums[wave][0][t * 8 + (lane & 7)][col] = g;
-          sums[wave][1][t * 8 + (lane & 7)][col] = u;
-        }
-      }
+        for (int r = 0; r < 4; ++r) sums[turn][half][which][t * 8 + (lane & 7)][((4 * q + r) & 7) * 8 + j] = acc[t][j][r];
+  }
   __syncthreads();
-  for (int id = threadIdx.x; id < kRows * kFewCols; id += WAVES * kWave) {
+  for (int id = threadIdx.x; id < rows * kFewCols; id += 2 * kTurns * kWave) {
     const int row = id / kFewCols, col = id % kFewCols;
     const int64_t f = (int64_t)blockIdx.x * kFewCols + col;
-    if (row >= rows || f >= F) continue;
+    if (f >= F) continue;
     float g = 0.0f, u = 0.0f;
 #pragma unroll
-    for (int v = 0; v < WAVES; ++v) {
-      g += sums[v][0][row][col];
-      u += sums[v][1][row][col];
+    for (int t = 0; t < kTurns; ++t) {
+      g += sums[t][0][0][row][col] + sums[t][1][0][row][col];
+      u += sums[t][0][1][row][col] + sums[t][1][1][row][col];
     }
     h[row * F + f] = (bf16_t)f32_to_bf16_bits(gate_of(act, g) * u);
   }
@@ -225,11 +229,11 @@ int gated_few_launch(const void *x, const void *wg, const void *wu, void *h, int
       return GA_EUNSUPPORTED;
   } else {
     if (rows <= 8)
-      hipLaunchKernelGGL((gated_few_bf16_kernel<1, 8>), dim3((unsigned)grid), dim3(8 * kWave), 0, s, (const bf16_t *)x,
-                         (const bf16_t *)wg, (const bf16_t *)wu, (bf16_t *)h, (int)rows, K, F, act);
+      hipLaunchKernelGGL((gated_few_bf16_kernel<1, 4>), dim3((unsigned)grid), dim3(2 * kTurns * kWave), 0, s,
+                         (const bf16_t *)x, (const bf16_t *)wg, (const bf16_t *)wu, (bf16_t *)h, (int)rows, K, F, act);
     else if (rows <= 16)
-      hipLaunchKernelGGL((gated_few_bf16_kernel<2, 8>), dim3((unsigned)grid), dim3(8 * kWave), 0, s, (const bf16_t *)x,
-                         (const bf16_t *)wg, (const bf16_t *)wu, (bf16_t *)h, (int)rows, K, F, act);
+      hipLaunchKernelGGL((gated_few_bf16_kernel<2, 2>), dim3((unsigned)grid), dim3(2 * kTurns * kWave), 0, s,
+                         (const bf16_t *)x, (const bf16_t *)wg, (const bf16_t *)wu, (bf16_t *)h, (int)rows, K, F, act);
     else
       return GA_EUNSUPPORTED;
   }

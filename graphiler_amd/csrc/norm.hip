@@ -155,9 +155,11 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(
   for (int64_t row = (int64_t)blockIdx.x * groups + group; row < rows; row += (int64_t)gridDim.x * groups) {
     float t[NCH][kVec], g[NCH][kVec];
     float ss = 0.0f, dot = 0.0f;
+    int end = cols;                                    // opaque: its comparisons are made again for every row, not kept
+    asm volatile("" : "+s"(end));
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (lane + i * step) * kVec, n = cols - c;
+      const int c = (lane + i * step) * kVec, n = end - c;
       load_group(t_in + row * cols + c, n, t[i]);
       load_group(gy + row * cols + c, n, g[i]);
 #pragma unroll
@@ -170,9 +172,10 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(
     dot = lanes_sum<WIDE>(dot, lanes, across);
     const float inv = 1.0f / sqrtf(ss / cols + eps);
     const float back = inv * inv * inv * (dot / cols);
+    asm volatile("" : "+s"(end));
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (lane + i * step) * kVec, n = cols - c;
+      const int c = (lane + i * step) * kVec, n = end - c;
       float o[kVec];
       if (gt) load_group(gt + row * cols + c, n, o);
 #pragma unroll

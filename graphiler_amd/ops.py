@@ -1427,13 +1427,19 @@ def _check_rows(x, name: str) -> int:
 
 
 def _check_like(x, name: str, shape, like) -> None:
+    if x.shape == shape and x.dtype is like.dtype and x.get_device() == like.get_device() and x.is_contiguous():
+        return
     _check_input(x, name)
     if x.shape != shape or x.dtype != like.dtype or x.get_device() != like.get_device():
         raise RuntimeError(f"{name} must be {tuple(shape)}, of the dtype and on the device of the rows")
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_grad_form(what: str, *tensors) -> None:
@@ -1471,7 +1477,7 @@ def _scratch(n_bytes: int, device) -> Optional[torch.Tensor]:
 
 def _norm_args(x, weight, residual, eps):
     dt = _check_rows(x, "x")
-    rows, cols = int(x.shape[0]), int(x.shape[1])
+    rows, cols = x.shape
     if cols > RMS_NORM_MAX_COLS:
         raise RuntimeError(f"x must have at most {RMS_NORM_MAX_COLS} columns")
     if not eps >= 0:

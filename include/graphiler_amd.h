@@ -835,7 +835,7 @@ int ga_gated_linear_backward(const void *grad_h, const void *x, const void *w_ga
  * ga_rms_norm_fp8 write them, w8 (M, K) and w_scales as ga_quantize_weight_fp8 does; K is the padded
  * width, a multiple of 128.  y (rows, M) of `out_dtype`, accumulated in fp32 by the matrix
  * instruction, which adds eight products at a time and drops of those what lies 2^-13 below the largest.
- * A scale byte of 255 (NaN) makes its products NaN.  GA_EUNSUPPORTED when K exceeds 2^22.
+ * A scale byte of 255 (NaN) makes its products NaN.  GA_EUNSUPPORTED when K exceeds 32768.
  */
 int ga_linear_fp8(const void *x8, const void *x_scales, const void *w8, const void *w_scales, void *y,
                   int64_t rows, int64_t K, int64_t M, int out_dtype, ga_stream_t stream);

@@ -99,7 +99,7 @@ def test_fp8_codes():
     assert call(k=200) == EINVAL and call(k=0) == EINVAL and call(m=0) == EINVAL and call(rows=-3) == EINVAL
     assert call(xs=None) == EINVAL and call(w=None) == EINVAL and call(y=None) == EINVAL
     assert call(x=PTR + 8) == EALIGN and call(w=PTR + 1) == EALIGN and call(y=PTR + 1) == EALIGN
-    assert call(dt=9) == EUNSUPPORTED and call(k=1 << 23) == EUNSUPPORTED
+    assert call(dt=9) == EUNSUPPORTED and call(k=1 << 23) == EUNSUPPORTED and call(k=32896) == EUNSUPPORTED
     assert gated(act=5) == EUNSUPPORTED and gated(wu=None) == EINVAL and gated(us=None) == EINVAL
     assert gated(wu=PTR + 4) == EALIGN and gated(k=130) == EINVAL
 
