@@ -286,7 +286,7 @@ int norm_launch(const void *x, const void *res, const void *w, void *y, void *y8
   const RowShape r = row_shape(cols);
   const int padded = (int)((cols + kScaleBlock - 1) / kScaleBlock * kScaleBlock);
   const int64_t grid = r.wide ? rows : (rows + kBlock / r.lanes - 1) / (kBlock / r.lanes);
-  if (grid > 0x7fffffff) return GA_EUNSUPPORTED;
+  if (grid > kMostLanes / kBlock) return GA_EUNSUPPORTED;
 #define GA_NORM(N, W)                                                                                    \
   hipLaunchKernelGGL((norm_kernel<T, N, W, MODE>), dim3((unsigned)grid), dim3(kBlock), 0, s,             \
                      (const T *)x, (const T *)res, (const T *)w, (T *)y, (uint8_t *)y8,                  \
@@ -403,7 +403,7 @@ int ga_quantize_weight_fp8(const void *w, void *w8, void *scales, int64_t K, int
   if (!w || !w8 || !scales) return GA_EINVAL;
   if (!elem_aligned(dtype, w, nullptr, nullptr, nullptr, nullptr) || !aligned(w8, 16)) return GA_EALIGN;
   const int64_t kb = (K + kScaleBlock - 1) / kScaleBlock, mb = (M + kScaleBlock - 1) / kScaleBlock;
-  if (kb > 0x7fffffff || mb > 65535) return GA_EUNSUPPORTED;
+  if (kb > kMostLanes / kBlock || mb > 65535) return GA_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)kb, (unsigned)mb);
   if (dtype == GA_F32)

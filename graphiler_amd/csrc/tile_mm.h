@@ -18,7 +18,7 @@
 // The matrix instruction is given B as its first operand: a lane then holds four adjacent columns
 // of one row of C.
 #pragma once
-#include "common.h"
+#include "vec8.h"
 
 namespace ga {
 
@@ -661,7 +661,7 @@ template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, int WM, int WN, int
 int tile_mm_launch_as(const TileMm &p, const Epi &epi, hipStream_t s) {
   constexpr int kT = Mma<FP8>::kTile;
   const int64_t tiles = tiles_of(p.rows, p.cols, WM * TM * kT, WN * TN * kT / (PAIR ? 2 : 1));
-  if (tiles > 0x7fffffff || p.splits > 65535) return GA_EUNSUPPORTED;
+  if (tiles > kMostLanes / (WM * WN * kWave) || p.splits > 65535) return GA_EUNSUPPORTED;
   hipLaunchKernelGGL((tile_mm_kernel<FP8, A_ACROSS, B_ACROSS, PAIR, WM, WN, TM, TN, BLOCKS, Epi>),
                      dim3((unsigned)tiles, (unsigned)p.splits), dim3(WM * WN * kWave), 0, s, p, epi);
   return launch_status();

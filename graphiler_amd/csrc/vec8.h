@@ -7,6 +7,7 @@
 namespace ga {
 
 constexpr int kVec = 8;
+constexpr int64_t kMostLanes = 0xffffffff;   // of a launch, along one dimension of its grid
 
 struct __attribute__((packed, aligned(2))) Raw16 { uint32_t w[4]; };
 

@@ -809,7 +809,7 @@ int ga_rms_norm_backward(const void *grad_y, const void *sum, const void *weight
  * w_up (K, F), h (rows, F), all of `dtype`, sums in fp32, h rounded once.  activation: ga_gate
  * (silu: g / (1 + exp(-g)); gelu with the error function; relu).  fp32 products are formed from bf16
  * pieces as in ga_linear_attn (less than 2^-22 of a product is left out; inputs that are not finite
- * give NaN, operands below 2^-110 lose bits).  bf16 tensors whose rows are whole 16-byte pieces have to
+ * give NaN, operands below 2^-110 lose bits), of at most 16 rows by the fp32 instruction.  bf16 tensors whose rows are whole 16-byte pieces have to
  * be 16-byte aligned.  GA_EUNSUPPORTED when K or F exceeds 2^20.
  */
 enum ga_gate { GA_GATE_SILU = 0, GA_GATE_GELU = 1, GA_GATE_RELU = 2 };

@@ -104,6 +104,19 @@ def test_fp8_codes():
     assert gated(wu=PTR + 4) == EALIGN and gated(k=130) == EINVAL
 
 
+def test_more_workgroups_than_a_launch_takes_are_refused():
+    lib, many = capi.load(), 1 << 40
+    assert lib.ga_rms_norm(PTR, None, PTR, PTR, None, many, 64, 1e-6, capi.GA_F32, None) == EUNSUPPORTED
+    assert lib.ga_rms_norm(PTR, None, PTR, PTR, None, 1 << 24, 4096, 1e-6, capi.GA_F32, None) == EUNSUPPORTED
+    assert lib.ga_rms_norm_fp8(PTR, None, PTR, PTR, PTR, None, many, 64, 1e-6, capi.GA_BF16, None) == EUNSUPPORTED
+    assert lib.ga_quantize_fp8(PTR, PTR, PTR, many, 300, capi.GA_BF16, None) == EUNSUPPORTED
+    assert lib.ga_quantize_weight_fp8(PTR, PTR, PTR, many, 8, capi.GA_BF16, None) == EUNSUPPORTED
+    assert lib.ga_quantize_weight_fp8(PTR, PTR, PTR, 8, many, capi.GA_BF16, None) == EUNSUPPORTED
+    assert lib.ga_linear_fp8(PTR, PTR, PTR, PTR, PTR, 4, 128, many, capi.GA_BF16, None) == EUNSUPPORTED
+    assert lib.ga_linear_fp8(PTR, PTR, PTR, PTR, PTR, many, 128, 64, capi.GA_BF16, None) == EUNSUPPORTED
+    assert lib.ga_gated_linear(PTR, PTR, PTR, PTR, many, 64, 64, 0, capi.GA_BF16, None, 0, None) == EUNSUPPORTED
+
+
 def test_operators_refuse_host_tensors_and_names():
     x, w = torch.randn(3, 8), torch.ones(8)
     for call in (lambda: ops.rms_norm(x, w), lambda: ops.rms_norm_fp8(x, w), lambda: ops.quantize_fp8(x),
