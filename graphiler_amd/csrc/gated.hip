@@ -15,8 +15,8 @@
 // call, as are operands whose rows are not whole 16-byte pieces.
 //
 // Measured, bf16, K = 1024, F = 4096: 16,384 rows 228 us (1.20 PFLOP/s), gradients of 8,192 rows 378 us: dg and du
-// 145-155 (both products and 201 MB), grad_x 121, the weights' 122.  fp32, 2,708 x 128 -> 341: 12 us and 4 to lay out;
-// gradients of 2,001 x 300 -> 700: 28 + 22 + 22, 12 to add up parts, 5 to lay out.  At most 16 rows: gated_few.hip.
+// 145-155 (both products and 201 MB), grad_x 121, the weights' 122.  fp32, 4,096 x 256 -> 1024: 35 us; forward products of
+// few tiles: gated_f32.hip.  fp32 gradients of 2,001 x 300 -> 700: 28 + 22 + 22, 12 to add up parts, 5 to lay out.  At most 16 rows: gated_few.hip.
 #include "gated_few.h"
 #include "vec8.h"
 
@@ -361,7 +361,8 @@ extern "C" {
 
 size_t ga_gated_linear_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype) {
   if (ga::check_gated(rows, K, F, GA_GATE_SILU, dtype) != GA_OK) return 0;
-  return rows <= ga::kGatedFewRows ? 0 : ga::plan_of(rows, K, F, dtype, false).bytes;
+  if (rows <= ga::kGatedFewRows || (dtype == GA_F32 && ga::gated_f32_taken(rows, K, F))) return 0;
+  return ga::plan_of(rows, K, F, dtype, false).bytes;
 }
 
 int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h, int64_t rows, int64_t K, int64_t F,
@@ -375,6 +376,8 @@ int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h
     return GA_EALIGN;
   if (rows <= kGatedFewRows)
     return gated_few_launch(x, w_gate, w_up, h, rows, K, F, activation, dtype, (hipStream_t)stream);
+  if (dtype == GA_F32 && gated_f32_taken(rows, K, F))
+    return gated_f32_launch(x, w_gate, w_up, h, rows, K, F, activation, (hipStream_t)stream);
   const Plan p = plan_of(rows, K, F, dtype, false);
   if (p.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return GA_EWORKSPACE;
   hipStream_t s = (hipStream_t)stream;

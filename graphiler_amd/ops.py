@@ -1689,8 +1689,8 @@ def gated_linear(x, w_gate, w_up, activation: str = "silu"):
     """act(x @ w_gate) * (x @ w_up) from one kernel: the first half of a feed-forward block
     (:func:`linear` is the other).  x (rows, K), w_gate and w_up (K, F) of one dtype; activation
     "silu" | "gelu" (with the error function) | "relu".  Sums in fp32, one rounding; fp32
-    products are those of :func:`linear_attn` (of at most 16 rows: the fp32 instruction's).  A bf16
-    tensor whose rows are whole 16-byte pieces has to begin at one.  Differentiable in all three."""
+    products are those of :func:`linear_attn`, or the fp32 instruction's where that is faster (few
+    rows, columns or tiles).  A bf16 tensor whose rows are whole 16-byte pieces has to begin at one.  Differentiable in all three."""
     if _wants_grad(x, w_gate, w_up):
         return _GatedLinear.apply(x, w_gate, w_up, activation)
     return _gated_linear(x, w_gate, w_up, activation)

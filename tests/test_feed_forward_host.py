@@ -59,7 +59,7 @@ def test_norm_backward_codes():
 @pytest.mark.parametrize("dt", [capi.GA_F32, capi.GA_BF16])
 def test_gated_codes(dt):
     lib = capi.load()
-    rows, k, f = 40, 65, 33
+    rows, k, f = 20_000, 65, 133
     n = lib.ga_gated_linear_workspace_bytes(rows, k, f, dt)
     assert n > 0 and lib.ga_gated_linear_workspace_bytes(3, k, f, dt) == 0
     assert lib.ga_gated_linear_workspace_bytes(rows, 64, 64, capi.GA_BF16) == 0

@@ -91,6 +91,27 @@ def test_forward_against_float64(rows, k, f, dtype):
     check_forward(rows, k, f, dtype, "silu")
 
 
+# fp32: tiles of 32 and of 64 rows on the fp32 instruction, ends in k, rows and columns, one step and several;
+# then few columns; then pieces in tiles of 64 and of 128 rows
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("rows,k,f", [(50, 63, 97), (70, 64, 128), (33, 130, 31), (2708, 65, 341), (3001, 1, 353), (2720, 256, 352),
+                                      (9001, 33, 96), (2048, 300, 704), (3000, 72, 1000)])
+def test_fp32_tiles(rows, k, f, act):
+    check_forward(rows, k, f, torch.float32, act)
+
+
+@pytest.mark.parametrize("rows", [20, 2708])
+def test_fp32_infinities_and_small_values_of_few_tiles(rows):
+    x = torch.zeros(rows, 96)
+    x[0, 3], x[1, 4], x[rows - 1] = math.inf, 1e-36, 1.0
+    w = torch.ones(96, 341)
+    got = ops.gated_linear(x.cuda(), w.cuda(), w.cuda(), "relu").cpu()
+    assert (got[0] == math.inf).all() and (got[rows - 1] == 96 * 96).all()
+    got = ops.gated_linear(x.cuda(), w.cuda(), 1e36 * w.cuda(), "relu").cpu()
+    # 1e-36 times (1e-36 times 1e36): two roundings of operands, two of products, one of the bound
+    assert ((got[1].double() / 1e-36 - 1.0).abs() <= 5 * 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("rows,k,f", [(4, 96, 80), (150, 75, 133)])

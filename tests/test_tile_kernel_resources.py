@@ -13,7 +13,7 @@ HIPCC = "/opt/rocm/bin/hipcc"
 
 
 @pytest.mark.skipif(not (os.path.exists(HIPCC) or shutil.which("hipcc")), reason="no hipcc")
-@pytest.mark.parametrize("source", ["norm", "gated", "gated_few", "fp8_mm"])
+@pytest.mark.parametrize("source", ["norm", "gated", "gated_few", "gated_f32", "fp8_mm"])
 def test_nothing_is_spilled(tmp_path, source):
     r = subprocess.run([HIPCC if os.path.exists(HIPCC) else "hipcc", "--offload-arch=gfx950", "-O3",
                         "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang",
