@@ -17,8 +17,8 @@ namespace {
 // Few rows: a workgroup takes 16 rows of w, its eight wavefronts take turns along K and add up what they have in
 // LDS; each reads 32 bytes a lane of w and of x for an instruction of 16 x 16 x 128, several ahead.  What counts is
 // how much of w is on its way: with RT > 2 the rows of x take the registers of two of the four steps.  One row by
-// 4096 x 4096, 16.8 MB: 4.9 us (3.4 TB/s).  Rows up to 64 come here because a grid of tiles has 1/8 of the
-// workgroups for the same weights.
+// 4096 x 4096, 16.8 MB: 4.9 us (3.4 TB/s).  Up to 64 rows: 33 x 8192 -> 4096
+// 19 us, in tiles 37; 64 rows 27 and 37; further blocks of 64 rows read w again, 100 rows 46 and 37.
 constexpr int kFewWaves = 8;
 template <int RT, bool PAIR, typename T>
 __global__ __launch_bounds__(kFewWaves *kWave) void few_fp8_kernel(

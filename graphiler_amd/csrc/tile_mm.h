@@ -685,16 +685,21 @@ int tile_mm_launch(const TileMm &p, const Epi &epi, hipStream_t s) {
   const int tile = tile_for(p, PAIR);
   if constexpr (Epi::kLarge) {
     if (tile == kTile256 && blocks <= 64)
-      return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, 64>(p, epi, s);
+      return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, FP8 ? 64 : 0>(p, epi, s);
   }
-  if (tile == kTile64 && blocks <= 32) {
-    if constexpr (!FP8) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, 2, 4, 32>(p, epi, s);
-    else if constexpr (PAIR) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 1, 2, 2, 2, 32>(p, epi, s);
-    else return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 1, 4, 2, 1, 32>(p, epi, s);
+  if constexpr (!FP8) {
+    if (tile == kTile64) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, 2, 4, 0>(p, epi, s);
+    return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 0>(p, epi, s);
+  } else {
+    // room for the scales of 64 blocks or of all: with more of it fewer workgroups share a compute unit
+    constexpr int kSide = PAIR ? 2 : 4, kNext = PAIR ? 2 : 1;
+    if (tile == kTile64) {
+      if (blocks <= 64) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 1, kSide, 2, kNext, 64>(p, epi, s);
+      return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 1, kSide, 2, kNext, kMostBlocks>(p, epi, s);
+    }
+    if (blocks <= 64) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 64>(p, epi, s);
+    return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, kMostBlocks>(p, epi, s);
   }
-  if (blocks <= 32) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 32>(p, epi, s);
-  if constexpr (FP8) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, kMostBlocks>(p, epi, s);
-  return GA_EUNSUPPORTED;
 }
 
 }  // namespace ga

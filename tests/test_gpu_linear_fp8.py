@@ -92,6 +92,24 @@ def test_whole_numbers_are_exact(rows, k, m):
     assert torch.equal(y.double(), wide(x8, xs, 1) @ wide(w8, ws, 128).t())
 
 
+@pytest.mark.parametrize("rows,k,m", [(70, 4224, 130), (70, 8192, 130), (70, 8320, 130), (100, 32768, 96), (2300, 8192, 2100),
+                                      (2300, 8320, 2100), (3900, 8320, 3900)])
+def test_many_blocks(rows, k, m):
+    """Around the numbers of blocks that change what a tile keeps: whole numbers, so that all sums are exact (below
+    2^24 of the smallest), and of the gated form one rounding of a product of exact numbers."""
+    gen = torch.Generator().manual_seed(k)
+    x = torch.randint(-4, 5, (rows, k), generator=gen).to(torch.float8_e4m3fn).cuda()
+    wg, wu = (torch.randint(-4, 5, (m, k), generator=gen).to(torch.float8_e4m3fn).cuda() for _ in range(2))
+    ex = torch.randint(-9, 9, (rows, 1), generator=gen).expand(rows, k // 128).contiguous()
+    ex[:, -1] += 1                                       # the last block's scale is its own
+    xs = (ex + 127).to(torch.uint8).view(torch.float8_e8m0fnu).cuda()
+    ws = torch.full((-(-m // 128), k // 128), 125, dtype=torch.uint8).view(torch.float8_e8m0fnu).cuda()
+    g, u = (wide(x, xs, 1) @ wide(w, ws, 128).t() for w in (wg, wu))
+    assert torch.equal(ops.linear_fp8(x, xs, wg, ws, out_dtype=torch.float32).double(), g)
+    h = ops.gated_linear_fp8(x, xs, wg, ws, wu, ws, activation="relu", out_dtype=torch.float32)
+    assert torch.equal(h, torch.relu(g).float() * u.float())
+
+
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("rows,k,f", [(1, 256, 512), (3, 128, 5), (17, 300, 127), (130, 256, 129), (70, 640, 1000),
