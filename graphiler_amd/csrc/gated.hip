@@ -72,7 +72,6 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 template <typename T, int ACT = -1>
 struct GradEpi : Stored<bf16_t> {
   static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1, kOut = 2 * kPieces;
-  static constexpr bool kLarge = true;
   const T *gh;
   int64_t gh_cols;
   bf16_t *dg, *du;
@@ -138,16 +137,6 @@ struct GradEpi : Stored<bf16_t> {
     bf16_t *to = (k < kPieces ? dg : du) + k % kPieces * plane;
     store_chunk(to + row * ld + col, w, n);
   }
-};
-
-// The sums behind dg and du: bf16 results in tiles of either size, fp32 ones (parts of a sum among them) in small ones.
-template <typename T> struct RowsEpi : StoreEpi<T> {
-  static constexpr bool kLarge = sizeof(T) == 2;
-  using StoreEpi<T>::StoreEpi;
-};
-template <typename T> struct WeightsEpi : StorePairEpi<T> {
-  static constexpr bool kLarge = sizeof(T) == 2;
-  using StorePairEpi<T>::StorePairEpi;
 };
 
 // Sums of the parts of a contraction, `all` values each: n of the first result, then the second's.
@@ -308,10 +297,10 @@ int backward(const void *gh, const void *x, const void *wg, const void *wu, void
     m.a_plane = 2 * d_plane;
     m.b_plane = 2 * w_plane;
     if (p.x_splits == 1) {
-      if (int rc = tile_mm_launch<false, false, false, false>(m, RowsEpi<T>((T *)gx, K, 0), s)) return rc;
+      if (int rc = tile_mm_launch<false, false, false, false>(m, StoreEpi<T>((T *)gx, K, 0), s)) return rc;
     } else {
       float *parts = (float *)(ws + p.parts);
-      if (int rc = tile_mm_launch<false, false, false, false>(m, RowsEpi<float>(parts, K, rows * K), s)) return rc;
+      if (int rc = tile_mm_launch<false, false, false, false>(m, StoreEpi<float>(parts, K, rows * K), s)) return rc;
       hipLaunchKernelGGL((join_parts_kernel<T>), dim3(stream_grid(rows * K)), dim3(kBlock), 0, s, parts, (T *)gx,
                          (T *)nullptr, rows * K, rows * K, p.x_splits);
       if (int rc = launch_status()) return rc;
@@ -332,9 +321,9 @@ int backward(const void *gh, const void *x, const void *wg, const void *wu, void
   m.a_plane = 2 * x_plane;
   m.b_plane = 2 * d_plane;
   if (p.splits == 1)
-    return tile_mm_launch<false, true, true, true>(m, WeightsEpi<T>((T *)gwg, (T *)gwu, F, 0), s);
+    return tile_mm_launch<false, true, true, true>(m, StorePairEpi<T>((T *)gwg, (T *)gwu, F, 0), s);
   float *parts = (float *)(ws + p.parts);
-  const WeightsEpi<float> e(parts, parts + K * F, F, 2 * K * F);
+  const StorePairEpi<float> e(parts, parts + K * F, F, 2 * K * F);
   if (int rc = tile_mm_launch<false, true, true, true>(m, e, s)) return rc;
   hipLaunchKernelGGL((join_parts_kernel<T>), dim3(stream_grid(2 * K * F)), dim3(kBlock), 0, s, parts, (T *)gwg,
                      (T *)gwu, K * F, 2 * K * F, p.splits);

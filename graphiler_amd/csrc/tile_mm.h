@@ -590,7 +590,6 @@ __device__ __forceinline__ float gate_slope(int act, float g) {
 template <typename T>
 struct StoreEpi : Stored<T> {            // C as it is; of part z of the contraction `part` values further on
   static constexpr int kOut = 1;
-  static constexpr bool kLarge = true;   // whether tiles of 256 x 256 are taken
   T *out;
   int64_t ld, part;
   StoreEpi(T *o, int64_t l, int64_t n) : out(o), ld(l), part(n) {}
@@ -606,7 +605,6 @@ struct StoreEpi : Stored<T> {            // C as it is; of part z of the contrac
 template <typename T>
 struct StorePairEpi : Stored<T> {        // both products of a PAIR, likewise
   static constexpr int kOut = 2;
-  static constexpr bool kLarge = true;
   T *out0, *out1;
   int64_t ld, part;
   StorePairEpi(T *o0, T *o1, int64_t l, int64_t n) : out0(o0), out1(o1), ld(l), part(n) {}
@@ -623,7 +621,6 @@ struct StorePairEpi : Stored<T> {        // both products of a PAIR, likewise
 template <typename T, int ACT = -1>
 struct GateEpi : Stored<T> {             // act(first) * second
   static constexpr int kOut = 1;
-  static constexpr bool kLarge = true;
   T *out;
   int64_t ld;
   int act;
@@ -683,10 +680,8 @@ int tile_mm_launch(const TileMm &p, const Epi &epi, hipStream_t s) {
   const int blocks = FP8 ? (int)((p.K + 127) / 128) : 0;
   if (blocks > kMostBlocks) return GA_EUNSUPPORTED;
   const int tile = tile_for(p, PAIR);
-  if constexpr (Epi::kLarge) {
-    if (tile == kTile256 && blocks <= 64)
-      return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, FP8 ? 64 : 0>(p, epi, s);
-  }
+  if (tile == kTile256 && blocks <= 64)
+    return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, FP8 ? 64 : 0>(p, epi, s);
   if constexpr (!FP8) {
     if (tile == kTile64) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, 2, 4, 0>(p, epi, s);
     return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 0>(p, epi, s);

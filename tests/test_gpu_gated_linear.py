@@ -177,9 +177,10 @@ def test_gradients_with_large_tiles_and_long_sums(rows, k, f, dtype):
     check_backward(rows, k, f, dtype, "silu")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,k,f", [(8192, 1280, 40), (70, 2048, 2600)])
-def test_gradients_of_rows_and_of_weights_with_large_tiles(rows, k, f):
-    check_backward(rows, k, f, torch.bfloat16, "silu")
+def test_gradients_of_rows_and_of_weights_with_large_tiles(rows, k, f, dtype):
+    check_backward(rows, k, f, dtype, "silu")
 
 
 def test_gradients_against_differences():
