@@ -248,11 +248,21 @@ def feed_forward(x, w_gate, w_up, w_down, activation: str = "silu"):
     (K, F), (K, F) and (F, M) tensors of the rows' dtype, or all three the pairs that
     ``ops.quantize_weight_fp8`` makes of them; then the rows are cut to 8 bits in front of both
     products (``x``: features, or the pair that ``ops.rms_norm_fp8`` returned)."""
-    if not isinstance(w_gate, tuple):
+    in_8_bits = _in_8_bits(w_gate, w_up, w_down)
+    if isinstance(x, tuple) and not in_8_bits:
+        raise RuntimeError("rows in 8 bits need weights in 8 bits")
+    if not in_8_bits:
         return ops.linear(ops.gated_linear(x, w_gate, w_up, activation), w_down)
     out_dtype = torch.bfloat16 if isinstance(x, tuple) else x.dtype
     return _feed_forward_fp8(x if isinstance(x, tuple) else ops.quantize_fp8(x), w_gate, w_up,
                              w_down, activation, out_dtype)
+
+
+def _in_8_bits(*weights) -> bool:
+    pairs = [isinstance(w, tuple) for w in weights]
+    if any(pairs) != all(pairs):
+        raise RuntimeError("weights must be all tensors or all pairs in 8 bits")
+    return all(pairs)
 
 
 def _feed_forward_fp8(rows, w_gate, w_up, w_down, activation, out_dtype):
@@ -271,8 +281,9 @@ def hgt_block(g: DGLGraph, h, norm_attention, attention, norm_ff, ff, heads: int
     ``attention``: the eight weights that :func:`hgt_layer` takes after h, in its order; ``ff``: the
     three of :func:`feed_forward`, as tensors or in 8 bits.  The addition in front of the second
     norm is the norm kernel's, and with weights in 8 bits it writes the rows in 8 bits too."""
+    in_8_bits = _in_8_bits(*ff)
     a = hgt_layer(g, ops.rms_norm(h, norm_attention, eps=eps), *attention, heads=heads, fused=fused)
-    if isinstance(ff[0], tuple):
+    if in_8_bits:
         x8, scales, t = ops.rms_norm_fp8(a, norm_ff, residual=h, eps=eps)
         return t + _feed_forward_fp8((x8, scales), *ff, activation, h.dtype)
     x, t = ops.rms_norm(a, norm_ff, residual=h, eps=eps)

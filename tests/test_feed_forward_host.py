@@ -3,7 +3,7 @@ before they launch, the Python operators raise before they call."""
 import pytest
 import torch
 
-from graphiler_amd import capi, ops
+from graphiler_amd import capi, layers, ops
 
 PTR = 1 << 20            # a pointer that is aligned and never followed
 EINVAL, EUNSUPPORTED, EWORKSPACE, EALIGN = -1, -2, -3, -4
@@ -130,3 +130,12 @@ def test_operators_refuse_host_tensors_and_names():
         ops.gated_linear(x, torch.randn(8, 4), torch.randn(8, 4), activation="tanh")
     with pytest.raises(RuntimeError, match="activation"):
         ops.gated_linear_fp8(x, x, x, x, x, x, activation=None)
+
+
+def test_weights_of_a_block_are_all_of_one_kind():
+    x, w = torch.randn(3, 8), torch.randn(8, 8)
+    for call in (lambda: layers.feed_forward(x, (w, w), w, w), lambda: layers.feed_forward(x, w, w, (w, w)),
+                 lambda: layers.feed_forward((x, x), w, w, w),
+                 lambda: layers.hgt_block(None, x, w[0], (), w[0], (w, (w, w), w))):
+        with pytest.raises(RuntimeError, match="8 bits"):
+            call()
