@@ -247,12 +247,16 @@ def feed_forward(x, w_gate, w_up, w_down, activation: str = "silu"):
     """A gated feed-forward block, (act(x @ w_gate) * (x @ w_up)) @ w_down.  The weights are
     (K, F), (K, F) and (F, M) tensors of the rows' dtype, or all three the pairs that
     ``ops.quantize_weight_fp8`` makes of them; then the rows are cut to 8 bits in front of both
-    products (``x``: features, or the pair that ``ops.rms_norm_fp8`` returned)."""
+    products (``x``: features, or the pair that ``ops.rms_norm_fp8`` returned).  Differentiable with
+    weights that are tensors."""
     in_8_bits = _in_8_bits(w_gate, w_up, w_down)
     if isinstance(x, tuple) and not in_8_bits:
         raise RuntimeError("rows in 8 bits need weights in 8 bits")
     if not in_8_bits:
-        return ops.linear(ops.gated_linear(x, w_gate, w_up, activation), w_down)
+        hidden = ops.gated_linear(x, w_gate, w_up, activation)
+        if torch.is_grad_enabled() and (hidden.requires_grad or w_down.requires_grad):
+            return torch.mm(hidden, w_down)              # ops.linear's kernels have no gradients
+        return ops.linear(hidden, w_down)
     out_dtype = torch.bfloat16 if isinstance(x, tuple) else x.dtype
     return _feed_forward_fp8(x if isinstance(x, tuple) else ops.quantize_fp8(x), w_gate, w_up,
                              w_down, activation, out_dtype)
@@ -280,7 +284,11 @@ def hgt_block(g: DGLGraph, h, norm_attention, attention, norm_ff, ff, heads: int
 
     ``attention``: the eight weights that :func:`hgt_layer` takes after h, in its order; ``ff``: the
     three of :func:`feed_forward`, as tensors or in 8 bits.  The addition in front of the second
-    norm is the norm kernel's, and with weights in 8 bits it writes the rows in 8 bits too."""
+    norm is the norm kernel's, and with weights in 8 bits it writes the rows in 8 bits too.  Not
+    differentiable, as the layer is not."""
+    if torch.is_grad_enabled() and any(
+            isinstance(t, torch.Tensor) and t.requires_grad for t in (h, norm_attention, *attention, norm_ff, *ff)):
+        raise RuntimeError("hgt_block has no gradient: call it under torch.no_grad()")
     in_8_bits = _in_8_bits(*ff)
     a = hgt_layer(g, ops.rms_norm(h, norm_attention, eps=eps), *attention, heads=heads, fused=fused)
     if in_8_bits:

@@ -132,6 +132,16 @@ def test_operators_refuse_host_tensors_and_names():
         ops.gated_linear_fp8(x, x, x, x, x, x, activation=None)
 
 
+def test_a_block_without_gradients_says_so():
+    x, w = torch.randn(3, 8), torch.randn(8, 8)
+    for which in range(3):
+        leaf = torch.randn(8, 8, requires_grad=True)
+        args = [[x, w[0], (w,), w[0], (w, w, w)] for _ in range(3)][which]
+        args[(0, 2, 4)[which]] = (leaf, (leaf,), (w, w, leaf))[which]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            layers.hgt_block(None, *args)
+
+
 def test_weights_of_a_block_are_all_of_one_kind():
     x, w = torch.randn(3, 8), torch.randn(8, 8)
     for call in (lambda: layers.feed_forward(x, (w, w), w, w), lambda: layers.feed_forward(x, w, w, (w, w)),

@@ -124,6 +124,25 @@ def test_gradients_are_the_same_with_two_streams_and_no_order(device):
             assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("rows,m", [(300, 32), (20000, 48), (50, 130)])
+def test_gradients_of_a_feed_forward_block(device, rows, m):
+    """Those of the last weight too, at sizes whose product without gradients is the framework's own kernel."""
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 96, generator=gen).to(device)
+    wg, wu = (torch.randn(96, 200, generator=gen).to(device) / 10 for _ in range(2))
+    wd = torch.randn(200, m, generator=gen).to(device) / 14
+    leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+    out = layers.feed_forward(*leaves)
+    out.pow(2).sum().backward()
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    ((F.silu(wide[0] @ wide[1]) * (wide[0] @ wide[2])) @ wide[3]).pow(2).sum().backward()
+    for got, want in zip(leaves, wide):
+        assert ((got.grad.double() - want.grad).norm() / want.grad.norm()).item() <= 2.0 ** -18
+    with torch.no_grad():
+        again = layers.feed_forward(*leaves)
+    assert ((again - out).norm() / out.norm()).item() <= 2.0 ** -18
+
+
 def test_refusals(device):
     x, w = torch.randn(4, 64, device=device), torch.ones(64, device=device)
     wide = torch.randn(64, 32, device=device)
