@@ -160,8 +160,11 @@ __device__ __forceinline__ void tile_of(int id, int n_tiles, int row_tiles, int 
   const int t = x * per + min(x, more) + at;
   const int band = t / (8 * col_tiles), in = t % (8 * col_tiles);
   const int high = min(8, row_tiles - band * 8);
-  tr = band * 8 + in % high;
-  tc = in / high;
+  // In scalar registers by order: divisions are formed in vector registers, and where the compiler leaves the results
+  // there every descriptor made of them costs a loop over its lanes' values.  Behind such a loop no lane is active, and
+  // what is spilled there is lost (a build of 256 x 256 fp32 tiles spilled a tile's place and put all tiles at one).
+  tr = __builtin_amdgcn_readfirstlane(band * 8 + in % high);
+  tc = __builtin_amdgcn_readfirstlane(in / high);
 }
 
 // All but the youngest N loads of this wavefront have arrived.
