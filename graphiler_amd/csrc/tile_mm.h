@@ -349,6 +349,9 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   fetch(L0, 0);
   fetch(L0, 1);
   advance();
+  // The first wait is for all but the youngest moves: none of the second step's may go ahead of the first's.
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("; moves of the second step" ::: "memory");
   fetch(L1, 0);
 
   typename M::operand a[TM], b[2][TN];

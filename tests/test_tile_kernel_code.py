@@ -55,8 +55,8 @@ def loops_around_loads(lines):
 
 def test_a_tile_s_place_is_scalar_whatever_the_epilogue(tmp_path):
     """A descriptor in vector registers is taken lane by lane, in a loop behind which no lane is active: what the compiler
-    spills there is lost.  In the library as built what hides the epilogue's lane happens to keep descriptors scalar; here
-    they have to be without it."""
+    spills there is lost.  As the library is built, what hides the epilogue's lane happens to keep descriptors scalar; here
+    they have to be so without it."""
     folder = tmp_path / "graphiler_amd" / "csrc"
     folder.mkdir(parents=True)
     (tmp_path / "include").mkdir()
@@ -74,10 +74,29 @@ def test_a_tile_s_place_is_scalar_whatever_the_epilogue(tmp_path):
         assert not any("scratch_store" in line for line in lines)
 
 
-@pytest.mark.parametrize("source", ["gated", "fp8_mm"])
-def test_no_descriptor_is_taken_lane_by_lane(tmp_path, source):
-    kernels = assembly(source + ".hip", CSRC, tmp_path / "kernels.s")
+@pytest.fixture(scope="module", params=["gated", "fp8_mm"])
+def tile_kernels(request, tmp_path_factory):
+    kernels = assembly(request.param + ".hip", CSRC, tmp_path_factory.mktemp("code") / "kernels.s")
     tiles = {k: v for k, v in kernels.items() if "tile_mm_kernel" in k}
     assert tiles
-    for name, lines in tiles.items():
+    return tiles
+
+
+def test_no_descriptor_is_taken_lane_by_lane(tile_kernels):
+    for name, lines in tile_kernels.items():
         assert loops_around_loads(lines) == 0, name
+
+
+def test_the_first_wait_leaves_only_moves_of_the_second_step(tile_kernels):
+    """The wait in front of the first barrier counts: all loads but the youngest n have arrived.  The first step's tiles
+    are whole only if those n are moves of the second step, with every move of the first in front of them."""
+    for name, lines in tile_kernels.items():
+        moves = [i for i, line in enumerate(lines) if "buffer_load_dwordx4" in line and " lds" in line]
+        fence = [i for i, line in enumerate(lines) if "; moves of the second step" in line]
+        assert len(fence) == 1, name
+        barrier = next(i for i, line in enumerate(lines) if "s_barrier" in line)
+        assert fence[0] < barrier, name
+        counts = [re.search(r"vmcnt\((\d+)\)", line) for line in lines[fence[0]:barrier] if "s_waitcnt" in line]
+        n = int([c for c in counts if c][-1].group(1))
+        assert n > 0 and sum(fence[0] < i < barrier for i in moves) == n, name
+        assert sum(i < fence[0] for i in moves) in (2 * n - 1, 2 * n), name
