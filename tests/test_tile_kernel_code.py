@@ -100,3 +100,29 @@ def test_the_first_wait_leaves_only_moves_of_the_second_step(tile_kernels):
         n = int([c for c in counts if c][-1].group(1))
         assert n > 0 and sum(fence[0] < i < barrier for i in moves) == n, name
         assert sum(i < fence[0] for i in moves) in (2 * n - 1, 2 * n), name
+
+
+# 48 values that are all alive between two barriers, in 24 registers
+SPILLS = """
+#include "common.h"
+__global__ __attribute__((amdgpu_num_vgpr(24))) void spilling_kernel(float *p) {
+  float v[48];
+#pragma unroll
+  for (int i = 0; i < 48; ++i) v[i] = p[i * 64 + threadIdx.x];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 48; ++i) p[i * 64 + (threadIdx.x ^ 1)] = v[47 - i];
+}
+"""
+
+
+@pytest.mark.parametrize("spills", [True, False])
+def test_the_library_is_not_built_from_a_kernel_that_spills(tmp_path, spills):
+    csrc = tmp_path / "graphiler_amd" / "csrc"
+    shutil.copytree(CSRC, csrc, ignore=shutil.ignore_patterns("build"))
+    shutil.copytree(os.path.join(CSRC, "..", "..", "include"), tmp_path / "include")
+    (csrc / "gated_few.hip").write_text(SPILLS if spills else SPILLS.replace("amdgpu_num_vgpr(24)", "amdgpu_num_vgpr(128)"))
+    r = subprocess.run(["make", "-C", str(csrc), "build/gated_few.o"], capture_output=True, text=True, timeout=900)
+    assert (r.returncode != 0) == spills, r.stderr[-2000:]
+    assert (csrc / "build" / "gated_few.o").exists() != spills
+    assert ("gated_few.hip: a kernel spills" in r.stderr) == spills
