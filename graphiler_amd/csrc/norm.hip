@@ -4,7 +4,7 @@
 //   t = x + r                 (x alone without a residual), kept in 32 bits, stored rounded
 //   i = 1 / sqrt(mean(t^2) + eps)
 //   y = t i w
-//   grad_x = i (w gy) - t i^3 mean(t w gy) + gt,   grad_w = sum over rows of gy t i
+//   grad_x = i (w gy - t i mean(t i w gy)) + gt,   grad_w = sum over rows of gy t i
 //
 // 8-bit rows (e4m3): every 128 values of a row share a scale 2^e, the smallest with which the
 // block's largest finite magnitude is at most 448; e lies in [-126, 126] (a block of zeros: 0)
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(
     ss = lanes_sum<WIDE>(ss, lanes, across);
     dot = lanes_sum<WIDE>(dot, lanes, across);
     const float inv = 1.0f / sqrtf(ss / cols + eps);
-    const float back = inv * inv * inv * (dot / cols);
+    const float mean = inv * (dot / cols);             // of y gy; the cube of inv alone may leave the range
     asm volatile("" : "+s"(end));
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -184,9 +184,10 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(
       if (gt) load_group(gt + row * cols + c, n, o);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const float d = inv * (wv[i][j] * g[i][j]) - t[i][j] * back;
+        const float unit = t[i][j] * inv;
+        const float d = inv * (wv[i][j] * g[i][j] - unit * mean);
         o[j] = gt ? o[j] + d : d;
-        gw[i][j] = fmaf(g[i][j], t[i][j] * inv, gw[i][j]);
+        gw[i][j] = fmaf(g[i][j], unit, gw[i][j]);
       }
       store_group(gx + row * cols + c, n, o);
     }

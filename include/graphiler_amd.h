@@ -763,7 +763,8 @@ int ga_project_attn_strided(const void *X, const void *W, const float *a_l, cons
 /*
  * Root-mean-square norm with the residual's addition:
  *   t = x + residual (x alone where residual is NULL), y = t / sqrt(mean(t^2) + eps) * weight
- * x, residual, y, sum (rows, cols), weight (cols), all of `dtype`; t is kept in fp32 and, where
+ * x, residual, y, sum (rows, cols), weight (cols), all of `dtype`; the sum of t^2 has to be in fp32's
+ * range (values about 1e16 and, without eps, 1e-16 are); t is kept in fp32 and, where
  * sum is not NULL (residual only), stored rounded there.  sum may be residual or x itself.
  * GA_EUNSUPPORTED when cols > 16384.
  */
@@ -793,7 +794,7 @@ int ga_quantize_weight_fp8(const void *w, void *w8, void *scales, int64_t K, int
 
 /*
  * Gradients of ga_rms_norm from t (`sum`; x itself where there was no residual):
- *   grad_x = i (weight grad_y) - t i^3 mean(t weight grad_y) + grad_sum,  i = 1 / sqrt(mean(t^2) + eps)
+ *   grad_x = i (weight grad_y - t i mean(t i weight grad_y)) + grad_sum,  i = 1 / sqrt(mean(t^2) + eps)
  *   grad_weight = sum over rows of grad_y t i
  * grad_x is the gradient of x and of the residual alike; grad_sum (NULL: none) is what reaches t
  * from elsewhere.  grad_x may be grad_y or grad_sum itself.  Every sum is fp32; its order depends
