@@ -80,11 +80,11 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes, float *across) {
 enum { kNorm = 0, kNorm8 = 1, kCut8 = 2 };
 
 // WIDE: a workgroup per row, otherwise `lanes` (16, 32, 64) lanes of a wavefront.  NCH: groups of 8 a lane holds.
+// sum may be x or res, so these are not __restrict__: a group of both is read before its sum is stored.
 template <typename T, int NCH, bool WIDE, int MODE>
 __global__ __launch_bounds__(kBlock) void norm_kernel(
-    const T *__restrict__ x, const T *__restrict__ res, const T *__restrict__ w, T *__restrict__ y,
-    uint8_t *__restrict__ y8, uint8_t *__restrict__ scales, T *__restrict__ sum, int64_t rows, int cols,
-    int padded, float eps, int lanes) {
+    const T *x, const T *res, const T *__restrict__ w, T *__restrict__ y, uint8_t *__restrict__ y8,
+    uint8_t *__restrict__ scales, T *sum, int64_t rows, int cols, int padded, float eps, int lanes) {
   __shared__ float across[kBlock / kWave];
   const int lane = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (lanes - 1);
   const int64_t row = WIDE ? (int64_t)blockIdx.x
@@ -138,11 +138,12 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(
 
 // ---- gradients: each workgroup walks every gridDim-th set of rows and keeps grad_w's sums ----
 // 19,717 x 500 fp32: 26 us for 158 MB (6.0 TB/s), the sums of 1024 workgroups 4 us more; atomics on grad_w would
-// have needed zeros first and an order of their own at each run.
+// have needed zeros first and an order of their own at each run.  gx may be gy or gt, so these are not __restrict__: a
+// row of gy is read whole before any of gx is stored, a group of gt ahead of the store of the group before it.
 template <typename T, int NCH, bool WIDE>
 __global__ __launch_bounds__(kBlock) void norm_grad_kernel(
-    const T *__restrict__ gy, const T *__restrict__ t_in, const T *__restrict__ w, const T *__restrict__ gt,
-    T *__restrict__ gx, float *__restrict__ parts, int64_t rows, int cols, float eps, int lanes) {
+    const T *gy, const T *__restrict__ t_in, const T *__restrict__ w, const T *gt, T *gx, float *__restrict__ parts,
+    int64_t rows, int cols, float eps, int lanes) {
   __shared__ float across[kBlock / kWave];
   extern __shared__ float fold[];                      // WIDE: unused; else (kBlock / lanes, cols rounded up)
   const int lane = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (lanes - 1);
@@ -177,19 +178,20 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(
     const float inv = 1.0f / sqrtf(ss / cols + eps);
     const float mean = inv * (dot / cols);             // of y gy; the cube of inv alone may leave the range
     asm volatile("" : "+s"(end));
+    float o[2][kVec];
+    if (gt) load_group(gt + row * cols + lane * kVec, end - lane * kVec, o[0]);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = (lane + i * step) * kVec, n = end - c;
-      float o[kVec];
-      if (gt) load_group(gt + row * cols + c, n, o);
+      const int c = (lane + i * step) * kVec, behind = c + step * kVec;
+      if (gt && i + 1 < NCH) load_group(gt + row * cols + behind, end - behind, o[(i + 1) & 1]);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         const float unit = t[i][j] * inv;
         const float d = inv * (wv[i][j] * g[i][j] - unit * mean);
-        o[j] = gt ? o[j] + d : d;
+        o[i & 1][j] = gt ? o[i & 1][j] + d : d;
         gw[i][j] = fmaf(g[i][j], unit, gw[i][j]);
       }
-      store_group(gx + row * cols + c, n, o);
+      store_group(gx + row * cols + c, end - c, o[i & 1]);
     }
   }
   float *mine = parts + (int64_t)blockIdx.x * cols;

@@ -3,7 +3,7 @@ test_gpu_residual_norm.py."""
 import pytest
 import torch
 
-from graphiler_amd import ops
+from graphiler_amd import capi, ops
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16]
@@ -42,3 +42,39 @@ def test_gradients_of_rows_of_any_size(rows, cols, dtype, power, eps):
     within(gx, want, 4 * STEPS * size + (half_step + 2.0 ** -24) * want.abs())
     terms = (g * t * inv).abs().sum(0)
     within(gw, (g * t * inv).sum(0), (rows * 2.0 ** -24 + 2 * STEPS) * terms + half_step * terms)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(33, 100), (9, 500), (7, 1000), (5, 2000), (5, 4096), (4, 7000), (3, 16384)])
+def test_results_in_place_of_operands(rows, cols, dtype):
+    """sum over x or over the residual, grad_x over grad_y or over grad_sum: the same bits as beside them."""
+    lib, stream = capi.load(), torch.cuda.current_stream().cuda_stream
+    dt = capi.GA_F32 if dtype == torch.float32 else capi.GA_BF16
+    x, r, w, gy = make(cols, rows, cols, dtype)
+    y, t = ops.rms_norm(x, w, r, EPS)
+    y8, scales, _ = ops.rms_norm_fp8(x, w, r, EPS)
+    for over in ("x", "residual"):
+        a, b = x.clone(), r.clone()
+        total, mine = a if over == "x" else b, torch.empty_like(y)
+        assert lib.ga_rms_norm(a.data_ptr(), b.data_ptr(), w.data_ptr(), mine.data_ptr(), total.data_ptr(), rows, cols,
+                               EPS, dt, stream) == 0
+        assert torch.equal(mine, y) and torch.equal(total, t)
+        a, b = x.clone(), r.clone()
+        total, mine8, mine_scales = a if over == "x" else b, torch.empty_like(y8), torch.empty_like(scales)
+        assert lib.ga_rms_norm_fp8(a.data_ptr(), b.data_ptr(), w.data_ptr(), mine8.data_ptr(), mine_scales.data_ptr(),
+                                   total.data_ptr(), rows, cols, EPS, dt, stream) == 0
+        assert torch.equal(total, t) and torch.equal(mine8.view(torch.uint8), y8.view(torch.uint8))
+        assert torch.equal(mine_scales.view(torch.uint8), scales.view(torch.uint8))
+    n = lib.ga_rms_norm_backward_workspace_bytes(rows, cols)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    for gt in (None, r):
+        gx, gw = ops.rms_norm_backward(gy, t, w, EPS, gt)
+        for over in ("grad_y", "grad_sum"):
+            if gt is None and over == "grad_sum":
+                continue
+            a, b, mine = gy.clone(), None if gt is None else gt.clone(), torch.empty_like(gw)
+            out = a if over == "grad_y" else b
+            assert lib.ga_rms_norm_backward(a.data_ptr(), t.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(),
+                                            out.data_ptr(), mine.data_ptr(), rows, cols, EPS, dt, ws.data_ptr(), n,
+                                            stream) == 0
+            assert torch.equal(out, gx) and torch.equal(mine, gw)
