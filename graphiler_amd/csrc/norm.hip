@@ -121,6 +121,11 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(
     if constexpr (MODE == kNorm) {
       store_group(y + row * cols + c, n, t[i]);
     } else {
+      if (MODE == kNorm8 && n < kVec) {                // zeros behind cols also where the root is not finite
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          if (j >= n) t[i][j] = 0.0f;
+      }
       float top = 0.0f;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) top = fmaxf(top, finite_size(t[i][j]));

@@ -78,3 +78,16 @@ def test_results_in_place_of_operands(rows, cols, dtype):
                                             out.data_ptr(), mine.data_ptr(), rows, cols, EPS, dt, ws.data_ptr(), n,
                                             stream) == 0
             assert torch.equal(out, gx) and torch.equal(mine, gw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [1, 100, 129, 300, 1000, 2047, 5001])
+def test_zeros_behind_rows_that_are_not_finite(cols, dtype):
+    x, r, w, _ = make(cols, 4, cols, dtype)
+    x[1, 0], x[2, cols - 1], x[3], r[3] = float("nan"), float("inf"), 0.0, 0.0
+    for residual in (None, r):
+        y8, scales = ops.rms_norm_fp8(x, w, residual, eps=0.0)[:2]
+        assert bool((y8[:, cols:].view(torch.uint8) == 0).all())
+        y = ops.rms_norm(x, w, residual, eps=0.0)
+        y = y if residual is None else y[0]
+        assert torch.equal(torch.isnan(y8[:, :cols].float()), ~torch.isfinite(y))
