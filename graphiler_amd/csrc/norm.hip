@@ -25,7 +25,8 @@ namespace ga {
 namespace {
 
 constexpr int kScaleBlock = 128;         // values that share a scale
-constexpr int kMaxCols = 16384;          // a block of 256 lanes with eight groups each
+constexpr int kMaxCols = 16384;          // of a norm: a block of 256 lanes with eight groups each
+constexpr int kMaxCutCols = 32768;       // of rows that are only cut, as wide as the 8-bit products take them
 
 __device__ __forceinline__ bool finite(float f) {
   return (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u;
@@ -291,7 +292,8 @@ RowShape row_shape(int64_t cols) {
   if (cols <= 2048) return {true, kBlock, 1};
   if (cols <= 4096) return {true, kBlock, 2};
   if (cols <= 8192) return {true, kBlock, 4};
-  return {true, kBlock, 8};
+  if (cols <= 16384) return {true, kBlock, 8};
+  return {true, kBlock, 16};
 }
 
 template <typename T, int MODE>
@@ -312,7 +314,9 @@ int norm_launch(const void *x, const void *res, const void *w, void *y, void *y8
     if (r.nch == 1) GA_NORM(1, true);
     else if (r.nch == 2) GA_NORM(2, true);
     else if (r.nch == 4) GA_NORM(4, true);
-    else GA_NORM(8, true);
+    else if (r.nch == 8) GA_NORM(8, true);
+    else if constexpr (MODE == kCut8) GA_NORM(16, true);
+    else return GA_EUNSUPPORTED;
   }
 #undef GA_NORM
   return launch_status();
@@ -354,10 +358,10 @@ int grad_launch(const void *gy, const void *t, const void *w, const void *gt, vo
   return launch_status();
 }
 
-int check_rows(int64_t rows, int64_t cols, int dtype) {
+int check_rows(int64_t rows, int64_t cols, int dtype, int64_t most = kMaxCols) {
   if (rows < 0 || cols <= 0) return GA_EINVAL;
   if (dtype != GA_F32 && dtype != GA_BF16) return GA_EUNSUPPORTED;
-  if (cols > kMaxCols) return GA_EUNSUPPORTED;
+  if (cols > most) return GA_EUNSUPPORTED;
   return GA_OK;
 }
 bool elem_aligned(int dtype, const void *a, const void *b, const void *c, const void *d, const void *e) {
@@ -399,7 +403,7 @@ int ga_rms_norm_fp8(const void *x, const void *residual, const void *weight, voi
 int ga_quantize_fp8(const void *x, void *x8, void *scales, int64_t rows, int64_t cols, int dtype,
                     ga_stream_t stream) {
   using namespace ga;
-  if (int rc = check_rows(rows, cols, dtype)) return rc;
+  if (int rc = check_rows(rows, cols, dtype, kMaxCutCols)) return rc;
   if (rows == 0) return GA_OK;
   if (!x || !x8 || !scales) return GA_EINVAL;
   if (!elem_aligned(dtype, x, nullptr, nullptr, nullptr, nullptr) || !aligned(x8, 16)) return GA_EALIGN;

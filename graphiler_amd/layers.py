@@ -270,6 +270,8 @@ def _in_8_bits(*weights) -> bool:
 
 
 def _feed_forward_fp8(rows, w_gate, w_up, w_down, activation, out_dtype):
+    if w_down[0].shape[1] > ops.FP8_MAX_COLS:
+        raise RuntimeError(f"w_down in 8 bits must have at most {ops.FP8_MAX_COLS} rows")
     hidden = ops.gated_linear_fp8(*rows, *w_gate, *w_up, activation=activation, out_dtype=out_dtype)
     return ops.linear_fp8(*ops.quantize_fp8(hidden), *w_down, out_dtype=out_dtype)
 

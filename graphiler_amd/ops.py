@@ -1409,6 +1409,7 @@ def linear_attn(x, weight, a_l=None, a_r=None):
 _GATES = {"silu": capi.GA_GATE_SILU, "gelu": capi.GA_GATE_GELU, "relu": capi.GA_GATE_RELU}
 FP8_BLOCK = 128          # values of a row, and rows and columns of a weight, that share a scale
 RMS_NORM_MAX_COLS = 16384
+FP8_MAX_COLS = 32768     # of rows in 8 bits, and of what an 8-bit product adds up
 
 
 def _gate(name) -> int:
@@ -1571,8 +1572,8 @@ def quantize_fp8(x):
     _no_grad_form("quantize_fp8", x)
     dt = _check_rows(x, "x")
     rows, cols = int(x.shape[0]), int(x.shape[1])
-    if cols > RMS_NORM_MAX_COLS:
-        raise RuntimeError(f"x must have at most {RMS_NORM_MAX_COLS} columns")
+    if cols > FP8_MAX_COLS:
+        raise RuntimeError(f"x must have at most {FP8_MAX_COLS} columns")
     x8, scales = _rows_8bit(rows, cols, x.device)
     _launch("ga_quantize_fp8", x.get_device(), x.data_ptr(), x8.data_ptr(), scales.data_ptr(), rows, cols, dt)
     return x8, scales

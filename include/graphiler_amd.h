@@ -780,7 +780,10 @@ int ga_rms_norm(const void *x, const void *residual, const void *weight, void *y
 int ga_rms_norm_fp8(const void *x, const void *residual, const void *weight, void *y8, void *scales,
                     void *sum, int64_t rows, int64_t cols, float eps, int dtype, ga_stream_t stream);
 
-/* Rows x (rows, cols) of `dtype` cut to 8 bits: x8 and scales as ga_rms_norm_fp8 writes them. */
+/*
+ * Rows x (rows, cols) of `dtype` cut to 8 bits: x8 and scales as ga_rms_norm_fp8 writes them.
+ * GA_EUNSUPPORTED when cols > 32768, the widest rows that ga_linear_fp8 takes.
+ */
 int ga_quantize_fp8(const void *x, void *x8, void *scales, int64_t rows, int64_t cols, int dtype,
                     ga_stream_t stream);
 

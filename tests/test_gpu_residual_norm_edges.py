@@ -3,7 +3,7 @@ test_gpu_residual_norm.py."""
 import pytest
 import torch
 
-from graphiler_amd import capi, ops
+from graphiler_amd import capi, layers, ops
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16]
@@ -91,3 +91,39 @@ def test_zeros_behind_rows_that_are_not_finite(cols, dtype):
         y = ops.rms_norm(x, w, residual, eps=0.0)
         y = y if residual is None else y[0]
         assert torch.equal(torch.isnan(y8[:, :cols].float()), ~torch.isfinite(y))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [16385, 20001, 32640, 32768])
+def test_rows_as_wide_as_the_8_bit_products_are_cut(cols, dtype):
+    """Blocks of 128 are cut by themselves: the same bits as two narrower halves."""
+    x = make(cols, 3, cols, dtype)[0]
+    x[1, cols - 1] = float("inf")
+    x8, scales = ops.quantize_fp8(x)
+    assert x8.shape == (3, -(-cols // 128) * 128) and scales.shape == (3, -(-cols // 128))
+    for part in (slice(0, 16384), slice(16384, cols)):
+        a8, a_scales = ops.quantize_fp8(x[:, part].contiguous())
+        blocks = slice(part.start // 128, part.start // 128 + a_scales.shape[1])
+        assert torch.equal(x8[:, part.start:part.start + a8.shape[1]].view(torch.uint8), a8.view(torch.uint8))
+        assert torch.equal(scales[:, blocks].view(torch.uint8), a_scales.view(torch.uint8))
+
+
+def test_a_block_as_wide_as_the_8_bit_products():
+    gen = torch.Generator().manual_seed(5)
+    for f in (16385, 32768):
+        x = torch.randn(5, 64, generator=gen).cuda()
+        w = [torch.randn(64, f, generator=gen).cuda() / 8 for _ in range(2)] + [torch.randn(f, 32, generator=gen).cuda() / f ** 0.5]
+        w8 = [ops.quantize_weight_fp8(t) for t in w]
+        got = layers.feed_forward(x, *w8)
+        hidden = ops.gated_linear_fp8(*ops.quantize_fp8(x), *w8[0], *w8[1], out_dtype=torch.float32)
+
+        def held(values, scales, rows_each):             # what the 8 bits stand for
+            s = torch.exp2(scales.view(torch.uint8).double() - 127).repeat_interleave(rows_each, 0)[:values.shape[0]]
+            return values.double() * s.repeat_interleave(128, 1)
+
+        h, down = held(*ops.quantize_fp8(hidden), 1), held(*w8[2], 128)
+        want, size = h @ down.t(), h.abs() @ down.t().abs()
+        # of eight products what is 2^-13 below the largest is dropped, then f sums in fp32, one rounding
+        assert ((got.double() - want).abs() <= (2.0 ** -10 + f * 2.0 ** -24) * size + 2.0 ** -24 * want.abs()).all()
+        with pytest.raises(RuntimeError, match="at most 32768 columns"):
+            ops.quantize_fp8(torch.zeros(1, 32769, device="cuda"))
