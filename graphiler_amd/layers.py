@@ -288,9 +288,8 @@ def hgt_block(g: DGLGraph, h, norm_attention, attention, norm_ff, ff, heads: int
     three of :func:`feed_forward`, as tensors or in 8 bits.  The addition in front of the second
     norm is the norm kernel's, and with weights in 8 bits it writes the rows in 8 bits too.  Not
     differentiable, as the layer is not."""
-    if torch.is_grad_enabled() and any(
-            isinstance(t, torch.Tensor) and t.requires_grad for t in (h, norm_attention, *attention, norm_ff, *ff)):
-        raise RuntimeError("hgt_block has no gradient: call it under torch.no_grad()")
+    ops._no_grad_form("hgt_block", *(t for t in (h, norm_attention, *attention, norm_ff, *ff)
+                                     if isinstance(t, torch.Tensor)))
     in_8_bits = _in_8_bits(*ff)
     a = hgt_layer(g, ops.rms_norm(h, norm_attention, eps=eps), *attention, heads=heads, fused=fused)
     if in_8_bits:

@@ -1443,7 +1443,22 @@ def _wants_grad(*tensors) -> bool:
     return False
 
 
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
+def _check_seen(what: str, *tensors) -> None:
+    """What follows a tensor's operators without requires_grad, a tangent or a trace, does not see a
+    kernel: its result would have no tangent, or come back unwritten from every later call."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative")
+    if _tracing():
+        raise RuntimeError(f"{what} cannot be traced")
+
+
 def _no_grad_form(what: str, *tensors) -> None:
+    _check_seen(what, *tensors)
     if _wants_grad(*tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
@@ -1525,7 +1540,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6):
     y = t / sqrt(mean(t^2) + eps) * weight for (rows, cols) features and a (cols,) weight of the
     same dtype.  Returns y, or (y, t) with a residual: t is the stream that the next addition
     takes.  t is summed and squared in fp32 and rounded only where it is stored.  Differentiable in x, weight
-    and residual."""
+    and residual (backward mode)."""
+    _check_seen("rms_norm", x, weight, residual)
     if _wants_grad(x, weight, residual):
         return _RmsNorm.apply(x, weight, residual, eps)
     return _rms_norm(x, weight, residual, eps)
@@ -1534,7 +1550,9 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6):
 def rms_norm_backward(grad_y, total, weight, eps: float = 1e-6, grad_sum=None):
     """Gradients of :func:`rms_norm`: ``total`` is the t it returned (x itself without a
     residual), ``grad_sum`` what reaches t from elsewhere (None: nothing).  Returns
-    (gradient of x and of the residual alike, gradient of weight)."""
+    (gradient of x and of the residual alike, gradient of weight), which have no gradients of
+    their own."""
+    _check_seen("rms_norm_backward", grad_y, total, weight, grad_sum)
     dt, rows, cols = _norm_args(total, weight, None, eps)
     _check_like(grad_y, "grad_y", total.shape, total)
     if grad_sum is not None:
@@ -1617,7 +1635,9 @@ def _out_8bit(x8, m: int, out_dtype):
 
 def linear_fp8(x8, x_scales, w8, w_scales, out_dtype=torch.bfloat16):
     """x @ weight for rows and a weight in 8 bits (:func:`quantize_fp8` or :func:`rms_norm_fp8`,
-    :func:`quantize_weight_fp8`): (rows, M) of ``out_dtype``, accumulated in fp32."""
+    :func:`quantize_weight_fp8`): (rows, M) of ``out_dtype``, accumulated in fp32.  Not
+    differentiable."""
+    _no_grad_form("linear_fp8", x8, x_scales, w8, w_scales)
     _check_8bit(x8, x_scales, "x8", x8.get_device(), 1)
     k = int(x8.shape[1])
     _check_8bit(w8, w_scales, "w8", x8.get_device(), FP8_BLOCK, k)
@@ -1631,7 +1651,8 @@ def linear_fp8(x8, x_scales, w8, w_scales, out_dtype=torch.bfloat16):
 def gated_linear_fp8(x8, x_scales, wg8, wg_scales, wu8, wu_scales, activation: str = "silu",
                      out_dtype=torch.bfloat16):
     """:func:`gated_linear` for rows and weights in 8 bits: act(x @ w_gate) * (x @ w_up) from one
-    kernel."""
+    kernel.  Not differentiable."""
+    _no_grad_form("gated_linear_fp8", x8, x_scales, wg8, wg_scales, wu8, wu_scales)
     act = _gate(activation)
     _check_8bit(x8, x_scales, "x8", x8.get_device(), 1)
     k = int(x8.shape[1])
@@ -1692,6 +1713,7 @@ def gated_linear(x, w_gate, w_up, activation: str = "silu"):
     "silu" | "gelu" (with the error function) | "relu".  Sums in fp32, one rounding; fp32
     products are those of :func:`linear_attn`, or the fp32 instruction's where that is faster (few
     rows, columns or tiles).  A bf16 tensor whose rows are whole 16-byte pieces has to begin at one.  Differentiable in all three."""
+    _check_seen("gated_linear", x, w_gate, w_up)
     if _wants_grad(x, w_gate, w_up):
         return _GatedLinear.apply(x, w_gate, w_up, activation)
     return _gated_linear(x, w_gate, w_up, activation)
@@ -1699,7 +1721,9 @@ def gated_linear(x, w_gate, w_up, activation: str = "silu"):
 
 def gated_linear_backward(grad_h, x, w_gate, w_up, activation: str = "silu"):
     """Gradients of :func:`gated_linear`: (of x, of w_gate, of w_up).  Both products are formed
-    again; nothing but the operands is kept from the forward pass."""
+    again; nothing but the operands is kept from the forward pass.  The results have no gradients
+    of their own."""
+    _check_seen("gated_linear_backward", grad_h, x, w_gate, w_up)
     act = _gate(activation)
     dt, rows, k, f = _gated_args(x, w_gate, w_up)
     _check_like(grad_h, "grad_h", (rows, f), x)
