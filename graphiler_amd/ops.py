@@ -1712,7 +1712,9 @@ def gated_linear(x, w_gate, w_up, activation: str = "silu"):
     (:func:`linear` is the other).  x (rows, K), w_gate and w_up (K, F) of one dtype; activation
     "silu" | "gelu" (with the error function) | "relu".  Sums in fp32, one rounding; fp32
     products are those of :func:`linear_attn`, or the fp32 instruction's where that is faster (few
-    rows, columns or tiles).  A bf16 tensor whose rows are whole 16-byte pieces has to begin at one.  Differentiable in all three."""
+    rows, columns or tiles); an fp32 operand that is not finite gives infinities and NaN as the
+    definition does with the latter, NaN with the former.  A bf16 tensor whose rows are whole 16-byte
+    pieces has to begin at one.  Differentiable in all three (backward mode)."""
     _check_seen("gated_linear", x, w_gate, w_up)
     if _wants_grad(x, w_gate, w_up):
         return _GatedLinear.apply(x, w_gate, w_up, activation)
