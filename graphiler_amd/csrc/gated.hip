@@ -361,13 +361,14 @@ int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h
   if (int rc = check_gated(rows, K, F, activation, dtype)) return rc;
   if (rows == 0) return GA_OK;
   if (!x || !w_gate || !w_up || !h) return GA_EINVAL;
-  if (!operand_aligned(x, K, dtype) || !operand_aligned(w_gate, F, dtype) || !operand_aligned(w_up, F, dtype) ||
-      !aligned(h, dtype == GA_F32 ? 4 : 2))
-    return GA_EALIGN;
-  if (rows <= kGatedFewRows)
+  const size_t e = dtype == GA_F32 ? 4 : 2;
+  if (!aligned(x, e) || !aligned(w_gate, e) || !aligned(w_up, e) || !aligned(h, e)) return GA_EALIGN;
+  if (rows <= kGatedFewRows)             // takes any address
     return gated_few_launch(x, w_gate, w_up, h, rows, K, F, activation, dtype, (hipStream_t)stream);
   if (dtype == GA_F32 && gated_f32_taken(rows, K, F))
     return gated_f32_launch(x, w_gate, w_up, h, rows, K, F, activation, (hipStream_t)stream);
+  if (!operand_aligned(x, K, dtype) || !operand_aligned(w_gate, F, dtype) || !operand_aligned(w_up, F, dtype))
+    return GA_EALIGN;
   const Plan p = plan_of(rows, K, F, dtype, false);
   if (p.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return GA_EWORKSPACE;
   hipStream_t s = (hipStream_t)stream;

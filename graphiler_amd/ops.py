@@ -1680,6 +1680,11 @@ def _gated_args(x, w_gate, w_up):
     return dt, rows, k, f
 
 
+def _whole_pieces(t):
+    """Where few rows of bf16 may begin anywhere, their gradients take whole 16-byte pieces."""
+    return t.clone() if t.data_ptr() % 16 and t.dtype is torch.bfloat16 and t.shape[1] % 8 == 0 else t
+
+
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, activation):
@@ -1693,7 +1698,8 @@ class _GatedLinear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_h):
         _not_recorded("gated_linear")
-        return (*gated_linear_backward(grad_h.contiguous(), *ctx.saved_tensors, ctx.activation), None)
+        operands = (_whole_pieces(t) for t in ctx.saved_tensors)
+        return (*gated_linear_backward(grad_h.contiguous(), *operands, ctx.activation), None)
 
 
 def _gated_linear(x, w_gate, w_up, activation):
@@ -1713,8 +1719,9 @@ def gated_linear(x, w_gate, w_up, activation: str = "silu"):
     "silu" | "gelu" (with the error function) | "relu".  Sums in fp32, one rounding; fp32
     products are those of :func:`linear_attn`, or the fp32 instruction's where that is faster (few
     rows, columns or tiles); an fp32 operand that is not finite gives infinities and NaN as the
-    definition does with the latter, NaN with the former.  A bf16 tensor whose rows are whole 16-byte
-    pieces has to begin at one.  Differentiable in all three (backward mode)."""
+    definition does with the latter, NaN with the former.  With more than 16 rows (and in
+    :func:`gated_linear_backward` always) a bf16 tensor whose rows are whole 16-byte pieces has to
+    begin at one.  Differentiable in all three (backward mode)."""
     _check_seen("gated_linear", x, w_gate, w_up)
     if _wants_grad(x, w_gate, w_up):
         return _GatedLinear.apply(x, w_gate, w_up, activation)

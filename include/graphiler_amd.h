@@ -814,7 +814,8 @@ int ga_rms_norm_backward(const void *grad_y, const void *sum, const void *weight
  * (silu: g / (1 + exp(-g)); gelu with the error function; relu).  fp32 products are formed from bf16
  * pieces as in ga_linear_attn (less than 2^-22 of a product is left out; inputs that are not finite
  * give NaN, operands below 2^-110 lose bits) or, where that is faster (few rows, columns or tiles), by
- * the fp32 instruction.  bf16 tensors whose rows are whole 16-byte pieces have to be 16-byte aligned.  GA_EUNSUPPORTED when K or F exceeds 2^20.
+ * the fp32 instruction.  With more than 16 rows, bf16 operands whose rows are whole 16-byte pieces have to
+ * be 16-byte aligned.  GA_EUNSUPPORTED when K or F exceeds 2^20.
  */
 enum ga_gate { GA_GATE_SILU = 0, GA_GATE_GELU = 1, GA_GATE_RELU = 2 };
 size_t ga_gated_linear_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype);
@@ -826,7 +827,8 @@ int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h
  * Its gradients: with gate = x @ w_gate, up = x @ w_up (formed again), du = grad_h act(gate),
  * dg = grad_h up act'(gate) (both rounded to bf16 where the tensors are bf16):
  *   grad_x = dg @ w_gate^T + du @ w_up^T, grad_gate = x^T @ dg, grad_up = x^T @ du.
- * The slope of relu at 0 is 0.  fp32 products are those of pieces.  No order of a sum depends on anything but the sizes.
+ * The slope of relu at 0 is 0.  fp32 products are those of pieces.  No order of a sum depends on
+ * anything but the sizes.  bf16 operands whose rows are whole 16-byte pieces have to be 16-byte aligned.
  */
 size_t ga_gated_linear_backward_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype);
 int ga_gated_linear_backward(const void *grad_h, const void *x, const void *w_gate, const void *w_up,

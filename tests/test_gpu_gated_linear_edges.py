@@ -72,3 +72,26 @@ def test_operands_at_any_address(rows, k, f, dtype):
     for a, b in zip(ops.gated_linear_backward(moved(gh), moved(x), moved(wg), moved(wu)),
                     ops.gated_linear_backward(gh, x, wg, wu)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,f", [(1, 64, 64), (9, 256, 512), (16, 1024, 136)])
+def test_few_rows_at_any_address(rows, k, f, dtype):
+    """Rows that are whole 16-byte pieces too, as long as there are few."""
+    x, wg, wu, _ = make(rows + f, rows, k, f, dtype)
+    want = ops.gated_linear(x, wg, wu)
+    for i in range(3):
+        args = [x, wg, wu]
+        args[i] = moved(args[i])
+        assert torch.equal(ops.gated_linear(*args), want)
+    gh = torch.randn_like(want)
+    leaves = [moved(t).requires_grad_() for t in (x, wg, wu)]
+    got = torch.autograd.grad(ops.gated_linear(*leaves), leaves, moved(gh))
+    for a, b in zip(got, ops.gated_linear_backward(gh, x, wg, wu)):
+        assert torch.equal(a, b)
+    x = make(1, 17, k, f, dtype)[0]
+    if dtype == torch.bfloat16:
+        with pytest.raises(RuntimeError, match="(?i)align"):
+            ops.gated_linear(moved(x), wg, wu)
+    else:
+        assert torch.equal(ops.gated_linear(moved(x), wg, wu), ops.gated_linear(x, wg, wu))
