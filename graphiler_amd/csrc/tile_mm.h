@@ -167,15 +167,11 @@ __device__ __forceinline__ void tile_of(int id, int n_tiles, int row_tiles, int 
   tc = __builtin_amdgcn_readfirstlane(in / high);
 }
 
-// All but the youngest N loads of this wavefront have arrived.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(N < 64, "six bits");
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
-}
-// ... of every wavefront, and every wavefront has what it read or written in LDS behind it.
+// All but the youngest N loads of every wavefront have arrived, and every wavefront has what it read or written in LDS
+// behind it.
 template <int N>
 __device__ __forceinline__ void landed() {
+  static_assert(N < 64, "six bits");
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
   __builtin_amdgcn_s_barrier();
