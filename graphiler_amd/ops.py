@@ -1435,7 +1435,22 @@ def _check_like(x, name: str, shape, like) -> None:
         raise RuntimeError(f"{name} must be {tuple(shape)}, of the dtype and on the device of the rows")
 
 
-def _wants_grad(*tensors) -> bool:
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
+def _check_seen(what: str, *tensors) -> None:
+    """What follows a tensor's operators without requires_grad, a tangent or a trace, does not see a
+    kernel: its result would have no tangent, or come back unwritten from every later call."""
+    if _tracing():
+        raise RuntimeError(f"{what} cannot be traced")
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
+def _wants_grad(what: str, *tensors) -> bool:
+    _check_seen(what, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -1443,23 +1458,8 @@ def _wants_grad(*tensors) -> bool:
     return False
 
 
-_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
-
-
-def _check_seen(what: str, *tensors) -> None:
-    """What follows a tensor's operators without requires_grad, a tangent or a trace, does not see a
-    kernel: its result would have no tangent, or come back unwritten from every later call."""
-    if getattr(forward_ad, "_current_level", 0) >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{what} has no forward-mode derivative")
-    if _tracing():
-        raise RuntimeError(f"{what} cannot be traced")
-
-
 def _no_grad_form(what: str, *tensors) -> None:
-    _check_seen(what, *tensors)
-    if _wants_grad(*tensors):
+    if _wants_grad(what, *tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
@@ -1541,8 +1541,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6):
     same dtype.  Returns y, or (y, t) with a residual: t is the stream that the next addition
     takes.  t is summed and squared in fp32 and rounded only where it is stored.  Differentiable in x, weight
     and residual (backward mode)."""
-    _check_seen("rms_norm", x, weight, residual)
-    if _wants_grad(x, weight, residual):
+    if _wants_grad("rms_norm", x, weight, residual):
         return _RmsNorm.apply(x, weight, residual, eps)
     return _rms_norm(x, weight, residual, eps)
 
@@ -1637,7 +1636,7 @@ def linear_fp8(x8, x_scales, w8, w_scales, out_dtype=torch.bfloat16):
     """x @ weight for rows and a weight in 8 bits (:func:`quantize_fp8` or :func:`rms_norm_fp8`,
     :func:`quantize_weight_fp8`): (rows, M) of ``out_dtype``, accumulated in fp32.  Not
     differentiable."""
-    _no_grad_form("linear_fp8", x8, x_scales, w8, w_scales)
+    _no_grad_form("linear_fp8", x8, w8)
     _check_8bit(x8, x_scales, "x8", x8.get_device(), 1)
     k = int(x8.shape[1])
     _check_8bit(w8, w_scales, "w8", x8.get_device(), FP8_BLOCK, k)
@@ -1652,7 +1651,7 @@ def gated_linear_fp8(x8, x_scales, wg8, wg_scales, wu8, wu_scales, activation: s
                      out_dtype=torch.bfloat16):
     """:func:`gated_linear` for rows and weights in 8 bits: act(x @ w_gate) * (x @ w_up) from one
     kernel.  Not differentiable."""
-    _no_grad_form("gated_linear_fp8", x8, x_scales, wg8, wg_scales, wu8, wu_scales)
+    _no_grad_form("gated_linear_fp8", x8, wg8, wu8)
     act = _gate(activation)
     _check_8bit(x8, x_scales, "x8", x8.get_device(), 1)
     k = int(x8.shape[1])
@@ -1722,8 +1721,7 @@ def gated_linear(x, w_gate, w_up, activation: str = "silu"):
     definition does with the latter, NaN with the former.  With more than 16 rows (and in
     :func:`gated_linear_backward` always) a bf16 tensor whose rows are whole 16-byte pieces has to
     begin at one.  Differentiable in all three (backward mode)."""
-    _check_seen("gated_linear", x, w_gate, w_up)
-    if _wants_grad(x, w_gate, w_up):
+    if _wants_grad("gated_linear", x, w_gate, w_up):
         return _GatedLinear.apply(x, w_gate, w_up, activation)
     return _gated_linear(x, w_gate, w_up, activation)
 
