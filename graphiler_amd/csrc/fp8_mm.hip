@@ -2,12 +2,12 @@
 // scale for every 128 values of a row of x and for every 128 x 128 values of w, and the gated form
 // act(x wg^T) * (x wu^T) of a feed-forward block.
 //
-// v_mfma_scale_f32_16x16x128_f8f6f4 takes 128 values of k at a time, exactly a block, and
-// multiplies by both scales itself: the products of all blocks add up in one fp32 accumulator with no
+// v_mfma_scale_f32_16x16x128_f8f6f4 (few rows) takes 128 values of k at a time, exactly a block, v_mfma_scale_f32_32x32x64
+// (tiles) half of one, and both multiply by both scales themselves: the products of all blocks add up in one fp32 accumulator with no
 // other instruction, at twice the rate of bf16.  Of every eight products that the instruction adds
 // first it keeps what lies within 2^-13 of the largest (measured); everything after that is fp32.
-// 16,384 x 4096 x 4096: 211 us, 2.61 PFLOP/s (vendor's, with one scale for all, 181); 19,717 x 256 -> 2 x 1000, two steps
-// of k, 28 us, of which 8-10 are the activation's instructions and the rest the five rounds of short workgroups.
+// 16,384 x 4096 x 4096: 215 us, 2.56 PFLOP/s (vendor's, with one scale for all, 181); 19,717 x 256 -> 2 x 1000, two steps
+// of k, 29-31 us, of which 8-10 are the activation's instructions and the rest the five rounds of short workgroups.
 #include "tile_mm.h"
 #include "vec8.h"
 

@@ -14,8 +14,8 @@
 // that are not finite give NaN, operands below 2^-110 lose bits).  The pieces are laid out once a
 // call, as are operands whose rows are not whole 16-byte pieces.
 //
-// Measured, bf16, K = 1024, F = 4096: 16,384 rows 228 us (1.20 PFLOP/s), gradients of 8,192 rows 378 us: dg and du
-// 145-155 (both products and 201 MB), grad_x 121, the weights' 122.  fp32, 4,096 x 256 -> 1024: 35 us, gradients
+// Measured, bf16, K = 1024, F = 4096: 16,384 rows 229 us (1.20 PFLOP/s), gradients of 8,192 rows 383 us: dg and du
+// 149-158 (both products and 201 MB), grad_x and the weights' 124-127 each.  fp32, 4,096 x 256 -> 1024: 37 us, gradients
 // of 2,001 x 300 -> 700: 28 + 22 + 22, 12 to add up parts, 5 to lay out.  At most 16 rows: gated_few.hip; fp32
 // products of few tiles: gated_f32.hip.
 #include "gated_few.h"

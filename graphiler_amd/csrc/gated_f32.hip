@@ -153,7 +153,7 @@ static int64_t f32_tiles(int64_t rows, int64_t F, int64_t tile_rows) {
   return tiles_of(rows, F, (int)tile_rows, kF32Cols);
 }
 
-// Against the pieces, us (pieces | here): 2708 x 128 -> 341 15.4 | 10.3, x 1024 73 | 55; 1000 x 512 -> 512 29 | 14.5;
+// Against the pieces, us a call repeated, silu (pieces | here; gelu 0.5 more): 2708 x 128 -> 341 15.4 | 10.3, x 1024 73 | 55; 1000 x 512 -> 512 29 | 14.5;
 // 17 x 1024 -> 1024 51 | 17.  At 704 tiles (2048 -> 704) K = 32 13.6 | 10.1, 512 36.9 | 35.7, 2048 115 | 130; at 968
 // 32 13.8 | 11.5, 128 16.2 | 15.7, 512 39 | 45; at 1408 14.0 | 16.5, 20 | 22, 49 | 65.  To few columns the pieces of x cost more than
 // their product saves: 20,000 -> 64 K = 128 23 | 12.4, 40,000 -> 64 K = 512 74 | 57.

@@ -1,8 +1,8 @@
 // act(x Wg) * (x Wu) for few rows of x: a query that is answered by itself.  All there is to do is
 // to read both weights once, with enough of them on their way: 64 columns a workgroup (128 or 256
 // bytes of a weight's row), its wavefronts take turns along k and add up what they have in
-// LDS, in their order.  Three rows, 1024 to 4096, bf16 (16.8 MB): 5.7 us, 2.9 TB/s; a wavefront that
-// read 64 of k of both weights and then multiplied took 10.2.
+// LDS, in their order.  Three rows, 1024 to 4096, bf16 (16.8 MB): 4.7 us recorded in a graph (3.6 TB/s), 5.4-7.3 in
+// traces; a wavefront that read 64 of k of both weights and then multiplied took 10.2 there.
 //
 // bf16 on v_mfma_f32_16x16x32_bf16.  A lane reads 16 bytes of eight rows of W, k = 8 (lane / 8) ... + 7 of 64,
 // columns 8 (lane % 8) ... + 7, and turns that 8 x 8 block in registers: for every column of it one

@@ -18,9 +18,9 @@
 // The matrix instruction is given B as its first operand: a lane then holds four adjacent columns
 // of one row of C.
 //
-// Bound by the matrix instructions where there are many steps, 16,384 x 1024 x 2 x 4096 in bf16 228 us (1.20 PFLOP/s; the
-// vendor's plain product of this size 251) and 16,384 x 4096 x 4096 in 8 bits 211 us (2.61 PFLOP/s); they are busy .55 of
-// the time, at the clock that the power leaves.  What it was before: steps of 64 bytes with three or four buffers 287-302
+// Bound by the matrix instructions where there are many steps, 16,384 x 1024 x 2 x 4096 in bf16 229 us (1.20 PFLOP/s; the
+// vendor's plain product of this size 251) and 16,384 x 4096 x 4096 in 8 bits 215 us (2.56 PFLOP/s); they are busy .58 and
+// .65 of the time, at the clock that the power leaves.  What it was before: steps of 64 bytes with three or four buffers 287-302
 // and 285 (half a line a row, bank conflicts in a third of the reads), moves and stores not dealt out between products 262
 // and 259.  With few steps (K of 128 or 256) a tile is bound by what surrounds them: its arguments, the
 // first loads' latency and the activation, 4 us a round of 512 workgroups.
