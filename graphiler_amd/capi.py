@@ -152,6 +152,13 @@ SIGNATURES = {
     "ga_gated_linear_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int,
                                         _int, _vp, _sz, _vp]),
     "ga_linear_fp8": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "ga_segment_attention_workspace_bytes": (_sz, [_i64] * 6 + [_int]),
+    "ga_segment_attention": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp,
+                                    _i64, _i64, _i64, _i64, _i64, _int, ctypes.c_float, _int, _vp, _sz, _vp]),
+    "ga_segment_attention_backward_workspace_bytes": (_sz, [_i64] * 6 + [_int]),
+    "ga_segment_attention_backward": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+                                             _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int,
+                                             ctypes.c_float, _int, _vp, _sz, _vp]),
     "ga_gated_linear_fp8": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int,
                                    _vp]),
 }

@@ -1,0 +1,396 @@
+// Gradients of attention inside segments, from the log-sum-exps that the forward pass left:
+//
+//   p_ij = exp(s_ij - lse_i), delta_i = <do_i, o_i>, ds_ij = p_ij (<do_i, v_j> - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i
+//
+// Two passes, each over 32 x 32 tiles that never leave the registers: one with 32 queries a wavefront over the keys (dq, and
+// delta on the way), one with 32 keys a wavefront over the queries of all heads that share them (dk and dv).  Both form the
+// scores again, seven products instead of the five of a single pass, which would have to add up dq from many workgroups in
+// an order of its own; here every sum has one.  p and ds are rounded to bf16 as operands (bf16 tensors), once each: what that
+// adds to a gradient is as large as its own rounding.
+#include "segment_attn.h"
+
+namespace ga {
+namespace {
+
+struct Backward : SegAttn {
+  const void *out, *grad;                // (nq, heads, dim), rows and heads as far apart as these say (bytes)
+  int64_t out_row, out_head, grad_row, grad_head;
+  const float *lse;                      // (heads, nq)
+  float *delta;                          // (heads, nq)
+  void *gq, *gk, *gv;                    // (rows, heads, dim), contiguous
+  int64_t tiles;
+};
+
+// Products of results w (operand over rows 32 b ... of `t`) and its columns onto acc.  CLEAN: values of t that are not finite
+// count as zero; whether there were any.
+template <typename T, int WIDE, bool CLEAN>
+__device__ __forceinline__ bool add_columns(const lds_char *t, int col_at, int b, const floatx16 &w,
+                                            floatx16 (&acc)[Rows<T, WIDE>::kCols]) {
+  typedef Rows<T, WIDE> R;
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < R::kParts; ++i) {
+    const uintx4 o = operand_of<T>(w, i);
+#pragma unroll
+    for (int d = 0; d < R::kCols; ++d) {
+      uintx4 v = R::col(t, col_at, b, i, d);
+      if constexpr (CLEAN) found |= cleaned<T>(v);
+      acc[d] = mma_piece<T>(v, o, acc[d]);
+    }
+  }
+  return found;
+}
+
+// dq: WAVES wavefronts with 32 queries of a head each share tiles of KEYS keys.
+template <typename T, int WIDE, int WAVES, int KEYS>
+__device__ __forceinline__ void segment_attn_dq(const Backward &p) {
+  typedef Rows<T, WIDE> R;
+  typedef RowMoves<T, WIDE, KEYS, WAVES> Moves;
+  constexpr int BM = 32 * WAVES, kStage = 2 * Moves::kBytes;
+  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage];
+  int head;
+  int64_t tile;
+  head_tile(blockIdx.x, p.tiles, p.heads, head, tile);
+  if (p.causal) tile = p.tiles - 1 - tile;
+  Segment seg;
+  if (!segment_of<BM>(p, tile, 1, false, seg)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x & (kWave - 1), n = lane & 31, h = lane >> 5;
+  const int kv = head / p.group;
+  const int first = seg.tile * BM + wave * 32, query = first + n;
+  const bool there = query < seg.q_len;
+  const int64_t at = seg.q0 + query;
+
+  uintx4 q[R::kSteps], g[R::kSteps];
+  load_row<T, WIDE>((const char *)p.q + at * p.q_row + head * p.q_head, there, p.dim, q);
+  load_row<T, WIDE>((const char *)p.grad + at * p.grad_row + head * p.grad_head, there, p.dim, g);
+  float delta = 0.0f;
+  {
+    uintx4 o[R::kSteps];
+    load_row<T, WIDE>((const char *)p.out + at * p.out_row + head * p.out_head, there, p.dim, o);
+#pragma unroll
+    for (int i = 0; i < R::kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          delta = fmaf(__uint_as_float(o[i][j]), __uint_as_float(g[i][j]), delta);
+        } else {
+          delta = fmaf(bf16_lo(o[i][j]), bf16_lo(g[i][j]), delta);
+          delta = fmaf(bf16_hi(o[i][j]), bf16_hi(g[i][j]), delta);
+        }
+      }
+    delta += other_half(delta);
+  }
+  float lse = there ? p.lse[head * p.nq + at] * kLog2e : 0.0f;
+  if (lse == -INFINITY) lse = INFINITY;                      // a query that sees nothing: p = 0
+  if (there && h == 0) p.delta[head * p.nq + at] = delta;
+  const float c = p.scale * kLog2e;
+
+  const int more = seg.k_len - seg.q_len;
+  const int seen = p.causal ? max(0, min(seg.k_len, query + 1 + more)) : seg.k_len;
+  const int by_all = p.causal ? max(0, min(seg.k_len, first + 1 + more)) : seg.k_len;
+  const int by_any = first >= seg.q_len ? 0 : p.causal ? max(0, min(seg.k_len, min(first + 32, seg.q_len) + more)) : seg.k_len;
+  const int block_last = min(seg.tile * BM + BM, seg.q_len);
+  const int wanted = p.causal ? max(0, min(seg.k_len, block_last + more)) : seg.k_len;
+  const int end = (wanted + KEYS - 1) / KEYS;
+
+  Moves mk, mv;
+  mk.init(p.k_row, p.dim, wave);
+  mv.init(p.v_row, p.dim, wave);
+  const char *k_at = (const char *)p.k + seg.k0 * p.k_row + kv * p.k_head;
+  const char *v_at = (const char *)p.v + seg.k0 * p.v_row + kv * p.v_head;
+  int to_fetch = 0;
+  auto fetch = [&](lds_char *to) {
+    if (to_fetch >= end) return;
+    const int left = seg.k_len - to_fetch * KEYS;
+    mk.move(k_at, left, to);
+    mv.move(v_at, left, to + Moves::kBytes);
+    k_at += KEYS * p.k_row;
+    v_at += KEYS * p.v_row;
+    ++to_fetch;
+  };
+  const int row_at = R::row_at(), col_at = R::col_at();
+  floatx16 dq[R::kCols];
+#pragma unroll
+  for (int d = 0; d < R::kCols; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
+
+  auto block = [&](const lds_char *keys, const lds_char *values, int b, int key0, auto edge) {
+    constexpr bool kEdge = decltype(edge)::value;
+    floatx16 s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R::kSteps; ++i) s = mma_piece<T>(R::row(keys, row_at, b, i), q[i], s);
+#pragma unroll
+    for (int i = 0; i < R::kSteps; ++i) dp = mma_piece<T>(R::row(values, row_at, b, i), g[i], dp);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float ds = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+      s[r] = !kEdge || key0 + result_row(r) + 4 * h < seen ? ds : 0.0f;
+    }
+    // A key that is not finite has scores that are not, which is what reaches the queries that see it.
+    add_columns<T, WIDE, kEdge>(keys, col_at, b, s, dq);
+  };
+  auto step = [&](int t, lds_char *here, lds_char *next) {
+    landed<0>();
+    fetch(next);
+#pragma unroll
+    for (int b = 0; b < KEYS / 32; ++b) {
+      const int key0 = t * KEYS + b * 32;
+      if (key0 >= by_any) continue;
+      if (key0 + 32 <= by_all) block(here, here + Moves::kBytes, b, key0, std::false_type());
+      else block(here, here + Moves::kBytes, b, key0, std::true_type());
+    }
+  };
+  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1;
+  fetch(L0);
+  int t = 0;
+  for (; t + 2 <= end; t += 2) {
+    step(t, L0, L1);
+    step(t + 1, L1, L0);
+  }
+  if (t < end) step(t, L0, L1);
+  store_row<T, R::kCols>((T *)p.gq + (at * p.heads + head) * p.dim, there, p.dim, dq, p.scale);
+}
+template <typename T, int WIDE, int WAVES, int KEYS>
+__global__ __launch_bounds__(WAVES *kWave) void segment_attn_dq_kernel(Backward p) {
+  segment_attn_dq<T, WIDE, WAVES, KEYS>(p);
+}
+
+// A lane's share of 32 numbers, as it holds 16 of 32 rows of results; zeros behind the `left` that there are.
+__device__ __forceinline__ void load_numbers(const float *from, int64_t left, floatx4 (&f)[4]) {
+  const int h = (threadIdx.x >> 5) & 1;
+  const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, (int)(min((int64_t)32, left) * 4), 0x00020000);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    f[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, (i * 8 + h * 4) * 4, 0, 0));
+}
+
+// dk and dv: WAVES wavefronts with 32 keys of a head each share tiles of QUERIES queries.
+template <typename T, int WIDE, int WAVES, int QUERIES>
+__device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
+  typedef Rows<T, WIDE> R;
+  typedef RowMoves<T, WIDE, QUERIES, WAVES> Moves;
+  constexpr int BN = 32 * WAVES, kStage = 2 * Moves::kBytes;
+  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage];
+  int kv;
+  int64_t tile;
+  head_tile(blockIdx.x, p.tiles, p.heads / p.group, kv, tile);
+  Segment seg;
+  if (!segment_of<BN>(p, tile, 1, true, seg)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x & (kWave - 1), n = lane & 31, h = lane >> 5;
+  const int first = seg.tile * BN + wave * 32, key = first + n;
+  const bool there = key < seg.k_len;
+  const int64_t at = seg.k0 + key;
+
+  uintx4 k[R::kSteps], v[R::kSteps];
+  load_row<T, WIDE>((const char *)p.k + at * p.k_row + kv * p.k_head, there, p.dim, k);
+  load_row<T, WIDE>((const char *)p.v + at * p.v_row + kv * p.v_head, there, p.dim, v);
+  const float c = p.scale * kLog2e;
+
+  // the first query that sees the lane's key, the wavefront's first and last and the workgroup's first
+  const int less = seg.q_len - seg.k_len;
+  const int by = p.causal ? key + less : 0;
+  const int by_any = p.causal ? first + less : 0, by_all = p.causal ? first + 31 + less : 0;
+  const int begin = p.causal ? max(0, seg.tile * BN + less) / QUERIES : 0;
+  const int end = (seg.q_len + QUERIES - 1) / QUERIES;
+  const int tiles = max(0, end - begin), all = tiles * p.group;
+
+  Moves mq, mg;
+  mq.init(p.q_row, p.dim, wave);
+  mg.init(p.grad_row, p.dim, wave);
+  const int64_t begin_row = seg.q0 + (int64_t)begin * QUERIES;
+  const char *q_at = (const char *)p.q + begin_row * p.q_row + kv * p.group * p.q_head;
+  const char *g_at = (const char *)p.grad + begin_row * p.grad_row + kv * p.group * p.grad_head;
+  const int64_t q_step = QUERIES * p.q_row, g_step = QUERIES * p.grad_row;
+  const int64_t q_next = p.q_head - tiles * q_step, g_next = p.grad_head - tiles * g_step;      // the first tile of the next head
+  int to_fetch = all, fetch_tile = begin;
+  auto fetch = [&](lds_char *to) {
+    if (to_fetch == 0) return;
+    const int left = seg.q_len - fetch_tile * QUERIES;
+    mq.move(q_at, left, to);
+    mg.move(g_at, left, to + Moves::kBytes);
+    q_at += q_step;
+    g_at += g_step;
+    --to_fetch;
+    if (++fetch_tile == end) {
+      fetch_tile = begin;
+      q_at += q_next;
+      g_at += g_next;
+    }
+  };
+  const int row_at = R::row_at(), col_at = R::col_at();
+  floatx16 dk[R::kCols], dv[R::kCols];
+#pragma unroll
+  for (int d = 0; d < R::kCols; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
+
+  auto block = [&](const lds_char *queries, const lds_char *grads, int b, int query0, int q_head, auto edge) {
+    constexpr bool kEdge = decltype(edge)::value;
+    // of the 32 queries, four adjacent ones a group; what lies behind the segment is not counted, behind the tensor zero
+    floatx4 lse[4], delta[4];
+    const int64_t row = q_head * p.nq + seg.q0 + query0, left = p.nq - seg.q0 - query0;
+    load_numbers(p.lse + row, left, lse);
+    load_numbers(p.delta + row, left, delta);
+    floatx16 s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R::kSteps; ++i) s = mma_piece<T>(R::row(queries, row_at, b, i), k[i], s);
+#pragma unroll
+    for (int i = 0; i < R::kSteps; ++i) dp = mma_piece<T>(R::row(grads, row_at, b, i), v[i], dp);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float l = lse[r / 4][r % 4];
+      const float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, l == -INFINITY ? -INFINITY : -kLog2e * l));
+      const float ds = w * (dp[r] - delta[r / 4][r % 4]);
+      const int query = query0 + result_row(r) + 4 * h;
+      const bool counts = !kEdge || (query >= by && query < seg.q_len);
+      s[r] = counts ? w : 0.0f;
+      dp[r] = counts ? ds : 0.0f;
+    }
+    const bool found = add_columns<T, WIDE, kEdge>(grads, col_at, b, s, dv);
+    if constexpr (kEdge) {
+      if (__ballot(found)) {             // what is not finite counts for the keys that its query sees and for no other
+#pragma unroll 1
+        for (int r = 0; r < 32; ++r)
+          add_not_finite<T, WIDE>(grads, b * 32 + r, query0 + r >= by && query0 + r < seg.q_len, dv);
+      }
+    }
+    add_columns<T, WIDE, kEdge>(queries, col_at, b, dp, dk);
+  };
+  int in_tile = begin, q_head = kv * p.group;
+  auto step = [&](lds_char *here, lds_char *next) {
+    landed<0>();
+    fetch(next);
+#pragma unroll
+    for (int b = 0; b < QUERIES / 32; ++b) {
+      const int query0 = in_tile * QUERIES + b * 32;
+      if (first >= seg.k_len || query0 >= seg.q_len || query0 + 31 < by_any) continue;
+      if (query0 >= by_all && query0 + 32 <= seg.q_len) block(here, here + Moves::kBytes, b, query0, q_head, std::false_type());
+      else block(here, here + Moves::kBytes, b, query0, q_head, std::true_type());
+    }
+    if (++in_tile == end) {
+      in_tile = begin;
+      ++q_head;
+    }
+  };
+  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1;
+  fetch(L0);
+  int t = 0;
+  for (; t + 2 <= all; t += 2) {
+    step(L0, L1);
+    step(L1, L0);
+  }
+  if (t < all) step(L0, L1);
+  const int64_t to = (at * (p.heads / p.group) + kv) * p.dim;
+  store_row<T, R::kCols>((T *)p.gk + to, there, p.dim, dk, p.scale);
+  store_row<T, R::kCols>((T *)p.gv + to, there, p.dim, dv, 1.0f);
+}
+template <typename T, int WIDE, int WAVES, int QUERIES>
+__global__ __launch_bounds__(WAVES *kWave, 1) void segment_attn_dkv_kernel(Backward p) {
+  segment_attn_dkv<T, WIDE, WAVES, QUERIES>(p);
+}
+
+template <typename T, int WIDE, int WAVES, int DEEP>
+int launch(Backward p, hipStream_t s) {
+  p.tiles = segment_tiles(p.nq, 1, p.segments, 32 * WAVES);
+  const int64_t dq_grid = p.tiles * p.heads;
+  const int64_t k_tiles = segment_tiles(p.nk, 1, p.segments, 32 * WAVES), dkv_grid = k_tiles * (p.heads / p.group);
+  if ((dq_grid > dkv_grid ? dq_grid : dkv_grid) > kMostLanes / (WAVES * kWave)) return GA_EUNSUPPORTED;
+  if (p.nq > 0) {
+    hipLaunchKernelGGL((segment_attn_dq_kernel<T, WIDE, WAVES, DEEP>), dim3((unsigned)dq_grid), dim3(WAVES * kWave), 0, s, p);
+    if (int rc = launch_status()) return rc;
+  }
+  p.tiles = k_tiles;
+  if (p.nk > 0) {
+    hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, WAVES, DEEP>), dim3((unsigned)dkv_grid), dim3(WAVES * kWave), 0, s, p);
+    if (int rc = launch_status()) return rc;
+  }
+  return GA_OK;
+}
+template <typename T>
+int backward(const Backward &p, hipStream_t s) {
+  if (p.dim <= 32) return launch<T, 32, 4, 64>(p, s);
+  if (p.dim <= 64) return launch<T, 64, 4, 64>(p, s);
+  return launch<T, 128, 4, sizeof(T) == 2 ? 64 : 32>(p, s);
+}
+
+}  // namespace
+}  // namespace ga
+
+extern "C" {
+
+size_t ga_segment_attention_backward_workspace_bytes(int64_t n_segments, int64_t n_queries, int64_t n_keys, int64_t heads,
+                                                     int64_t kv_heads, int64_t dim, int dtype) {
+  using namespace ga;
+  if (segment_attn_sizes(n_segments, n_queries, n_keys, heads, kv_heads, dim, dtype)) return 0;
+  int64_t n = (n_queries * heads * 4 + 255) / 256 * 256;
+  if (!whole_rows(dim, dtype))
+    n += 2 * segment_attn_laid_bytes(n_queries, heads, dim, dtype) + 2 * segment_attn_laid_bytes(n_keys, kv_heads, dim, dtype);
+  return (size_t)n;
+}
+
+int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q_row, int64_t q_head, const void *k,
+                                  int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
+                                  const float *lse, const int64_t *q_pointer, const int64_t *k_pointer, int64_t n_segments,
+                                  void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
+                                  int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
+                                  size_t workspace_bytes, ga_stream_t stream) {
+  using namespace ga;
+  Backward p{};
+  if (int rc = segment_attn_check(p, q, k, v, q_row, q_head, k_row, k_head, v_row, v_head, q_pointer, k_pointer, n_segments,
+                                  n_queries, n_keys, heads, kv_heads, dim, causal, scale, dtype))
+    return rc;
+  if ((n_queries > 0 && (!grad_out || !out || !lse || !grad_q)) || (n_keys > 0 && (!grad_k || !grad_v))) return GA_EINVAL;
+  const int64_t e = dtype == GA_F32 ? 4 : 2;
+  if (!aligned(grad_out, e) || !aligned(out, e) || !aligned(lse, 4) || !aligned(grad_q, e) || !aligned(grad_k, e) ||
+      !aligned(grad_v, e))
+    return GA_EALIGN;
+  const bool whole = whole_rows(dim, dtype);
+  auto pieces_aligned = [](const void *a, int64_t row, int64_t head) { return aligned(a, 16) && row % 16 == 0 && head % 16 == 0; };
+  if (whole && ((n_keys > 0 && (!pieces_aligned(k, p.k_row, p.k_head) || !pieces_aligned(v, p.v_row, p.v_head))) ||
+                (n_queries > 0 && (!pieces_aligned(q, p.q_row, p.q_head) || !aligned(grad_out, 16)))))
+    return GA_EALIGN;
+  const size_t bytes = ga_segment_attention_backward_workspace_bytes(n_segments, n_queries, n_keys, heads, kv_heads, dim, dtype);
+  if (bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < bytes)) return GA_EWORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  p.out = out;
+  p.grad = grad_out;
+  p.out_head = p.grad_head = dim * e;
+  p.out_row = p.grad_row = heads * dim * e;
+  p.lse = lse;
+  p.delta = (float *)workspace;
+  p.gq = grad_q;
+  p.gk = grad_k;
+  p.gv = grad_v;
+  if (!whole) {
+    char *at = (char *)workspace + (n_queries * heads * 4 + 255) / 256 * 256;
+    const int64_t of_q = segment_attn_laid_bytes(n_queries, heads, dim, dtype);
+    const int64_t of_k = segment_attn_laid_bytes(n_keys, kv_heads, dim, dtype);
+    const int64_t head = (dim * e + 15) / 16 * 16;
+    if (int rc = segment_attn_lay(q, at, n_queries, p.q_row, p.q_head, heads, grad_out, at + of_q, n_queries, p.grad_row,
+                                  p.grad_head, heads, dim, dtype, s))
+      return rc;
+    p.q = at;
+    p.grad = at + of_q;
+    p.q_head = p.grad_head = head;
+    p.q_row = p.grad_row = head * heads;
+    at += 2 * of_q;
+    if (int rc = segment_attn_lay(k, at, n_keys, p.k_row, p.k_head, kv_heads, v, at + of_k, n_keys, p.v_row, p.v_head, kv_heads,
+                                  dim, dtype, s))
+      return rc;
+    p.k = at;
+    p.v = at + of_k;
+    p.k_head = p.v_head = head;
+    p.k_row = p.v_row = head * kv_heads;
+  }
+  return dtype == GA_F32 ? backward<float>(p, s) : backward<bf16_t>(p, s);
+}
+
+}  // extern "C"

@@ -1740,3 +1740,137 @@ def gated_linear_backward(grad_h, x, w_gate, w_up, activation: str = "silu"):
     _launch("ga_gated_linear_backward", x.get_device(), grad_h.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
             w_up.data_ptr(), gx.data_ptr(), gg.data_ptr(), gu.data_ptr(), rows, k, f, act, dt, _ptr(ws), n)
     return gx, gg, gu
+
+
+# ------------------------------------------- transformers over graphs: attention inside segments ----
+SEGMENT_ATTENTION_MAX_DIM = 128
+
+
+def _rows_heads(x, name: str, like=None) -> None:
+    """(rows, heads, dim) whose dim values lie next to each other; rows and heads may lie anywhere."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if x.dim() != 3 or x.shape[1] == 0 or not 0 < x.shape[2] <= SEGMENT_ATTENTION_MAX_DIM:
+        raise RuntimeError(f"{name} must be (rows, heads, dim) with at most {SEGMENT_ATTENTION_MAX_DIM} dim")
+    if x.shape[2] > 1 and x.stride(2) != 1:
+        raise RuntimeError(f"the last dimension of {name} must be contiguous")
+    if like is not None and (x.dtype != like.dtype or x.get_device() != like.get_device()):
+        raise RuntimeError(f"{name} must be of the dtype and on the device of q")
+
+
+def _check_pointer(pointer, name: str, device) -> None:
+    _check_input(pointer, name)
+    if pointer.dtype != torch.int64 or pointer.dim() != 1 or pointer.numel() == 0 or pointer.get_device() != device:
+        raise RuntimeError(f"{name} must be (segments + 1,) int64 on the device of q")
+
+
+def _in_pieces(x):
+    """Heads whose rows are whole 16-byte pieces, as the kernels read them; a copy where they lie otherwise."""
+    size = x.element_size()
+    if x.shape[2] * size % 16 == 0 and (x.data_ptr() % 16 or x.stride(0) * size % 16 or x.stride(1) * size % 16):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _attention_args(q, k, v, q_pointer, k_pointer, scale):
+    _rows_heads(q, "q")
+    dt = _feat_dtype(q, "q")
+    _rows_heads(k, "k", q)
+    _rows_heads(v, "v", q)
+    if k.shape != v.shape or k.shape[2] != q.shape[2] or q.shape[1] % k.shape[1]:
+        raise RuntimeError("k and v must be (rows, kv_heads, dim) with q's dim and a divisor of its heads")
+    _check_pointer(q_pointer, "q_pointer", q.get_device())
+    if k_pointer is None:
+        k_pointer = q_pointer
+    else:
+        _check_pointer(k_pointer, "k_pointer", q.get_device())
+    if k_pointer.numel() != q_pointer.numel():
+        raise RuntimeError("q_pointer and k_pointer must have one entry more than there are segments")
+    if k_pointer is q_pointer and k.shape[0] != q.shape[0]:
+        raise RuntimeError("k and v must have q's rows where there is no k_pointer")
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    if scale == 0 or not abs(scale) < float("inf"):
+        raise RuntimeError("scale must be finite and not 0")
+    sizes = (int(q_pointer.numel()) - 1, int(q.shape[0]), int(k.shape[0]), int(q.shape[1]), int(k.shape[1]),
+             int(q.shape[2]))
+    return dt, k_pointer, scale, sizes
+
+
+def _placed(x):
+    return x.data_ptr(), x.stride(0), x.stride(1)
+
+
+class _SegmentAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_pointer, k_pointer, causal, scale):
+        _not_recorded("segment_attention")
+        out, lse = _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, True)
+        ctx.causal, ctx.scale = causal, scale
+        ctx.save_for_backward(q, k, v, out, lse, q_pointer, k_pointer)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out, grad_lse=None):
+        _not_recorded("segment_attention")
+        if grad_out is None:
+            return (None,) * 7
+        q, k, v, out, lse, q_pointer, k_pointer = ctx.saved_tensors
+        return (*segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, ctx.causal, ctx.scale),
+                None, None, None, None)
+
+
+def _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, return_lse):
+    dt, k_pointer, scale, sizes = _attention_args(q, k, v, q_pointer, k_pointer, scale)
+    k, v = _in_pieces(k), _in_pieces(v)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if return_lse else None
+    n = capi.load().ga_segment_attention_workspace_bytes(*sizes, dt)
+    ws = _scratch(n, q.device)
+    _launch("ga_segment_attention", q.get_device(), *_placed(q), *_placed(k), *_placed(v), q_pointer.data_ptr(),
+            k_pointer.data_ptr(), sizes[0], out.data_ptr(), _ptr(lse), *sizes[1:], bool(causal), scale, dt, _ptr(ws), n)
+    return (out, lse) if return_lse else out
+
+
+def segment_attention(q, k, v, q_pointer, k_pointer=None, causal: bool = False, scale=None, return_lse: bool = False):
+    """Softmax attention of packed rows inside their segments: every node of a graph of a batch over the
+    nodes of its graph, a sequence of nodes, a readout's queries over a graph (:func:`dot_attention_sum` is the same along
+    edges).  q (queries, heads, dim), k and v (keys, kv_heads, dim), heads a multiple of kv_heads: head h reads
+    key head h // (heads // kv_heads).  Segment s has the queries q_pointer[s] to q_pointer[s + 1] and the
+    keys k_pointer[s] to k_pointer[s + 1] (int64, ascending; without k_pointer those of the queries).  With
+    ``causal`` the query at place i of its segment sees the keys at places up to i + (keys - queries).
+    ``scale`` (1 / sqrt(dim)) multiplies the scores.  Returns (queries, heads, dim); with ``return_lse`` also the
+    (heads, queries) fp32 logarithms of the sums of exponentials.  A query that sees no key gives zeros and
+    -inf, as do rows in no segment.  float32 or bfloat16, dim up to 128; rows and heads may be strided (columns of one
+    projection), dim not.  Scores and sums are fp32; bf16 weights are rounded once as operands.  Differentiable in q, k
+    and v (backward mode)."""
+    if _wants_grad("segment_attention", q, k, v):
+        got = _SegmentAttention.apply(q, k, v, q_pointer, q_pointer if k_pointer is None else k_pointer, bool(causal), scale)
+        return got if return_lse else got[0]
+    return _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, return_lse)
+
+
+def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer=None, causal: bool = False,
+                               scale=None):
+    """Gradients of :func:`segment_attention`: (of q, of k, of v), contiguous, from what it returned with
+    ``return_lse``.  Rows in no segment get zeros.  The results have no gradients of their own."""
+    _check_seen("segment_attention_backward", grad_out, q, k, v, out)
+    dt, k_pointer, scale, sizes = _attention_args(q, k, v, q_pointer, k_pointer, scale)
+    _check_like(out, "out", q.shape, q)
+    _check_input(lse, "lse")
+    if lse.dtype != torch.float32 or lse.shape != (q.shape[1], q.shape[0]) or lse.get_device() != q.get_device():
+        raise RuntimeError("lse must be the (heads, queries) float32 tensor that segment_attention returned")
+    _rows_heads(grad_out, "grad_out", q)
+    if grad_out.shape != q.shape:
+        raise RuntimeError("grad_out must have q's shape")
+    grad_out = grad_out.contiguous()
+    q, k, v, grad_out = _in_pieces(q), _in_pieces(k), _in_pieces(v), _in_pieces(grad_out)
+    gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    n = capi.load().ga_segment_attention_backward_workspace_bytes(*sizes, dt)
+    ws = _scratch(n, q.device)
+    _launch("ga_segment_attention_backward", q.get_device(), grad_out.data_ptr(), *_placed(q), *_placed(k), *_placed(v),
+            out.data_ptr(), lse.data_ptr(), q_pointer.data_ptr(), k_pointer.data_ptr(), sizes[0], gq.data_ptr(),
+            gk.data_ptr(), gv.data_ptr(), *sizes[1:], bool(causal), scale, dt, _ptr(ws), n)
+    return gq, gk, gv

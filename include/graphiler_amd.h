@@ -850,6 +850,49 @@ int ga_gated_linear_fp8(const void *x8, const void *x_scales, const void *wg8, c
                         const void *wu8, const void *wu_scales, void *h, int64_t rows, int64_t K,
                         int64_t F, int activation, int out_dtype, ga_stream_t stream);
 
+/* ---- transformers over graphs: attention inside segments of packed rows ---------------- */
+
+/*
+ * Attention of packed rows inside their segments (the nodes of a graph of a batch, a sequence of nodes):
+ *   out[i, h] = sum over j of exp(s - lse) v[j, g],  s = scale <q[i, h], k[j, g]>,  lse = log of the sum of exp(s)
+ * over the keys j of query i's segment; with `causal` those whose place in the segment is at most i's plus (keys - queries).
+ * Segment s has the queries q_pointer[s] ... q_pointer[s + 1] - 1 and the keys k_pointer[s] ... k_pointer[s + 1] - 1.
+ * A query that sees no key, and rows in front of the first and behind the last segment, give zeros (lse -inf).
+ *   q, out   (n_queries, heads, dim), k, v (n_keys, kv_heads, dim), all of `dtype`; heads is a multiple of kv_heads, and
+ *            g = h / (heads / kv_heads).  q_row ... v_head: values from row to row and from head to head of q, k and v,
+ *            whose dim values lie next to each other; out is contiguous
+ *   lse      (heads, n_queries) fp32, or NULL
+ *   pointers n_segments + 1 ascending int64 on the device (values outside the rows are taken as the nearest bound; rows
+ *            in two segments get one's result or the other's)
+ * Scores, their softmax and all sums are fp32; the weights are rounded to bf16 as operands where the tensors are bf16.  A value
+ * row that is not finite reaches the queries that see it and no others.  Where dim values are whole 16-byte pieces, k and
+ * v and their distances have to be 16-byte aligned; where they are not, k and v are laid out in the workspace.
+ * GA_EINVAL for a scale that is 0 or not finite; GA_EUNSUPPORTED when dim > 128 or rows are more than 16 MB apart.
+ */
+size_t ga_segment_attention_workspace_bytes(int64_t n_segments, int64_t n_queries, int64_t n_keys, int64_t heads,
+                                            int64_t kv_heads, int64_t dim, int dtype);
+int ga_segment_attention(const void *q, int64_t q_row, int64_t q_head, const void *k, int64_t k_row, int64_t k_head,
+                         const void *v, int64_t v_row, int64_t v_head, const int64_t *q_pointer, const int64_t *k_pointer,
+                         int64_t n_segments, void *out, float *lse, int64_t n_queries, int64_t n_keys, int64_t heads,
+                         int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
+                         size_t workspace_bytes, ga_stream_t stream);
+
+/*
+ * Its gradients, from out and lse: with p = exp(s - lse), ds = p (<grad_out[i], v[j]> - <grad_out[i], out[i]>),
+ *   grad_q[i] = scale sum_j ds k[j], grad_k[j] = scale sum_i ds q[i], grad_v[j] = sum_i p grad_out[i],
+ * those of k and v over all heads that share them; rows outside the segments get zeros.  grad_out, out and the gradients are
+ * contiguous; p and ds are rounded to bf16 as operands where the tensors are bf16.  No sum's order depends on anything but the
+ * sizes.  Where dim values are whole 16-byte pieces, q and grad_out have to be 16-byte aligned as k and v are.
+ */
+size_t ga_segment_attention_backward_workspace_bytes(int64_t n_segments, int64_t n_queries, int64_t n_keys, int64_t heads,
+                                                     int64_t kv_heads, int64_t dim, int dtype);
+int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q_row, int64_t q_head, const void *k,
+                                  int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
+                                  const float *lse, const int64_t *q_pointer, const int64_t *k_pointer, int64_t n_segments,
+                                  void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
+                                  int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
+                                  size_t workspace_bytes, ga_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
