@@ -19,55 +19,10 @@
 // of 2,001 x 300 -> 700: 28 + 22 + 22, 12 to add up parts, 5 to lay out.  At most 16 rows: gated_few.hip; fp32
 // products of few tiles: gated_f32.hip.
 #include "gated_few.h"
-#include "vec8.h"
+#include "mm_parts.h"
 
 namespace ga {
 namespace {
-
-// x = p0 + p1 + p2 as bf16, as split8 forms them
-__device__ __forceinline__ void pieces(float x, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
-  p0 = __float_as_uint(x) >> 16;
-  const float r = x - bf16_lo(p0);
-  p1 = f32_to_bf16_bits(r);
-  p2 = f32_to_bf16_bits(r - bf16_lo(p1));
-}
-
-// Rows (rows, cols) as bf16 rows of `wide` values (a multiple of 8; zeros behind cols): the values
-// themselves or, of fp32, three planes of pieces.  Up to three matrices a launch.
-struct LayOut {
-  const void *from[3];
-  bf16_t *to[3];
-  int64_t rows[3];
-  int cols[3], wide[3];
-};
-template <typename T>
-__global__ __launch_bounds__(kBlock) void lay_out_kernel(LayOut p) {
-  const int m = blockIdx.y;
-  const int groups = p.wide[m] / kVec;
-  const int64_t all = p.rows[m] * groups;
-  for (int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x; id < all; id += (int64_t)gridDim.x * kBlock) {
-    const int64_t row = id / groups;
-    const int c = (int)(id % groups) * kVec;
-    float f[kVec];
-    load_group((const T *)p.from[m] + row * p.cols[m] + c, p.cols[m] - c, f);
-    bf16_t *to = p.to[m] + row * p.wide[m] + c;
-    if constexpr (sizeof(T) == 2) {
-      store8(to, f);
-    } else {
-      uint4 a, b, d;
-      split8(f, a, b, d);
-      const int64_t plane = p.rows[m] * p.wide[m];
-      *reinterpret_cast<uint4 *>(to) = a;
-      *reinterpret_cast<uint4 *>(to + plane) = b;
-      *reinterpret_cast<uint4 *>(to + 2 * plane) = d;
-    }
-  }
-}
-
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-}
 
 // dg and du of a tile, as operands of the products after: bf16 rows of `ld` values, of fp32 three planes of pieces.
 template <typename T, int ACT = -1>
@@ -89,29 +44,7 @@ struct GradEpi : Stored<bf16_t> {
   }
   __device__ __forceinline__ void make(const TileMm &p, int64_t row, int64_t col, const floatx4 &g, const floatx4 &u,
                                        uintx2 (&o)[kOut]) const {
-    // no branch around a load, so that many are on their way: what is not there is out of range, 0
-    const int64_t row0 = row & ~(int64_t)255;                // the same for a tile's rows
-    const rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<T *>(gh + uniform(row0) * gh_cols), 0,
-        (int)(min((int64_t)256, max(p.rows - uniform(row0), (int64_t)0)) * gh_cols * (int)sizeof(T)), 0x00020000);
-    const uint32_t at = ((uint32_t)(row - row0) * (uint32_t)gh_cols + (uint32_t)col) * sizeof(T);
-    floatx4 t;
-    if (whole) {
-      const uint32_t o = col < gh_cols ? at : kOutside;
-      if constexpr (sizeof(T) == 4) {
-        t = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(src, o, 0, 0));
-      } else {
-        const uintx2 w = __builtin_bit_cast(uintx2, __builtin_amdgcn_raw_buffer_load_b64(src, o, 0, 0));
-        t = floatx4{bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t o = col + r < gh_cols ? at + r * sizeof(T) : kOutside;
-        if constexpr (sizeof(T) == 4) t[r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src, o, 0, 0));
-        else t[r] = bf16_lo((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(src, o, 0, 0));
-      }
-    }
+    const floatx4 t = four_at(gh, gh_cols, p.rows, row, col, whole);
     floatx4 a, b;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -122,49 +55,15 @@ struct GradEpi : Stored<bf16_t> {
       o[0] = pack(a);
       o[1] = pack(b);
     } else {
-      cut(a, o[0], o[1], o[2]);
-      cut(b, o[3], o[4], o[5]);
+      cut_pieces(a, o[0], o[1], o[2]);
+      cut_pieces(b, o[3], o[4], o[5]);
     }
-  }
-  static __device__ __forceinline__ void cut(const floatx4 &v, uintx2 &o0, uintx2 &o1, uintx2 &o2) {
-    uint32_t p[3][4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) pieces(v[r], p[0][r], p[1][r], p[2][r]);
-    o0 = uintx2{p[0][0] | (p[0][1] << 16), p[0][2] | (p[0][3] << 16)};
-    o1 = uintx2{p[1][0] | (p[1][1] << 16), p[1][2] | (p[1][3] << 16)};
-    o2 = uintx2{p[2][0] | (p[2][1] << 16), p[2][2] | (p[2][3] << 16)};
   }
   __device__ __forceinline__ void store(const TileMm &, int k, int64_t row, int64_t col, const uintx4 &w, int64_t n) const {
     bf16_t *to = (k < kPieces ? dg : du) + k % kPieces * plane;
     store_chunk(to + row * ld + col, w, n);
   }
 };
-
-// Sums of the parts of a contraction, `all` values each: n of the first result, then the second's.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void join_parts_kernel(const float *__restrict__ parts, T *__restrict__ out0,
-                                                            T *__restrict__ out1, int64_t n, int64_t all,
-                                                            int splits) {
-  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < all; i += (int64_t)gridDim.x * kBlock) {
-    float s = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < splits; ++k) s += parts[k * all + i];
-    f32_to_elem(s, i >= n ? out1[i - n] : out0[i]);
-  }
-}
-template <typename T>
-__global__ __launch_bounds__(kBlock) void zeros_kernel(T *__restrict__ out0, T *__restrict__ out1, int64_t n) {
-  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) {
-    f32_to_elem(0.0f, out0[i]);
-    f32_to_elem(0.0f, out1[i]);
-  }
-}
-
-int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
-unsigned stream_grid(int64_t items) {
-  const int64_t g = (items + kBlock - 1) / kBlock;
-  return (unsigned)(g < 1 ? 1 : g > 8192 ? 8192 : g);
-}
 
 // Where the operands of a call lie in its workspace (bf16 values; -1: the caller's tensor itself).
 struct Plan {
@@ -175,13 +74,6 @@ struct Plan {
   int splits, x_splits;                  // parts of the sums of the weights' gradients and of x's
   size_t bytes;
 };
-// Into how many parts a contraction of `steps` steps is cut for `tiles` tiles: as many as give the
-// chip's 512 places a workgroup each, none of fewer than eight steps (a part writes and reads its results once more).
-int parts_of(int64_t tiles, int64_t steps) {
-  int64_t n = 512 / (tiles > 0 ? tiles : 1);
-  if (n > steps / 8) n = steps / 8;
-  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-}
 Plan plan_of(int64_t rows, int64_t K, int64_t F, int dtype, bool grad) {
   Plan p;
   p.Kp = round8(K);

@@ -1,4 +1,4 @@
-// act(x Wg) * (x Wu) in fp32 on the fp32 matrix instruction, for grids of few tiles.
+// act(x Wg) * (x Wu), and act(x W + b) + r, in fp32 on the fp32 matrix instruction, for grids of few tiles.
 //
 // The tile kernel of gated.hip multiplies bf16 pieces, six products a pair: 2.5 times the rate of v_mfma_f32_16x16x4_f32
 // where tiles fill the chip, but a workgroup then goes through six times the steps one after the other, behind a
@@ -39,20 +39,21 @@ __device__ __forceinline__ floatx4 four_of(const float *__restrict__ m, int64_t 
   return v;
 }
 
-// SPLIT: how many wavefronts share the k of a step; the tile has 64 / SPLIT rows.
-template <int SPLIT>
-__global__ __launch_bounds__(kBlock, 2) void gated_f32_kernel(
-    const float *__restrict__ x, const float *__restrict__ wg, const float *__restrict__ wu, float *__restrict__ h,
-    int64_t rows, int64_t K, int64_t F, int act, int row_tiles, int col_tiles) {
-  constexpr int kRows = kF32Rows / SPLIT;
+// SPLIT: how many wavefronts share the k of a step; the tile has 64 / SPLIT rows.  PAIR: both products, else twice the
+// columns of the first.
+template <int SPLIT, bool PAIR, typename Finish>
+__global__ __launch_bounds__(kBlock, 2) void few_tiles_f32_kernel(
+    const float *__restrict__ x, const float *__restrict__ wg, const float *__restrict__ wu, Finish finish,
+    int64_t rows, int64_t K, int64_t F, int row_tiles, int col_tiles) {
+  constexpr int kRows = kF32Rows / SPLIT, kCols = PAIR ? kF32Cols : 2 * kF32Cols;
   __shared__ __attribute__((aligned(16))) float xs[2][kRows * kF32Ld], ws[2][kF32Step * kF32Ld];
   int tr, tc;
   tile_of(blockIdx.x, row_tiles * col_tiles, row_tiles, col_tiles, tr, tc);
-  const int64_t row0 = (int64_t)tr * kRows, col0 = (int64_t)tc * kF32Cols;
+  const int64_t row0 = (int64_t)tr * kRows, col0 = (int64_t)tc * kCols;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n = lane & 15, q = lane >> 4;
   const int side = wave & 1, high = wave >> 1;               // 16 of the columns; 32 of the rows, or of a step's k
   const int wave_row = SPLIT == 1 ? 32 * high : 0, first_s = SPLIT == 1 ? 0 : 2 * high;
-  const bool columns = col0 + kF32Cols <= F;
+  const bool columns = col0 + kCols <= F;
 
   floatx4 acc[2][2][2];                                      // [s & 1][16 rows][gate, up]
 #pragma unroll
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(kBlock, 2) void gated_f32_kernel(
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      vw[i] = four_of<kWhole>(i < 2 ? wg : wu, k0 + wk + 32 * (i & 1), K, col0 + wc, F);
+      vw[i] = four_of<kWhole>(!PAIR || i < 2 ? wg : wu, k0 + wk + 32 * (i & 1), K, col0 + (!PAIR && i >= 2 ? kF32Cols : 0) + wc, F);
   };
   auto fetch = [&](int64_t k0) {
     if (columns && k0 + kF32Step <= K) take(std::true_type(), k0);
@@ -139,13 +140,33 @@ __global__ __launch_bounds__(kBlock, 2) void gated_f32_kernel(
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int64_t row = row0 + wave_row + t * 16 + n;
-    if (row >= rows || col >= F) continue;
-    floatx4 o;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = gate_of(act, sum[t][0][r]) * sum[t][1][r];
-    store_chunk(h + row * F + col, __builtin_bit_cast(uintx4, o), F - col);
+    if (row >= rows) continue;
+    if (col < F) finish(row, col, sum[t][0], sum[t][1], F);
+    if constexpr (!PAIR)
+      if (col + kF32Cols < F) finish(row, col + kF32Cols, sum[t][1], sum[t][1], F);
   }
 }
+
+// What becomes of the sums of four adjacent columns.
+struct Gated4 {
+  float *h;
+  int act;
+  __device__ __forceinline__ void operator()(int64_t row, int64_t col, const floatx4 &g, const floatx4 &u, int64_t F) const {
+    floatx4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = gate_of(act, g[r]) * u[r];
+    store_chunk(h + row * F + col, __builtin_bit_cast(uintx4, o), F - col);
+  }
+};
+struct Ended4 {
+  LinearEnd end;
+  __device__ __forceinline__ void operator()(int64_t row, int64_t col, const floatx4 &z, const floatx4 &, int64_t F) const {
+    const Ended<float> e(end);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col + r < F) e(row, col + r, z[r], 0.0f);
+  }
+};
 
 }  // namespace
 
@@ -161,22 +182,36 @@ bool gated_f32_taken(int64_t rows, int64_t K, int64_t F) {
   return F <= 96 || f32_tiles(rows, F, kF32Rows) <= (K <= 256 ? 1024 : 640);
 }
 
-int gated_f32_launch(const void *x, const void *wg, const void *wu, void *h, int64_t rows, int64_t K, int64_t F,
-                     int act, hipStream_t s) {
+template <bool PAIR, typename Finish>
+static int f32_launch(const void *x, const void *w0, const void *w1, const Finish &finish, int64_t rows, int64_t K, int64_t F,
+                      hipStream_t s) {
   // 32 rows a tile where all such tiles run at once, three a compute unit: 17 x 1024 -> 1024 27.5 -> 16.9 us,
   // 2708 x 1433 -> 256 63 -> 49; beyond, 2708 x 1024 -> 341 55 -> 62.
-  const bool low = f32_tiles(rows, F, kF32Rows / 2) <= 768;
+  constexpr int kCols = PAIR ? kF32Cols : 2 * kF32Cols;
+  const bool low = tiles_of(rows, F, kF32Rows / 2, kCols) <= 768;
   const int64_t row_tiles = (rows + (low ? kF32Rows / 2 : kF32Rows) - 1) / (low ? kF32Rows / 2 : kF32Rows);
-  const int64_t col_tiles = (F + kF32Cols - 1) / kF32Cols;
+  const int64_t col_tiles = (F + kCols - 1) / kCols;
   if (row_tiles * col_tiles > kMostLanes / kBlock) return GA_EUNSUPPORTED;
 #define GA_F32_LAUNCH(SPLIT)                                                                                          \
-  hipLaunchKernelGGL((gated_f32_kernel<SPLIT>), dim3((unsigned)(row_tiles * col_tiles)), dim3(kBlock), 0, s,          \
-                     (const float *)x, (const float *)wg, (const float *)wu, (float *)h, rows, K, F, act,             \
-                     (int)row_tiles, (int)col_tiles)
+  hipLaunchKernelGGL((few_tiles_f32_kernel<SPLIT, PAIR, Finish>), dim3((unsigned)(row_tiles * col_tiles)), dim3(kBlock), 0, s, \
+                     (const float *)x, (const float *)w0, (const float *)w1, finish, rows, K, F, (int)row_tiles,      \
+                     (int)col_tiles)
   if (low) GA_F32_LAUNCH(2);
   else GA_F32_LAUNCH(1);
 #undef GA_F32_LAUNCH
   return launch_status();
+}
+
+int gated_f32_launch(const void *x, const void *wg, const void *wu, void *h, int64_t rows, int64_t K, int64_t F,
+                     int act, hipStream_t s) {
+  return f32_launch<true>(x, wg, wu, Gated4{(float *)h, act}, rows, K, F, s);
+}
+
+bool linear_f32_taken(int64_t rows, int64_t K, int64_t M) {
+  return M <= 128 || tiles_of(rows, M, kF32Rows, 2 * kF32Cols) <= (K <= 256 ? 2048 : 1280);
+}
+int linear_f32_launch(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, hipStream_t s) {
+  return f32_launch<false>(x, w, nullptr, Ended4{end}, rows, K, M, s);
 }
 
 }  // namespace ga

@@ -1,5 +1,5 @@
-// act(x Wg) * (x Wu) for few rows of x: a query that is answered by itself.  All there is to do is
-// to read both weights once, with enough of them on their way: 64 columns a workgroup (128 or 256
+// act(x Wg) * (x Wu), and act(x W + b) + r, for few rows of x: a query that is answered by itself.  All there is to do is
+// to read the weights once, with enough of them on their way: 64 columns a workgroup (128 or 256
 // bytes of a weight's row), its wavefronts take turns along k and add up what they have in
 // LDS, in their order.  Three rows, 1024 to 4096, bf16 (16.8 MB): 4.7 us recorded in a graph (3.6 TB/s), 5.4-7.3 in
 // traces; a wavefront that read 64 of k of both weights and then multiplied took 10.2 there.
@@ -54,17 +54,17 @@ __device__ __forceinline__ void few_products(const uintx4 (&w)[8], const bf16x8 
   }
 }
 
-// Eight wavefronts, four for each weight, with CHUNKS times 64 of k on their way each: what the
+// Eight wavefronts, four for each weight of a PAIR, with CHUNKS times 64 of k on their way each: what the
 // registers hold beside RT times 32 sums.
-constexpr int kTurns = 4;
-template <int RT, int CHUNKS>
-__global__ __launch_bounds__(2 * kTurns *kWave) void gated_few_bf16_kernel(
-    const bf16_t *__restrict__ x, const bf16_t *__restrict__ wg, const bf16_t *__restrict__ wu, bf16_t *__restrict__ h,
-    int rows, int64_t K, int64_t F, int act) {
+template <int RT, int CHUNKS, bool PAIR, typename Finish>
+__global__ __launch_bounds__(8 * kWave) void few_bf16_kernel(
+    const bf16_t *__restrict__ x, const bf16_t *__restrict__ wg, const bf16_t *__restrict__ wu, Finish finish,
+    int rows, int64_t K, int64_t F) {
   constexpr int kRows = 8 * RT, kLd = kFewCols + 4;                    // rows of sums four banks apart
-  __shared__ float sums[kTurns][2][2][kRows][kLd];                     // turn, half of k, weight
+  constexpr int kWeights = PAIR ? 2 : 1, kTurns = 8 / kWeights;
+  __shared__ float sums[kTurns][2][kWeights][kRows][kLd];              // turn, half of k, weight
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int turn = wave >> 1, which = wave & 1;
+  const int turn = PAIR ? wave >> 1 : wave, which = PAIR ? wave & 1 : 0;
   const bf16_t *__restrict__ w = which ? wu : wg;
   const int64_t c = (int64_t)blockIdx.x * kFewCols + (lane & 7) * 8;
   const int half = (lane >> 3) & 1, q = lane >> 4;                     // of operand x: rows lane % 8, k 8 (2 q + half) ...
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(2 * kTurns *kWave) void gated_few_bf16_kernel(
         for (int r = 0; r < 4; ++r) sums[turn][half][which][t * 8 + (lane & 7)][((4 * q + r) & 7) * 8 + j] = acc[t][j][r];
   }
   __syncthreads();
-  for (int id = threadIdx.x; id < rows * kFewCols; id += 2 * kTurns * kWave) {
+  for (int id = threadIdx.x; id < rows * kFewCols; id += 8 * kWave) {
     const int row = id / kFewCols, col = id % kFewCols;
     const int64_t f = (int64_t)blockIdx.x * kFewCols + col;
     if (f >= F) continue;
@@ -116,9 +116,9 @@ __global__ __launch_bounds__(2 * kTurns *kWave) void gated_few_bf16_kernel(
 #pragma unroll
     for (int t = 0; t < kTurns; ++t) {
       g += sums[t][0][0][row][col] + sums[t][1][0][row][col];
-      u += sums[t][0][1][row][col] + sums[t][1][1][row][col];
+      if constexpr (PAIR) u += sums[t][0][1][row][col] + sums[t][1][1][row][col];
     }
-    h[row * F + f] = (bf16_t)f32_to_bf16_bits(gate_of(act, g) * u);
+    finish(row, f, g, u);
   }
 }
 
@@ -141,12 +141,12 @@ __device__ __forceinline__ floatx4 weight4(const float *__restrict__ w, int64_t 
   return r;
 }
 
-template <int RT, int WAVES>
-__global__ __launch_bounds__(WAVES *kWave) void gated_few_f32_kernel(
-    const float *__restrict__ x, const float *__restrict__ wg, const float *__restrict__ wu, float *__restrict__ h,
-    int rows, int64_t K, int64_t F, int act) {
-  constexpr int kRows = 16 * RT, kDeep = 8;                            // fours of k on their way
-  __shared__ float sums[WAVES / 2][2][kRows][kFewCols];
+template <int RT, int WAVES, bool PAIR, typename Finish>
+__global__ __launch_bounds__(WAVES *kWave) void few_f32_kernel(
+    const float *__restrict__ x, const float *__restrict__ wg, const float *__restrict__ wu, Finish finish, int rows,
+    int64_t K, int64_t F) {
+  constexpr int kRows = 16 * RT, kDeep = PAIR ? 8 : 16;                // fours of k on their way
+  __shared__ float sums[WAVES / 2][PAIR ? 2 : 1][kRows][kFewCols];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, n = lane & 15, q = lane >> 4;
   const int64_t c = (int64_t)blockIdx.x * kFewCols + n * 4;
   floatx4 gate[RT][4], up[RT][4];
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_f32_kernel(
           else xv[t][i] = row < rows && k < K ? x[row * K + k] : 0.0f;
         }
         g[i] = weight4<kWhole>(wg, k, K, c, F);
-        u[i] = weight4<kWhole>(wu, k, K, c, F);
+        if constexpr (PAIR) u[i] = weight4<kWhole>(wu, k, K, c, F);
       }
     };
     if (k0 + 4 * kDeep <= K && (int64_t)(blockIdx.x + 1) * kFewCols <= F) take(std::true_type());
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_f32_kernel(
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           gate[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[i][j], xv[t][i], gate[t][j], 0, 0, 0);
-          up[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[i][j], xv[t][i], up[t][j], 0, 0, 0);
+          if constexpr (PAIR) up[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[i][j], xv[t][i], up[t][j], 0, 0, 0);
         }
   }
   // lane: row n, results 4 q + r: column 4 (4 q + r) + j.  The upper half of the wavefronts hands its sums to the lower.
@@ -193,9 +193,12 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_f32_kernel(
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float *g = &sums[slot][0][t * 16 + n][4 * (4 * q + r) + j], *u = &sums[slot][1][t * 16 + n][4 * (4 * q + r) + j];
+          float *g = &sums[slot][0][t * 16 + n][4 * (4 * q + r) + j];
           *g = add ? gate[t][j][r] + *g : gate[t][j][r];
-          *u = add ? up[t][j][r] + *u : up[t][j][r];
+          if constexpr (PAIR) {
+            float *u = &sums[slot][1][t * 16 + n][4 * (4 * q + r) + j];
+            *u = add ? up[t][j][r] + *u : up[t][j][r];
+          }
         }
   };
   if (wave >= WAVES / 2) place(false);
@@ -210,34 +213,50 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_f32_kernel(
 #pragma unroll
     for (int v = 0; v < WAVES / 2; ++v) {
       g += sums[v][0][row][col];
-      u += sums[v][1][row][col];
+      if constexpr (PAIR) u += sums[v][1][row][col];
     }
-    h[row * F + f] = gate_of(act, g) * u;
+    finish(row, f, g, u);
   }
+}
+
+// What becomes of the sums of a row and column.
+template <typename T>
+struct Gated {
+  T *h;
+  int64_t F;
+  int act;
+  __device__ __forceinline__ void operator()(int row, int64_t f, float g, float u) const {
+    f32_to_elem(gate_of(act, g) * u, h[row * F + f]);
+  }
+};
+
+// PAIR: both products of x, else the first alone.
+template <bool PAIR, typename T, typename Finish>
+int few_launch(const void *x, const void *w0, const void *w1, const Finish &finish, int64_t rows, int64_t K, int64_t F,
+               hipStream_t s) {
+  const int64_t grid = (F + kFewCols - 1) / kFewCols;
+  if (rows > kGatedFewRows) return GA_EUNSUPPORTED;
+#define GA_FEW_LAUNCH(...)                                                                                             \
+  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)grid), dim3(8 * kWave), 0, s, (const T *)x, (const T *)w0,           \
+                     (const T *)w1, finish, (int)rows, K, F)
+  if constexpr (sizeof(T) == 4) GA_FEW_LAUNCH(few_f32_kernel<1, 8, PAIR, Finish>);
+  else if (rows <= 8) GA_FEW_LAUNCH(few_bf16_kernel<1, PAIR ? 4 : 2, PAIR, Finish>);
+  else GA_FEW_LAUNCH(few_bf16_kernel<2, 2, PAIR, Finish>);
+#undef GA_FEW_LAUNCH
+  return launch_status();
 }
 
 }  // namespace
 
 int gated_few_launch(const void *x, const void *wg, const void *wu, void *h, int64_t rows, int64_t K, int64_t F,
                      int act, int dtype, hipStream_t s) {
-  const int64_t grid = (F + kFewCols - 1) / kFewCols;
-  if (dtype == GA_F32) {
-    if (rows <= 16)
-      hipLaunchKernelGGL((gated_few_f32_kernel<1, 8>), dim3((unsigned)grid), dim3(8 * kWave), 0, s, (const float *)x,
-                         (const float *)wg, (const float *)wu, (float *)h, (int)rows, K, F, act);
-    else
-      return GA_EUNSUPPORTED;
-  } else {
-    if (rows <= 8)
-      hipLaunchKernelGGL((gated_few_bf16_kernel<1, 4>), dim3((unsigned)grid), dim3(2 * kTurns * kWave), 0, s,
-                         (const bf16_t *)x, (const bf16_t *)wg, (const bf16_t *)wu, (bf16_t *)h, (int)rows, K, F, act);
-    else if (rows <= 16)
-      hipLaunchKernelGGL((gated_few_bf16_kernel<2, 2>), dim3((unsigned)grid), dim3(2 * kTurns * kWave), 0, s,
-                         (const bf16_t *)x, (const bf16_t *)wg, (const bf16_t *)wu, (bf16_t *)h, (int)rows, K, F, act);
-    else
-      return GA_EUNSUPPORTED;
-  }
-  return launch_status();
+  return dtype == GA_F32 ? few_launch<true, float>(x, wg, wu, Gated<float>{(float *)h, F, act}, rows, K, F, s)
+                         : few_launch<true, bf16_t>(x, wg, wu, Gated<bf16_t>{(bf16_t *)h, F, act}, rows, K, F, s);
+}
+int linear_few_launch(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, int dtype,
+                      hipStream_t s) {
+  return dtype == GA_F32 ? few_launch<false, float>(x, w, nullptr, Ended<float>(end), rows, K, M, s)
+                         : few_launch<false, bf16_t>(x, w, nullptr, Ended<bf16_t>(end), rows, K, M, s);
 }
 
 }  // namespace ga

@@ -98,11 +98,11 @@ struct Tile {
     }
   }
   // Move i of a step.  `left`: values of k (across) or 16-byte pieces of k there are from this step on
-  __device__ __forceinline__ void move(const char *base, lds_char *to, int at, int left, int i) const {
+  __device__ __forceinline__ void move(const char *base, lds_char *to, int at, int left, int i, int bytes) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int kept = ACROSS ? i : i & 1;
     const uint32_t o = ACROSS ? off[kept] : off[kept] + i * ld8;
-    const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)range, 0x00020000);
+    const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, bytes, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + (at + (wave * kMoves + i) * 1024), 16,
                                              (ACROSS ? k[0] < left - i * kRowsMove : k[kept] < left) ? o : kOutside, 0, 0, 0);
   }
@@ -224,7 +224,11 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   typedef Mma<FP8> M;
   constexpr int kT = M::kTile;
   constexpr int kWaves = WM * WN, BM = WM * TM * kT, BN = WN * TN * kT;
-  constexpr int kPair = PAIR ? 2 : 1, BC = BN / kPair, TC = TN / kPair;      // columns of C
+  // One product of 256 columns of B across k is taken as two of 128, side by side: a wavefront then reads two tiles of either
+  // from one set of addresses (of four tiles in a row the addresses are spilled).
+  constexpr bool kSide = !PAIR && !FP8 && B_ACROSS && BN == 256;
+  constexpr int kPair = PAIR || kSide ? 2 : 1, BC = BN / kPair, TC = TN / kPair;   // columns of C in one of them
+  constexpr int kWide = kSide ? BN : BC;                     // and in all
   constexpr int kStepK = FP8 ? 128 : 64, kElem = FP8 ? 1 : 2;
   typedef Tile<A_ACROSS, BM, kWaves> TA;
   typedef Tile<B_ACROSS, BC, kWaves> TB;
@@ -234,10 +238,10 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   // 8 bits: scales of the tile's rows [block][wave row][row of the tile][tile], of the wavefronts' columns [block][..]
   __shared__ __attribute__((aligned(16))) uint8_t row_scales[FP8 ? BLOCKS * BM : 16], col_scales[FP8 ? BLOCKS * 8 : 16];
 
-  const int row_tiles = (int)((p.rows + BM - 1) / BM), col_tiles = (int)((p.cols + BC - 1) / BC);
+  const int row_tiles = (int)((p.rows + BM - 1) / BM), col_tiles = (int)((p.cols + kWide - 1) / kWide);
   int tr, tc;
   tile_of(blockIdx.x, row_tiles * col_tiles, row_tiles, col_tiles, tr, tc);
-  const int64_t row0 = (int64_t)tr * BM, col0 = (int64_t)tc * BC;
+  const int64_t row0 = (int64_t)tr * BM, col0 = (int64_t)tc * kWide;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / WN, wn = wave % WN;
   const int n = threadIdx.x & (kT - 1);
@@ -272,6 +276,9 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     b0_ptr = (const char *)(term ? p.b0[1] : p.b0[0]) + b_off;
     if constexpr (PAIR) b1_ptr = (const char *)p.b1[0] + b_off;
   };
+  // Of the columns on the side, those behind the last one are other values of the operand, for columns of C that are not
+  // stored; what lies behind the operand is out of range.
+  int side_range = 0;
   // What is left of k for the step to be fetched: values (across) and pieces of 16 bytes (by k, whose rows are
   // whole pieces).
   int a_left = 0, b_left = 0;
@@ -280,15 +287,18 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     const int pieces = (values * kElem + 15) / 16;
     a_left = A_ACROSS ? values : pieces;
     b_left = B_ACROSS ? values : pieces;
+    if constexpr (kSide)
+      side_range = (int)min(max((p.K - (int64_t)in_seg * kStepK) * p.ldb - (col0 + BC) * kElem, (int64_t)0), (int64_t)0x7fffffff);
   };
   // Half of the step's moves at a time: all in a row would hold up the products behind them.
   auto fetch = [&](lds_char *to, int part) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       if (i % 2 != part) continue;
-      if (i < TA::kMoves) ta.move(a_ptr, to, 0, a_left, i);
-      else if (i < TA::kMoves + TB::kMoves) tb.move(b0_ptr, to, TA::kBytes, b_left, i - TA::kMoves);
-      else tb.move(b1_ptr, to, TA::kBytes + TB::kBytes, b_left, i - TA::kMoves - TB::kMoves);
+      if (i < TA::kMoves) ta.move(a_ptr, to, 0, a_left, i, (int)ta.range);
+      else if (i < TA::kMoves + TB::kMoves) tb.move(b0_ptr, to, TA::kBytes, b_left, i - TA::kMoves, (int)tb.range);
+      else if constexpr (kSide) tb.move(b0_ptr + BC * kElem, to, TA::kBytes + TB::kBytes, b_left, i - TA::kMoves - TB::kMoves, side_range);
+      else tb.move(b1_ptr, to, TA::kBytes + TB::kBytes, b_left, i - TA::kMoves - TB::kMoves, (int)tb.range);
     }
   };
   auto advance = [&]() {
@@ -308,7 +318,7 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
     else return TA::read16(t, 0, lane_a, i, half);
   };
   auto read_b = [&](const lds_char *t, int j, int half) {
-    const bool second = PAIR && j >= TC;
+    const bool second = kPair == 2 && j >= TC;
     const int base = TA::kBytes + (second ? TB::kBytes : 0), i = second ? j - TC : j;
     if constexpr (FP8) return TB::read32(t, base, lane_b, i, half);
     else return TB::read16(t, base, lane_b, i, half);
@@ -457,9 +467,12 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   static_assert(kPass > 0 && kShare * (kWaves / 2) == kStage, "a wavefront's part holds a pass");
   landed<0>();                           // every wavefront is done with the tiles
   lds_char *const mine = (wave < kWaves / 2 ? L0 : L1) + wave % (kWaves / 2) * kShare;
-  const int64_t wave_row = row0 + wm * TM * kT, wave_col = col0 + wn * kCols;
-  const bool inside = wave_row + TM * kT <= p.rows && wave_col + kCols <= p.cols;
+  const int64_t wave_row = row0 + wm * TM * kT;
   epi.visit([&](const auto &e) {
+#pragma unroll
+    for (int j0 = 0; j0 < (kSide ? TN : TC); j0 += TC) {     // the second product's columns are those behind the first's
+    const int64_t wave_col = col0 + (kSide && j0 ? BC : 0) + wn * kCols;
+    const bool inside = wave_row + TM * kT <= p.rows && wave_col + kCols <= p.cols;
     // hidden here, so that addresses are reckoned where they are used and not for all forms at once before the choice
     int lane = threadIdx.x & (kWave - 1);
     asm volatile("" : "+v"(lane));
@@ -475,8 +488,8 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
             floatx4 u, v;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              u[r] = acc[i][j][4 * g + r];
-              v[r] = acc[i][PAIR ? j + TC : j][4 * g + r];
+              u[r] = acc[i][j0 + j][4 * g + r];
+              v[r] = acc[i][PAIR ? j + TC : j0 + j][4 * g + r];
             }
             typename Epi::bits o[kOut];
             const int col = j * kT + g * 8 + q * 4, row = (i - i0) * kT + n;
@@ -508,6 +521,7 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
         }
       }
       asm volatile("" ::: "memory");
+    }
     }
   });
 }
@@ -677,14 +691,16 @@ int tile_mm_launch_as(const TileMm &p, const Epi &epi, hipStream_t s) {
 }
 
 constexpr int kMostBlocks = 256;         // of 128 along k, whose scales have room in LDS
-template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, typename Epi>
+// SMALL: never 256 x 256, which some epilogues have no registers for and parts of sums never fill.
+template <bool FP8, bool A_ACROSS, bool B_ACROSS, bool PAIR, bool SMALL = false, typename Epi>
 int tile_mm_launch(const TileMm &p, const Epi &epi, hipStream_t s) {
   constexpr int kHigh = FP8 ? 4 : 8, kLow = kHigh / 2, kWide = FP8 ? 2 : 4;    // tiles of a wavefront
   const int blocks = FP8 ? (int)((p.K + 127) / 128) : 0;
   if (blocks > kMostBlocks) return GA_EUNSUPPORTED;
   const int tile = tile_for(p, PAIR);
-  if (tile == kTile256 && blocks <= 64)
-    return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, FP8 ? 64 : 0>(p, epi, s);
+  if constexpr (!SMALL)
+    if (tile == kTile256 && blocks <= 64)
+      return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 4, kHigh, kWide, FP8 ? 64 : 0>(p, epi, s);
   if constexpr (!FP8) {
     if (tile == kTile64) return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, 2, 4, 0>(p, epi, s);
     return tile_mm_launch_as<FP8, A_ACROSS, B_ACROSS, PAIR, 2, 2, kLow, kWide, 0>(p, epi, s);

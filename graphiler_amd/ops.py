@@ -1874,3 +1874,154 @@ def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer
             out.data_ptr(), lse.data_ptr(), q_pointer.data_ptr(), k_pointer.data_ptr(), sizes[0], gq.data_ptr(),
             gk.data_ptr(), gv.data_ptr(), *sizes[1:], bool(causal), scale, dt, _ptr(ws), n)
     return gq, gk, gv
+
+
+# ------------------------------- what is around that attention: projections and embedding rows ----
+def _gate_or_none(name) -> int:
+    return capi.GA_GATE_NONE if name is None else _gate(name)
+
+
+def _linear_act_args(x, weight, bias, residual, activation):
+    act = _gate_or_none(activation)
+    dt = _check_rows(x, "x")
+    rows, k = int(x.shape[0]), int(x.shape[1])
+    _check_input(weight, "weight")
+    if weight.dim() != 2 or weight.shape[0] != k or weight.shape[1] == 0:
+        raise RuntimeError("weight must be (K, M)")
+    m = int(weight.shape[1])
+    _check_like(weight, "weight", (k, m), x)
+    if bias is not None:
+        _check_like(bias, "bias", (m,), x)
+    if residual is not None:
+        _check_like(residual, "residual", (rows, m), x)
+    return act, dt, rows, k, m
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        _not_recorded("linear_act")
+        y = _linear_act(x, weight, bias, residual, activation)
+        ctx.activation, ctx.residual = activation, residual is not None
+        ctx.save_for_backward(x, weight, bias)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y):
+        _not_recorded("linear_act")
+        x, weight, bias = ctx.saved_tensors
+        gx = gw = gb = None
+        if any(ctx.needs_input_grad[:3]):
+            gx, gw, gb = _linear_act_backward(grad_y.contiguous(), x, weight, bias, ctx.activation,
+                                              ctx.needs_input_grad[:3])
+        return gx, gw, gb, grad_y if ctx.residual and ctx.needs_input_grad[3] else None, None
+
+
+def _linear_act(x, weight, bias, residual, activation):
+    act, dt, rows, k, m = _linear_act_args(x, weight, bias, residual, activation)
+    if rows > 16:                       # fewer are read from any address
+        x, weight = _whole_pieces(x), _whole_pieces(weight)
+    y = torch.empty((rows, m), dtype=x.dtype, device=x.device)
+    n = capi.load().ga_linear_act_workspace_bytes(rows, k, m, dt)
+    ws = _scratch(n, x.device)
+    _launch("ga_linear_act", x.get_device(), x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(),
+            rows, k, m, act, dt, _ptr(ws), n)
+    return y
+
+
+def linear_act(x, weight, bias=None, activation=None, residual=None):
+    """act(x @ weight + bias) + residual from one kernel (:func:`linear` is the bare product): the
+    projections around an attention layer and the halves of a plain feed-forward block.  x (rows, K), weight (K, M),
+    bias (M,), residual (rows, M), of one dtype (float32 or bfloat16); activation None | "silu" | "gelu" | "relu" as
+    in :func:`gated_linear`.  Sums, activation and additions are fp32 and rounded once; fp32 products are
+    those of :func:`gated_linear`.  Differentiable in all four tensors (backward mode)."""
+    if _wants_grad("linear_act", x, weight, bias, residual):
+        return _LinearAct.apply(x, weight, bias, residual, activation)
+    return _linear_act(x, weight, bias, residual, activation)
+
+
+def _linear_act_backward(grad_y, x, weight, bias, activation, wanted):
+    act, dt, rows, k, m = _linear_act_args(x, weight, bias, None, activation)
+    _check_like(grad_y, "grad_y", (rows, m), x)
+    grad_y, x, weight = _whole_pieces(grad_y), _whole_pieces(x), _whole_pieces(weight)
+    gx = torch.empty_like(x) if wanted[0] else None
+    gw = torch.empty_like(weight) if wanted[1] else None
+    gb = torch.empty_like(bias) if wanted[2] and bias is not None else None
+    n = capi.load().ga_linear_act_backward_workspace_bytes(rows, k, m, act, dt)
+    ws = _scratch(n, x.device)
+    _launch("ga_linear_act_backward", x.get_device(), grad_y.data_ptr(), x.data_ptr(), weight.data_ptr(), _ptr(bias),
+            _ptr(gx), _ptr(gw), _ptr(gb), rows, k, m, act, dt, _ptr(ws), n)
+    return gx, gw, gb
+
+
+def linear_act_backward(grad_y, x, weight, bias=None, activation=None):
+    """Gradients of :func:`linear_act`: (of x, of weight, of bias or None); that of the residual is grad_y
+    itself.  x @ weight is formed again where there is an activation; nothing but the operands is kept from the
+    forward pass.  The results have no gradients of their own."""
+    _check_seen("linear_act_backward", grad_y, x, weight, bias)
+    return _linear_act_backward(grad_y, x, weight, bias, activation, (True, True, True))
+
+
+_ID_BITS = {torch.int64: 64, torch.int32: 32}
+
+
+def _check_ids(ids, device) -> int:
+    _check_input(ids, "ids")
+    if ids.dtype not in _ID_BITS or ids.get_device() != device:
+        raise RuntimeError("ids must be int64 or int32, on the device of the rows")
+    return _ID_BITS[ids.dtype]
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale):
+        _not_recorded("embedding")
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale = int(table.shape[0]), scale
+        return _embedding(table, ids, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y):
+        _not_recorded("embedding")
+        return embedding_backward(grad_y.contiguous(), ctx.saved_tensors[0], ctx.rows, ctx.scale), None, None
+
+
+def _embedding(table, ids, scale):
+    dt = _check_rows(table, "table")
+    bits = _check_ids(ids, table.get_device())
+    cols = int(table.shape[1])
+    y = torch.empty((*ids.shape, cols), dtype=table.dtype, device=table.device)
+    if y.numel():
+        _launch("ga_embedding", table.get_device(), table.data_ptr(), ids.data_ptr(), bits, y.data_ptr(), ids.numel(),
+                int(table.shape[0]), cols, float(scale), dt)
+    return y
+
+
+def embedding(table, ids, scale: float = 1.0):
+    """scale * table[ids]: the rows that nodes (or a sequence's tokens) begin with, ids of any shape, int64 or int32.
+    An id outside the table (-1: padding) gives zeros.  The product is rounded once.  Differentiable in table (backward
+    mode); its gradient is summed in the order of the places, without atomics."""
+    if _wants_grad("embedding", table):
+        return _Embedding.apply(table, ids, scale)
+    return _embedding(table, ids, scale)
+
+
+def embedding_backward(grad_y, ids, rows: int, scale: float = 1.0):
+    """Gradient of the (rows, cols) table of :func:`embedding`: scale times the sum of the rows of grad_y whose id is
+    the row's; zeros for rows that no id names.  Summed in fp32, rounded once; the result has no gradient of its own."""
+    _check_seen("embedding_backward", grad_y)
+    _check_input(grad_y, "grad_y")
+    dt = _feat_dtype(grad_y, "grad_y")
+    bits = _check_ids(ids, grad_y.get_device())
+    if grad_y.dim() != ids.dim() + 1 or grad_y.shape[:-1] != ids.shape or grad_y.shape[-1] == 0 or rows < 0:
+        raise RuntimeError("grad_y must have a row for each id, and rows must not be negative")
+    cols = int(grad_y.shape[-1])
+    grad = torch.empty((int(rows), cols), dtype=grad_y.dtype, device=grad_y.device)
+    if grad.numel():
+        n = capi.load().ga_embedding_backward_workspace_bytes(ids.numel(), int(rows), cols)
+        ws = _scratch(n, grad.device)
+        _launch("ga_embedding_backward", grad_y.get_device(), grad_y.data_ptr(), ids.data_ptr(), bits, grad.data_ptr(),
+                ids.numel(), int(rows), cols, float(scale), dt, _ptr(ws), n)
+    return grad

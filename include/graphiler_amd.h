@@ -817,7 +817,7 @@ int ga_rms_norm_backward(const void *grad_y, const void *sum, const void *weight
  * the fp32 instruction.  With more than 16 rows, bf16 operands whose rows are whole 16-byte pieces have to
  * be 16-byte aligned.  GA_EUNSUPPORTED when K or F exceeds 2^20.
  */
-enum ga_gate { GA_GATE_SILU = 0, GA_GATE_GELU = 1, GA_GATE_RELU = 2 };
+enum ga_gate { GA_GATE_NONE = -1 /* ga_linear_act only */, GA_GATE_SILU = 0, GA_GATE_GELU = 1, GA_GATE_RELU = 2 };
 size_t ga_gated_linear_workspace_bytes(int64_t rows, int64_t K, int64_t F, int dtype);
 int ga_gated_linear(const void *x, const void *w_gate, const void *w_up, void *h, int64_t rows, int64_t K,
                     int64_t F, int activation, int dtype, void *workspace, size_t workspace_bytes,
@@ -892,6 +892,44 @@ int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q
                                   void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
                                   int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
                                   size_t workspace_bytes, ga_stream_t stream);
+
+/*
+ * A projection with what surrounds it: y = act(x @ weight + bias) + residual, x (rows, K), weight (K, M), bias (M) or NULL,
+ * residual (rows, M) or NULL, y (rows, M), all of `dtype`; sums, activation and additions in fp32, y rounded once.  activation:
+ * ga_gate, GA_GATE_NONE for none.  y may be residual itself.  fp32 products and alignment as ga_gated_linear has them.
+ * GA_EUNSUPPORTED when K or M exceeds 2^20.
+ */
+size_t ga_linear_act_workspace_bytes(int64_t rows, int64_t K, int64_t M, int dtype);
+int ga_linear_act(const void *x, const void *weight, const void *bias, const void *residual, void *y, int64_t rows, int64_t K,
+                  int64_t M, int activation, int dtype, void *workspace, size_t workspace_bytes, ga_stream_t stream);
+
+/*
+ * Its gradients: with z = x @ weight + bias (formed again where there is an activation) and dz = grad_y act'(z) (rounded to
+ * bf16 where the tensors are bf16), grad_x = dz @ weight^T, grad_weight = x^T @ dz, grad_bias = sum over rows of dz; that of
+ * the residual is grad_y itself.  Each may be NULL: not wanted.  The slope of relu at 0 is 0.  fp32 products are those of
+ * pieces.  No order of a sum depends on anything but the sizes.  bf16 operands whose rows are whole 16-byte pieces have to
+ * be 16-byte aligned.
+ */
+size_t ga_linear_act_backward_workspace_bytes(int64_t rows, int64_t K, int64_t M, int activation, int dtype);
+int ga_linear_act_backward(const void *grad_y, const void *x, const void *weight, const void *bias, void *grad_x,
+                           void *grad_weight, void *grad_bias, int64_t rows, int64_t K, int64_t M, int activation, int dtype,
+                           void *workspace, size_t workspace_bytes, ga_stream_t stream);
+
+/*
+ * Embedding rows: y[i] = scale * table[ids[i]], zeros for an id outside [0, n_table).  table (n_table, cols) and y (n_ids, cols)
+ * of `dtype`, ids int64 (idx_bits 64) or int32 (idx_bits 32); the product is rounded once.
+ */
+int ga_embedding(const void *table, const void *ids, int idx_bits, void *y, int64_t n_ids, int64_t n_table, int64_t cols,
+                 float scale, int dtype, ga_stream_t stream);
+
+/*
+ * The table's gradient: grad_table[v] = scale * sum of grad_y[i] over the i with ids[i] = v, in fp32 in the order of the i
+ * (inside runs whose bounds depend on the ids alone), rounded once; zeros for rows that no id names.  Ids outside the table
+ * give nothing.  workspace: 256-byte aligned.  GA_EUNSUPPORTED when n_ids or n_table exceeds 2^31 - 2.
+ */
+size_t ga_embedding_backward_workspace_bytes(int64_t n_ids, int64_t n_table, int64_t cols);
+int ga_embedding_backward(const void *grad_y, const void *ids, int idx_bits, void *grad_table, int64_t n_ids, int64_t n_table,
+                          int64_t cols, float scale, int dtype, void *workspace, size_t workspace_bytes, ga_stream_t stream);
 
 #ifdef __cplusplus
 }
