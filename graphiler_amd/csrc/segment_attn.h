@@ -35,6 +35,7 @@ struct SegAttn {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;       // bytes between rows and heads
   int segments, heads, group, dim, causal;
   float scale;
+  int q_whole;                           // rows of q are whole 16-byte pieces at 4-byte addresses
 };
 
 __device__ __forceinline__ int64_t clamped(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
@@ -91,14 +92,106 @@ inline int64_t segment_tiles(int64_t rows, int64_t pack, int64_t segments, int b
   return rows * pack / bm + segments + 2;
 }
 
+// Row of result r in half 0; in half 1 it is four more.
+__device__ __forceinline__ constexpr int result_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// How a launch is cut.  Shared: WAVES wavefronts with 32 rows each go through the same tiles of DEEP rows of the other side.
+// Apart: the same 32 rows for all, every wavefront goes through tiles of its own, and their sums are added up at the end.
+template <int WAVES_, int DEEP_, int STAGES_, bool APART_>
+struct Form {
+  static constexpr int kWaves = WAVES_, kDeep = DEEP_, kStages = STAGES_;
+  static constexpr bool kApart = APART_;
+  static constexpr int kRows = APART_ ? 32 : 32 * WAVES_;    // of a workgroup
+  static constexpr int kMovers = APART_ ? 1 : WAVES_;        // wavefronts that fetch a tile
+};
+
 // One of `heads` times `tiles` workgroups: the eight XCDs (workgroups are dealt to them in turn) get a run of neighbours
-// each, so that the tiles of a head share its keys in one L2.
-__device__ __forceinline__ void head_tile(int64_t id, int64_t tiles, int heads, int &head, int64_t &tile) {
+// each.  One behind the other lie the tiles of a head, which share its keys in one L2, or, of short segments, the heads of
+// a tile, which share cache lines.
+__device__ __forceinline__ void head_tile(int64_t id, int64_t tiles, int heads, bool by_tile, int &head, int64_t &tile) {
   const int64_t all = tiles * heads, per = all / 8, more = all % 8, x = id & 7, at = id >> 3;
-  const int64_t j = x * per + min(x, more) + at;
-  head = __builtin_amdgcn_readfirstlane((int)(j / tiles));
-  tile = scalar(j % tiles);
+  const int64_t j = x * per + min(x, more) + at, inner = by_tile ? heads : tiles;
+  const int64_t outer = j / inner, in = j % inner;
+  head = __builtin_amdgcn_readfirstlane((int)(by_tile ? in : outer));
+  tile = scalar(by_tile ? outer : in);
 }
+
+// A wavefront's own loads have arrived, and what it read in LDS is read.
+__device__ __forceinline__ void arrived() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  asm volatile("" ::: "memory");
+}
+
+// Goes through tiles [begin, end): fetch(to) sends for the next of the wavefront's tiles, if there is one, into an LDS
+// buffer, use(tile, there) multiplies one that has arrived.
+template <typename F, typename Fetch, typename Use>
+__device__ __forceinline__ void through_tiles(int begin, int end, int wave, lds_char *L0, lds_char *L1, Fetch fetch, Use use) {
+  constexpr int kStep = F::kApart ? F::kWaves : 1;
+  const int first = F::kApart ? begin + wave : begin;
+  fetch(L0);
+  if constexpr (F::kStages == 1) {
+    for (int t = first; t < end; t += kStep) {
+      if constexpr (F::kApart) arrived();
+      else landed<0>();
+      use(t, L0);
+      if (t + kStep < end) {             // the same for all that share the tile
+        if constexpr (F::kApart) arrived();
+        else landed<0>();
+        fetch(L0);
+      }
+    }
+  } else {
+    auto step = [&](int t, lds_char *here, lds_char *next) {
+      if constexpr (F::kApart) arrived();
+      else landed<0>();                  // this tile is there, and every wavefront is done with the one before
+      fetch(next);
+      use(t, here);
+    };
+    int t = first;
+    for (; t + kStep < end; t += 2 * kStep) {
+      step(t, L0, L1);
+      step(t + kStep, L1, L0);
+    }
+    if (t < end) step(t, L0, L1);
+  }
+}
+
+// Sums of the wavefronts that go through tiles apart: every one leaves its results, weighed by f, in `mine` as 32 rows of columns,
+// and takes WIDE / WAVES of the columns of all: of row n those from column part() on.  The region of wavefront w is `each` bytes
+// behind that of the one before.
+template <int WIDE, int WAVES>
+struct Gathered {
+  static constexpr int kOwn = WIDE / WAVES / 2;              // columns of a lane
+  float f[kOwn];
+  static __device__ __forceinline__ int part(int wave) { return (2 * wave + ((threadIdx.x >> 5) & 1)) * kOwn; }
+  static __device__ __forceinline__ void leave(lds_char *mine, const floatx16 (&o)[WIDE / 32], float f) {
+    const int n = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int d = 0; d < WIDE / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        *reinterpret_cast<__attribute__((address_space(3))) float *>(mine + ((d * 32 + result_row(r) + 4 * h) * 32 + n) * 4) = o[d][r] * f;
+  }
+  __device__ __forceinline__ void take(const lds_char *all, int each, int wave) {
+    const int n = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      f[j] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+        f[j] += *reinterpret_cast<const __attribute__((address_space(3))) float *>(all + w * each + ((part(wave) + j) * 32 + n) * 4);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T *row, bool there, int dim, int wave, float by) const {
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      const int c = part(wave) + j;
+      if (there && c < dim) f32_to_elem(f[j] * by, row[c]);
+    }
+  }
+};
 
 template <typename T> struct Elem;
 template <> struct Elem<bf16_t> { static constexpr int kPiece = 8; };
@@ -229,14 +322,25 @@ struct RowMoves {
   }
 };
 
-// A lane's row operand straight from memory: `row` (or zeros where there is none), 32 bytes a step.
+// A lane's row operand straight from memory, 32 bytes a step: the row `off` bytes from `base` (the same for the wavefront),
+// zeros where there is none.  `whole`: rows are whole 16-byte pieces, 4-byte aligned at least.
 template <typename T, int WIDE>
-__device__ __forceinline__ void load_row(const char *row, bool there, int dim, uintx4 (&f)[Rows<T, WIDE>::kSteps]) {
+__device__ __forceinline__ void load_row(const char *base, uint32_t off, bool there, int dim, bool whole,
+                                         uintx4 (&f)[Rows<T, WIDE>::kSteps]) {
   const int h = (threadIdx.x >> 5) & 1;
+  if (whole) {
+    const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-  for (int s = 0; s < Rows<T, WIDE>::kSteps; ++s) {
-    const int c = (2 * s + h) * Elem<T>::kPiece;
-    f[s] = load_piece<T>((const T *)row + c, there ? dim - c : 0);
+    for (int s = 0; s < Rows<T, WIDE>::kSteps; ++s)
+      f[s] = __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(
+                                            r, there && (2 * s + h) * Elem<T>::kPiece < dim ? off + (2 * s + h) * 16 : kOutside, 0, 0));
+  } else {
+#pragma unroll
+    for (int s = 0; s < Rows<T, WIDE>::kSteps; ++s) {
+      const int c = (2 * s + h) * Elem<T>::kPiece;
+      f[s] = load_piece<T>((const T *)(base + off) + c, there ? dim - c : 0);
+      __builtin_amdgcn_sched_barrier(0);                     // or the addresses of all take the registers
+    }
   }
 }
 
@@ -250,9 +354,6 @@ __device__ __forceinline__ uintx4 operand_of(const floatx16 &p, int i) {
     return uintx4{__float_as_uint(p[4 * i]), __float_as_uint(p[4 * i + 1]), __float_as_uint(p[4 * i + 2]),
                   __float_as_uint(p[4 * i + 3])};
 }
-// row of result r in half h
-__device__ __forceinline__ constexpr int result_row(int r) { return (r & 3) + 8 * (r >> 2); }
-
 // Zeros in the place of values that are not finite; whether there were any.
 template <typename T>
 __device__ __forceinline__ bool cleaned(uintx4 &a) {
@@ -276,7 +377,8 @@ __device__ __forceinline__ bool cleaned(uintx4 &a) {
 // path: one tile of columns at a time, so that it takes no registers of the common one.
 template <typename T, int WIDE>
 __device__ __forceinline__ void add_not_finite(const lds_char *t, int r, bool counts, floatx16 (&acc)[Rows<T, WIDE>::kCols]) {
-  const int h = (threadIdx.x >> 5) & 1;
+  int h = (threadIdx.x >> 5) & 1;
+  asm volatile("" : "+v"(h));            // or the places of all values are reckoned ahead of every loop, and kept
 #pragma unroll
   for (int d = 0; d < Rows<T, WIDE>::kCols; ++d)
 #pragma unroll

@@ -19,6 +19,7 @@ struct Forward : SegAttn {
   int64_t out_row, out_head;             // values
   int64_t tiles;                         // per head
   int pack;                              // heads of a group whose rows are one tile's: 1 or group
+  int cutting;
   int splits;                            // parts of the keys, each its own partial result
   float *parts;                          // (splits, nq, heads, dim) sums, then (splits, nq, heads, 2) maxima and sums
 };
@@ -45,6 +46,7 @@ struct Running {
     constexpr int kB = KEYS / 32;
     const int h = (threadIdx.x >> 5) & 1;
     floatx16 s[kB];
+    __builtin_amdgcn_s_setprio(1);       // products first: the other wavefront of the SIMD has its exponentials meanwhile
 #pragma unroll
     for (int b = 0; b < kB; ++b) {
 #pragma unroll
@@ -56,8 +58,9 @@ struct Running {
 #pragma unroll
       for (int b = 0; b < kB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[b][r] = b * 32 + result_row(r) + 4 * h < seen ? s[b][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[b][r] = b * 32 + result_row(r) < seen - 4 * h ? s[b][r] : -INFINITY;
     }
+    __builtin_amdgcn_s_setprio(0);
     float top = s[0][0];
 #pragma unroll
     for (int b = 0; b < kB; ++b)
@@ -83,6 +86,7 @@ struct Running {
       }
 #pragma unroll
     for (int b = 0; b < kB; ++b) {
+      if (b == 0) __builtin_amdgcn_s_setprio(1);
       bool found = false;
 #pragma unroll
       for (int i = 0; i < R::kParts; ++i) {
@@ -110,29 +114,31 @@ __device__ __forceinline__ float lse_of(float most, float sum) {
   return sum == 0.0f ? -INFINITY : (most + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// WAVES wavefronts with 32 queries each share tiles of KEYS keys.
-template <typename T, int WIDE, int WAVES, int KEYS>
+template <typename T, int WIDE, typename F>
 __device__ __forceinline__ void segment_attn(const Forward &p) {
   typedef Rows<T, WIDE> R;
-  typedef RowMoves<T, WIDE, KEYS, WAVES> Moves;
-  constexpr int BM = 32 * WAVES, kStage = 2 * Moves::kBytes;
-  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage];
+  constexpr int KEYS = F::kDeep;
+  typedef RowMoves<T, WIDE, KEYS, F::kMovers> Moves;
+  constexpr int kStage = 2 * Moves::kBytes, kRegions = F::kApart ? F::kWaves : 1, kLds = kStage * kRegions;
+  __shared__ __attribute__((aligned(1024))) char stage0[kLds], stage1[F::kStages == 2 ? kLds : 16];
   int head;
   int64_t tile;
-  head_tile(blockIdx.x, p.tiles, p.heads / p.pack, head, tile);
+  head_tile(blockIdx.x, p.tiles, p.heads / p.pack, F::kWaves == 1, head, tile);
   if (p.causal) tile = p.tiles - 1 - tile;                   // those with the most keys first
   Segment seg;
-  if (!segment_of<BM>(p, tile, p.pack, false, seg)) return;
+  if (!segment_of<F::kRows>(p, tile, p.pack, false, seg)) return;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x & (kWave - 1), n = lane & 31, h = lane >> 5;
   const int kv = p.pack > 1 ? head : head / p.group;
-  const int rows = seg.q_len * p.pack, first = seg.tile * BM + wave * 32, row = first + n;
+  const int rows = seg.q_len * p.pack, first = seg.tile * F::kRows + (F::kApart ? 0 : wave * 32), row = first + n;
   const int query = row / p.pack, q_head = p.pack > 1 ? head * p.pack + row % p.pack : head;
   const bool there = row < rows;
 
   uintx4 q[R::kSteps];
-  load_row<T, WIDE>((const char *)p.q + (seg.q0 + query) * p.q_row + q_head * p.q_head, there, p.dim, q);
+  const int query0 = first / p.pack, head0 = p.pack > 1 ? head * p.pack : head;          // of row `first`, and of its group
+  load_row<T, WIDE>((const char *)p.q + (seg.q0 + query0) * p.q_row + head0 * p.q_head,
+                    (uint32_t)((query - query0) * p.q_row + (q_head - head0) * p.q_head), there, p.dim, p.q_whole, q);
   if (p.scale < 0.0f) {                  // the larger score then is the smaller product
 #pragma unroll
     for (int i = 0; i < R::kSteps; ++i)
@@ -144,10 +150,10 @@ __device__ __forceinline__ void segment_attn(const Forward &p) {
   // keys seen: by the lane's query, by all and by any of the wavefront's and of the workgroup's
   const int more = seg.k_len - seg.q_len;
   const int seen = p.causal ? max(0, min(seg.k_len, query + 1 + more)) : seg.k_len;
-  const int by_all = p.causal ? max(0, min(seg.k_len, first / p.pack + 1 + more)) : seg.k_len;
+  const int by_all = p.causal ? max(0, min(seg.k_len, query0 + 1 + more)) : seg.k_len;
   const int last = min(first + 31, rows - 1) / p.pack;
   const int by_any = first >= rows ? 0 : p.causal ? max(0, min(seg.k_len, last + 1 + more)) : seg.k_len;
-  const int block_last = min(seg.tile * BM + BM, rows) - 1;
+  const int block_last = min(seg.tile * F::kRows + F::kRows, rows) - 1;
   const int wanted = p.causal ? max(0, min(seg.k_len, block_last / p.pack + 1 + more)) : seg.k_len;
   int begin = 0, end = (wanted + KEYS - 1) / KEYS;
   if (p.splits > 1) {
@@ -156,61 +162,77 @@ __device__ __forceinline__ void segment_attn(const Forward &p) {
     end = min(end, begin + share);
   }
 
+  constexpr int kTurn = F::kApart ? F::kWaves : 1;           // tiles from one of the wavefront's to its next
+  int to_fetch = F::kApart ? begin + wave : begin;
   Moves mk, mv;
-  mk.init(p.k_row, p.dim, wave);
-  mv.init(p.v_row, p.dim, wave);
-  const char *k_at = (const char *)p.k + (seg.k0 + (int64_t)begin * KEYS) * p.k_row + kv * p.k_head;
-  const char *v_at = (const char *)p.v + (seg.k0 + (int64_t)begin * KEYS) * p.v_row + kv * p.v_head;
-  int to_fetch = begin;
+  mk.init(p.k_row, p.dim, F::kApart ? 0 : wave);
+  mv.init(p.v_row, p.dim, F::kApart ? 0 : wave);
+  const char *k_at = (const char *)p.k + (seg.k0 + (int64_t)to_fetch * KEYS) * p.k_row + kv * p.k_head;
+  const char *v_at = (const char *)p.v + (seg.k0 + (int64_t)to_fetch * KEYS) * p.v_row + kv * p.v_head;
   auto fetch = [&](lds_char *to) {
     if (to_fetch >= end) return;
     const int left = seg.k_len - to_fetch * KEYS;
     mk.move(k_at, left, to);
     mv.move(v_at, left, to + Moves::kBytes);
-    k_at += KEYS * p.k_row;
-    v_at += KEYS * p.v_row;
-    ++to_fetch;
+    k_at += kTurn * KEYS * p.k_row;
+    v_at += kTurn * KEYS * p.v_row;
+    to_fetch += kTurn;
   };
   const int row_at = R::row_at(), col_at = R::col_at();
   Running<T, WIDE> st;
   st.clear();
-  auto step = [&](int t, lds_char *here, lds_char *next) {
-    landed<0>();                         // this tile is there, and every wavefront is done with the one before
-    fetch(next);
+  auto use = [&](int t, const lds_char *here) {
     const int key0 = t * KEYS;
-    if (key0 < by_any) {
-      if (key0 + KEYS <= by_all) st.template tile<KEYS, false>(here, here + Moves::kBytes, row_at, col_at, q, c, KEYS);
-      else st.template tile<KEYS, true>(here, here + Moves::kBytes, row_at, col_at, q, c, seen - key0);
-    }
+    if (key0 >= by_any) return;
+    if (key0 + KEYS <= by_all) st.template tile<KEYS, false>(here, here + Moves::kBytes, row_at, col_at, q, c, KEYS);
+    else st.template tile<KEYS, true>(here, here + Moves::kBytes, row_at, col_at, q, c, seen - key0);
   };
-  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1;
-  fetch(L0);
-  int t = begin;
-  for (; t + 2 <= end; t += 2) {
-    step(t, L0, L1);
-    step(t + 1, L1, L0);
-  }
-  if (t < end) step(t, L0, L1);
+  const int region = F::kApart ? wave * kStage : 0;
+  through_tiles<F>(begin, end, wave, (lds_char *)stage0 + region, (lds_char *)stage1 + (F::kStages == 2 ? region : 0), fetch, use);
 
-  const float sum = st.sum + other_half(st.sum);
+  float sum = st.sum + other_half(st.sum), most = st.most;
   const int64_t at = seg.q0 + query;
+  Gathered<WIDE, F::kApart ? F::kWaves : 1> all;
+  if constexpr (F::kApart) {
+    static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
+    __shared__ float maxima[F::kWaves][32], sums[F::kWaves][32];
+    if (h == 0) {
+      maxima[wave][n] = most;
+      sums[wave][n] = sum;
+    }
+    __syncthreads();
+    const float own = most;
+#pragma unroll
+    for (int w = 0; w < F::kWaves; ++w) most = fmaxf(most, maxima[w][n]);
+    const float from = most == -INFINITY ? 0.0f : most;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < F::kWaves; ++w) sum += sums[w][n] * __builtin_amdgcn_exp2f(maxima[w][n] - from);
+    all.leave((lds_char *)stage0 + region, st.o, __builtin_amdgcn_exp2f(own - from));
+    __syncthreads();
+    all.take((const lds_char *)stage0, kStage, wave);
+  }
+  const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (p.splits > 1) {
-    const int64_t all = p.nq * p.heads, id = (int64_t)blockIdx.y * all + at * p.heads + q_head;
-    store_row<float, R::kCols>(p.parts + id * p.dim, there, p.dim, st.o, 1.0f);
-    if (there && h == 0) {
-      float *ml = p.parts + (int64_t)p.splits * all * p.dim + id * 2;
-      ml[0] = st.most;
+    const int64_t n_all = p.nq * p.heads, id = (int64_t)blockIdx.y * n_all + at * p.heads + q_head;
+    if constexpr (F::kApart) all.store(p.parts + id * p.dim, there, p.dim, wave, 1.0f);
+    else store_row<float, R::kCols>(p.parts + id * p.dim, there, p.dim, st.o, 1.0f);
+    if (there && h == 0 && (!F::kApart || wave == 0)) {
+      float *ml = p.parts + (int64_t)p.splits * n_all * p.dim + id * 2;
+      ml[0] = most;
       ml[1] = sum;
     }
     return;
   }
-  store_row<T, R::kCols>((T *)p.out + at * p.out_row + q_head * p.out_head, there, p.dim, st.o,
-                         sum == 0.0f ? 0.0f : 1.0f / sum);
-  if (p.lse && there && h == 0) p.lse[q_head * p.nq + at] = lse_of(st.most, sum);
+  T *out = (T *)p.out + at * p.out_row + q_head * p.out_head;
+  if constexpr (F::kApart) all.store(out, there, p.dim, wave, by);
+  else store_row<T, R::kCols>(out, there, p.dim, st.o, by);
+  if (p.lse && there && h == 0 && (!F::kApart || wave == 0)) p.lse[q_head * p.nq + at] = lse_of(most, sum);
 }
-template <typename T, int WIDE, int WAVES, int KEYS>
-__global__ __launch_bounds__(WAVES *kWave) void segment_attn_kernel(Forward p) {
-  segment_attn<T, WIDE, WAVES, KEYS>(p);
+// bf16: two wavefronts a SIMD at least.
+template <typename T, int WIDE, typename F>
+__global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 ? 2 : 1) void segment_attn_kernel(Forward p) {
+  segment_attn<T, WIDE, F>(p);
 }
 
 // The parts of a query's keys: a wavefront for each row.
@@ -242,18 +264,22 @@ __global__ __launch_bounds__(kBlock) void segment_attn_join_kernel(Forward p) {
   if (p.lse && lane == 0) p.lse[head * p.nq + query] = lse_of(most, sum);
 }
 
-template <typename T, int WIDE, int WAVES, int KEYS>
+enum Cutting { kShared, kSingle, kApart };
+
+template <typename T, int WIDE, typename F>
 int launch(Forward p, hipStream_t s) {
-  p.tiles = segment_tiles(p.nq, p.pack, p.segments, 32 * WAVES);
+  p.tiles = segment_tiles(p.nq, p.pack, p.segments, F::kRows);
   const int64_t grid = p.tiles * (p.heads / p.pack);
-  if (grid > kMostLanes / (WAVES * kWave)) return GA_EUNSUPPORTED;
-  hipLaunchKernelGGL((segment_attn_kernel<T, WIDE, WAVES, KEYS>), dim3((unsigned)grid, (unsigned)p.splits),
-                     dim3(WAVES * kWave), 0, s, p);
+  if (grid > kMostLanes / (F::kWaves * kWave)) return GA_EUNSUPPORTED;
+  hipLaunchKernelGGL((segment_attn_kernel<T, WIDE, F>), dim3((unsigned)grid, (unsigned)p.splits), dim3(F::kWaves * kWave), 0, s, p);
   return launch_status();
 }
 template <typename T, int WIDE>
 int forward(const Forward &p, hipStream_t s) {
-  return launch<T, WIDE, 4, 64>(p, s);
+  constexpr bool kDeepRows = WIDE * sizeof(T) > 256;         // 512 bytes: tiles of 32 of them, or one at a time
+  if (p.cutting == kSingle) return launch<T, WIDE, Form<1, 64, 1, false>>(p, s);
+  if (p.cutting == kApart) return launch<T, WIDE, Form<4, 32, kDeepRows ? 1 : 2, true>>(p, s);
+  return launch<T, WIDE, Form<4, 64, 2, false>>(p, s);
 }
 template <typename T>
 int forward(const Forward &p, hipStream_t s) {
@@ -323,7 +349,7 @@ int segment_attn_check(SegAttn &p, const void *q, const void *k, const void *v, 
   if (!aligned(q, e) || !aligned(k, e) || !aligned(v, e) || !aligned(q_pointer, 8) || !aligned(k_pointer, 8)) return GA_EALIGN;
   // offsets inside a tile of 64 rows are 32-bit numbers
   const int64_t far = (int64_t)1 << 24;
-  if (q_row * e > far || k_row * e > far || v_row * e > far) return GA_EUNSUPPORTED;
+  if (q_row * e > far || k_row * e > far || v_row * e > far || q_head * (heads / kv_heads) * e > far * 32) return GA_EUNSUPPORTED;
   p.q = q;
   p.k = k;
   p.v = v;
@@ -343,6 +369,7 @@ int segment_attn_check(SegAttn &p, const void *q, const void *k, const void *v, 
   p.dim = (int)dim;
   p.causal = causal;
   p.scale = scale;
+  p.q_whole = whole_rows(dim, dtype) && aligned(q, 4) && p.q_row % 4 == 0 && p.q_head % 4 == 0;
   return GA_OK;
 }
 
@@ -353,16 +380,25 @@ static bool pieces_aligned(const void *p, int64_t row, int64_t head) {
 
 namespace {
 // How a call is cut up, from what the host knows: how many rows and segments there are, not how long which segment is.
-struct Cut { int pack, splits; int64_t laid, parts; size_t bytes; };
+struct Cut { int pack, cutting, splits; int64_t laid, parts; size_t bytes; };
 Cut cut_of(int64_t segments, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim, int dtype) {
   Cut c;
   const int64_t group = heads / kv_heads, some = segments > 0 ? segments : 1;
-  c.pack = nq * group <= 128 * some ? (int)group : 1;
-  const int64_t tiles = (nq * c.pack / 128 > some ? nq * c.pack / 128 : some) * (heads / c.pack);
-  const int64_t key_tiles = nk / some / 64;
-  int64_t n = 512 / tiles;
-  if (n > key_tiles / 4) n = key_tiles / 4;
-  c.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  const int64_t keys = nk / some;                            // of a segment, on average
+  auto tiles = [&](int64_t rows) {                           // at least so many, of all heads
+    const int64_t n = (nq * c.pack + rows - 1) / rows;
+    return (n > some ? n : some) * (heads / c.pack);
+  };
+  c.pack = nq * group <= 32 * some ? (int)group : 1;
+  c.splits = 1;
+  if (keys > 64 && tiles(128) < 256) {
+    c.cutting = kApart;
+    int64_t n = 512 / tiles(32);
+    if (n > keys / 512) n = keys / 512;
+    c.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  } else {
+    c.cutting = nq * c.pack <= 64 * some ? kSingle : kShared;
+  }
   c.laid = whole_rows(dim, dtype) ? 0 : segment_attn_laid_bytes(nk, kv_heads, dim, dtype);
   c.parts = 2 * c.laid;
   c.bytes = (size_t)(c.parts + (c.splits > 1 ? c.splits * nq * heads * (dim + 2) * 4 : 0));
@@ -413,6 +449,7 @@ int ga_segment_attention(const void *q, int64_t q_row, int64_t q_head, const voi
   p.out_head = dim;
   p.out_row = heads * dim;
   p.pack = c.pack;
+  p.cutting = c.cutting;
   p.splits = c.splits;
   p.parts = (float *)((char *)workspace + c.parts);
   return dtype == GA_F32 ? forward<float>(p, s) : forward<bf16_t>(p, s);

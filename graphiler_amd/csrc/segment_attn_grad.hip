@@ -20,6 +20,7 @@ struct Backward : SegAttn {
   float *delta;                          // (heads, nq)
   void *gq, *gk, *gv;                    // (rows, heads, dim), contiguous
   int64_t tiles;
+  int out_whole;                         // rows of out are whole pieces; the others always are, as they lie or laid out
 };
 
 // Products of results w (operand over rows 32 b ... of `t`) and its columns onto acc.  CLEAN: values of t that are not finite
@@ -37,38 +38,42 @@ __device__ __forceinline__ bool add_columns(const lds_char *t, int col_at, int b
       uintx4 v = R::col(t, col_at, b, i, d);
       if constexpr (CLEAN) found |= cleaned<T>(v);
       acc[d] = mma_piece<T>(v, o, acc[d]);
+      if constexpr (CLEAN) __builtin_amdgcn_sched_barrier(0);          // the rare tiles are not to decide what registers it takes
     }
   }
   return found;
 }
 
-// dq: WAVES wavefronts with 32 queries of a head each share tiles of KEYS keys.
-template <typename T, int WIDE, int WAVES, int KEYS>
+// dq: 32 queries of a head a wavefront.
+template <typename T, int WIDE, typename F>
 __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
   typedef Rows<T, WIDE> R;
-  typedef RowMoves<T, WIDE, KEYS, WAVES> Moves;
-  constexpr int BM = 32 * WAVES, kStage = 2 * Moves::kBytes;
-  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage];
+  constexpr int KEYS = F::kDeep;
+  typedef RowMoves<T, WIDE, KEYS, F::kMovers> Moves;
+  constexpr int kStage = 2 * Moves::kBytes, kRegions = F::kApart ? F::kWaves : 1, kLds = kStage * kRegions;
+  __shared__ __attribute__((aligned(1024))) char stage0[kLds], stage1[F::kStages == 2 ? kLds : 16];
   int head;
   int64_t tile;
-  head_tile(blockIdx.x, p.tiles, p.heads, head, tile);
+  head_tile(blockIdx.x, p.tiles, p.heads, F::kWaves == 1, head, tile);
   if (p.causal) tile = p.tiles - 1 - tile;
   Segment seg;
-  if (!segment_of<BM>(p, tile, 1, false, seg)) return;
+  if (!segment_of<F::kRows>(p, tile, 1, false, seg)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x & (kWave - 1), n = lane & 31, h = lane >> 5;
   const int kv = head / p.group;
-  const int first = seg.tile * BM + wave * 32, query = first + n;
+  const int first = seg.tile * F::kRows + (F::kApart ? 0 : wave * 32), query = first + n;
   const bool there = query < seg.q_len;
   const int64_t at = seg.q0 + query;
 
   uintx4 q[R::kSteps], g[R::kSteps];
-  load_row<T, WIDE>((const char *)p.q + at * p.q_row + head * p.q_head, there, p.dim, q);
-  load_row<T, WIDE>((const char *)p.grad + at * p.grad_row + head * p.grad_head, there, p.dim, g);
+  const int64_t row0 = seg.q0 + first;
+  load_row<T, WIDE>((const char *)p.q + row0 * p.q_row + head * p.q_head, (uint32_t)(n * p.q_row), there, p.dim, true, q);
+  load_row<T, WIDE>((const char *)p.grad + row0 * p.grad_row + head * p.grad_head, (uint32_t)(n * p.grad_row), there, p.dim, true, g);
   float delta = 0.0f;
   {
     uintx4 o[R::kSteps];
-    load_row<T, WIDE>((const char *)p.out + at * p.out_row + head * p.out_head, there, p.dim, o);
+    load_row<T, WIDE>((const char *)p.out + row0 * p.out_row + head * p.out_head, (uint32_t)(n * p.out_row), there, p.dim,
+                      p.out_whole, o);
 #pragma unroll
     for (int i = 0; i < R::kSteps; ++i)
 #pragma unroll
@@ -84,31 +89,31 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
   }
   float lse = there ? p.lse[head * p.nq + at] * kLog2e : 0.0f;
   if (lse == -INFINITY) lse = INFINITY;                      // a query that sees nothing: p = 0
-  if (there && h == 0) p.delta[head * p.nq + at] = delta;
   const float c = p.scale * kLog2e;
 
   const int more = seg.k_len - seg.q_len;
   const int seen = p.causal ? max(0, min(seg.k_len, query + 1 + more)) : seg.k_len;
   const int by_all = p.causal ? max(0, min(seg.k_len, first + 1 + more)) : seg.k_len;
   const int by_any = first >= seg.q_len ? 0 : p.causal ? max(0, min(seg.k_len, min(first + 32, seg.q_len) + more)) : seg.k_len;
-  const int block_last = min(seg.tile * BM + BM, seg.q_len);
+  const int block_last = min(seg.tile * F::kRows + F::kRows, seg.q_len);
   const int wanted = p.causal ? max(0, min(seg.k_len, block_last + more)) : seg.k_len;
   const int end = (wanted + KEYS - 1) / KEYS;
 
+  constexpr int kTurn = F::kApart ? F::kWaves : 1;           // tiles from one of the wavefront's to its next
+  int to_fetch = F::kApart ? wave : 0;
   Moves mk, mv;
-  mk.init(p.k_row, p.dim, wave);
-  mv.init(p.v_row, p.dim, wave);
-  const char *k_at = (const char *)p.k + seg.k0 * p.k_row + kv * p.k_head;
-  const char *v_at = (const char *)p.v + seg.k0 * p.v_row + kv * p.v_head;
-  int to_fetch = 0;
+  mk.init(p.k_row, p.dim, F::kApart ? 0 : wave);
+  mv.init(p.v_row, p.dim, F::kApart ? 0 : wave);
+  const char *k_at = (const char *)p.k + (seg.k0 + (int64_t)to_fetch * KEYS) * p.k_row + kv * p.k_head;
+  const char *v_at = (const char *)p.v + (seg.k0 + (int64_t)to_fetch * KEYS) * p.v_row + kv * p.v_head;
   auto fetch = [&](lds_char *to) {
     if (to_fetch >= end) return;
     const int left = seg.k_len - to_fetch * KEYS;
     mk.move(k_at, left, to);
     mv.move(v_at, left, to + Moves::kBytes);
-    k_at += KEYS * p.k_row;
-    v_at += KEYS * p.v_row;
-    ++to_fetch;
+    k_at += kTurn * KEYS * p.k_row;
+    v_at += kTurn * KEYS * p.v_row;
+    to_fetch += kTurn;
   };
   const int row_at = R::row_at(), col_at = R::col_at();
   floatx16 dq[R::kCols];
@@ -117,47 +122,69 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
 
-  auto block = [&](const lds_char *keys, const lds_char *values, int b, int key0, auto edge) {
+  // What a wavefront's queries see in one tile alone gives delta from the weights themselves, sum_j p_ij <do_i, v_j>: with
+  // few keys the rounding of out would be what their gradients are off by.
+  const bool alone = !F::kApart && by_any <= KEYS;
+  float weighed = 0.0f;
+  auto block = [&](const lds_char *keys, const lds_char *values, int b, int key0, auto edge, bool weigh) {
     constexpr bool kEdge = decltype(edge)::value;
     floatx16 s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < R::kSteps; ++i) s = mma_piece<T>(R::row(keys, row_at, b, i), q[i], s);
+    if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < R::kSteps; ++i) dp = mma_piece<T>(R::row(values, row_at, b, i), g[i], dp);
+    if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float ds = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
-      s[r] = !kEdge || key0 + result_row(r) + 4 * h < seen ? ds : 0.0f;
+      s[r] = !kEdge || result_row(r) < seen - key0 - 4 * h ? ds : 0.0f;
+      if constexpr (kEdge) weighed += s[r];
     }
+    if (kEdge && weigh) return;
     // A key that is not finite has scores that are not, which is what reaches the queries that see it.
     add_columns<T, WIDE, kEdge>(keys, col_at, b, s, dq);
   };
-  auto step = [&](int t, lds_char *here, lds_char *next) {
-    landed<0>();
-    fetch(next);
+  auto use = [&](int t, const lds_char *here) {
+    if (t * KEYS >= by_any) return;
+    // `alone`: once for delta, once with it
+    float known = delta;
+    if (alone) delta = weighed = 0.0f;
+#pragma unroll 1
+    for (int pass = alone ? 0 : 1; pass < 2; ++pass) {
 #pragma unroll
-    for (int b = 0; b < KEYS / 32; ++b) {
-      const int key0 = t * KEYS + b * 32;
-      if (key0 >= by_any) continue;
-      if (key0 + 32 <= by_all) block(here, here + Moves::kBytes, b, key0, std::false_type());
-      else block(here, here + Moves::kBytes, b, key0, std::true_type());
+      for (int b = 0; b < KEYS / 32; ++b) {
+        const int key0 = t * KEYS + b * 32;
+        if (key0 >= by_any) continue;
+        if (!alone && key0 + 32 <= by_all) block(here, here + Moves::kBytes, b, key0, std::false_type(), false);
+        else block(here, here + Moves::kBytes, b, key0, std::true_type(), pass == 0);
+      }
+      if (pass == 0) {
+        delta = weighed + other_half(weighed);
+        if (!(fabsf(delta) < INFINITY)) delta = known;
+      }
     }
   };
-  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1;
-  fetch(L0);
-  int t = 0;
-  for (; t + 2 <= end; t += 2) {
-    step(t, L0, L1);
-    step(t + 1, L1, L0);
+  const int region = F::kApart ? wave * kStage : 0;
+  through_tiles<F>(0, end, wave, (lds_char *)stage0 + region, (lds_char *)stage1 + (F::kStages == 2 ? region : 0), fetch, use);
+  if (there && h == 0 && (!F::kApart || wave == 0)) p.delta[head * p.nq + at] = delta;
+  T *out = (T *)p.gq + (at * p.heads + head) * p.dim;
+  if constexpr (F::kApart) {
+    static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
+    Gathered<WIDE, F::kWaves> all;
+    all.leave((lds_char *)stage0 + region, dq, 1.0f);
+    __syncthreads();
+    all.take((const lds_char *)stage0, kStage, wave);
+    all.store(out, there, p.dim, wave, p.scale);
+  } else {
+    store_row<T, R::kCols>(out, there, p.dim, dq, p.scale);
   }
-  if (t < end) step(t, L0, L1);
-  store_row<T, R::kCols>((T *)p.gq + (at * p.heads + head) * p.dim, there, p.dim, dq, p.scale);
 }
-template <typename T, int WIDE, int WAVES, int KEYS>
-__global__ __launch_bounds__(WAVES *kWave) void segment_attn_dq_kernel(Backward p) {
-  segment_attn_dq<T, WIDE, WAVES, KEYS>(p);
+template <typename T, int WIDE, typename F>
+__global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 && WIDE <= 64 ? 2 : 1) void segment_attn_dq_kernel(Backward p) {
+  segment_attn_dq<T, WIDE, F>(p);
 }
 
 // A lane's share of 32 numbers, as it holds 16 of 32 rows of results; zeros behind the `left` that there are.
@@ -169,59 +196,69 @@ __device__ __forceinline__ void load_numbers(const float *from, int64_t left, fl
     f[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, (i * 8 + h * 4) * 4, 0, 0));
 }
 
-// dk and dv: WAVES wavefronts with 32 keys of a head each share tiles of QUERIES queries.
-template <typename T, int WIDE, int WAVES, int QUERIES>
+// Which tile of which head of a group comes next.
+struct Place {
+  int head, tile;
+  __device__ __forceinline__ Place(int t, int tiles) : head(0), tile(t) { wrap(tiles); }
+  __device__ __forceinline__ void next(int by, int tiles) {
+    tile += by;
+    wrap(tiles);
+  }
+  __device__ __forceinline__ void wrap(int tiles) {
+    if (tiles > 0)
+      for (; tile >= tiles; ++head) tile -= tiles;
+  }
+};
+
+// dk and dv: 32 keys of a head a wavefront.
+template <typename T, int WIDE, typename F>
 __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
   typedef Rows<T, WIDE> R;
-  typedef RowMoves<T, WIDE, QUERIES, WAVES> Moves;
-  constexpr int BN = 32 * WAVES, kStage = 2 * Moves::kBytes;
-  __shared__ __attribute__((aligned(1024))) char stage0[kStage], stage1[kStage];
+  constexpr int QUERIES = F::kDeep;
+  typedef RowMoves<T, WIDE, QUERIES, F::kMovers> Moves;
+  constexpr int kStage = 2 * Moves::kBytes, kRegions = F::kApart ? F::kWaves : 1, kLds = kStage * kRegions;
+  __shared__ __attribute__((aligned(1024))) char stage0[kLds], stage1[F::kStages == 2 ? kLds : 16];
   int kv;
   int64_t tile;
-  head_tile(blockIdx.x, p.tiles, p.heads / p.group, kv, tile);
+  head_tile(blockIdx.x, p.tiles, p.heads / p.group, F::kWaves == 1, kv, tile);
   Segment seg;
-  if (!segment_of<BN>(p, tile, 1, true, seg)) return;
+  if (!segment_of<F::kRows>(p, tile, 1, true, seg)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x & (kWave - 1), n = lane & 31, h = lane >> 5;
-  const int first = seg.tile * BN + wave * 32, key = first + n;
+  const int first = seg.tile * F::kRows + (F::kApart ? 0 : wave * 32), key = first + n;
   const bool there = key < seg.k_len;
   const int64_t at = seg.k0 + key;
 
   uintx4 k[R::kSteps], v[R::kSteps];
-  load_row<T, WIDE>((const char *)p.k + at * p.k_row + kv * p.k_head, there, p.dim, k);
-  load_row<T, WIDE>((const char *)p.v + at * p.v_row + kv * p.v_head, there, p.dim, v);
+  const int64_t row0 = seg.k0 + first;
+  load_row<T, WIDE>((const char *)p.k + row0 * p.k_row + kv * p.k_head, (uint32_t)(n * p.k_row), there, p.dim, true, k);
+  load_row<T, WIDE>((const char *)p.v + row0 * p.v_row + kv * p.v_head, (uint32_t)(n * p.v_row), there, p.dim, true, v);
   const float c = p.scale * kLog2e;
 
   // the first query that sees the lane's key, the wavefront's first and last and the workgroup's first
   const int less = seg.q_len - seg.k_len;
   const int by = p.causal ? key + less : 0;
   const int by_any = p.causal ? first + less : 0, by_all = p.causal ? first + 31 + less : 0;
-  const int begin = p.causal ? max(0, seg.tile * BN + less) / QUERIES : 0;
+  const int begin = p.causal ? max(0, seg.tile * F::kRows + less) / QUERIES : 0;
   const int end = (seg.q_len + QUERIES - 1) / QUERIES;
   const int tiles = max(0, end - begin), all = tiles * p.group;
 
+  // tile t of all heads' is tile begin + t % tiles of head t / tiles
+  constexpr int kTurn = F::kApart ? F::kWaves : 1;
   Moves mq, mg;
-  mq.init(p.q_row, p.dim, wave);
-  mg.init(p.grad_row, p.dim, wave);
-  const int64_t begin_row = seg.q0 + (int64_t)begin * QUERIES;
-  const char *q_at = (const char *)p.q + begin_row * p.q_row + kv * p.group * p.q_head;
-  const char *g_at = (const char *)p.grad + begin_row * p.grad_row + kv * p.group * p.grad_head;
-  const int64_t q_step = QUERIES * p.q_row, g_step = QUERIES * p.grad_row;
-  const int64_t q_next = p.q_head - tiles * q_step, g_next = p.grad_head - tiles * g_step;      // the first tile of the next head
-  int to_fetch = all, fetch_tile = begin;
+  mq.init(p.q_row, p.dim, F::kApart ? 0 : wave);
+  mg.init(p.grad_row, p.dim, F::kApart ? 0 : wave);
+  const char *const q_first = (const char *)p.q + seg.q0 * p.q_row + kv * p.group * p.q_head;
+  const char *const g_first = (const char *)p.grad + seg.q0 * p.grad_row + kv * p.group * p.grad_head;
+  int to_fetch = F::kApart ? wave : 0;
+  Place fetched(to_fetch, tiles);
   auto fetch = [&](lds_char *to) {
-    if (to_fetch == 0) return;
-    const int left = seg.q_len - fetch_tile * QUERIES;
-    mq.move(q_at, left, to);
-    mg.move(g_at, left, to + Moves::kBytes);
-    q_at += q_step;
-    g_at += g_step;
-    --to_fetch;
-    if (++fetch_tile == end) {
-      fetch_tile = begin;
-      q_at += q_next;
-      g_at += g_next;
-    }
+    if (to_fetch >= all) return;
+    const int query0 = (begin + fetched.tile) * QUERIES;
+    mq.move(q_first + query0 * p.q_row + fetched.head * p.q_head, seg.q_len - query0, to);
+    mg.move(g_first + query0 * p.grad_row + fetched.head * p.grad_head, seg.q_len - query0, to + Moves::kBytes);
+    to_fetch += kTurn;
+    fetched.next(kTurn, tiles);
   };
   const int row_at = R::row_at(), col_at = R::col_at();
   floatx16 dk[R::kCols], dv[R::kCols];
@@ -242,15 +279,16 @@ __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < R::kSteps; ++i) s = mma_piece<T>(R::row(queries, row_at, b, i), k[i], s);
+    if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < R::kSteps; ++i) dp = mma_piece<T>(R::row(grads, row_at, b, i), v[i], dp);
+    if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float l = lse[r / 4][r % 4];
       const float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, l == -INFINITY ? -INFINITY : -kLog2e * l));
       const float ds = w * (dp[r] - delta[r / 4][r % 4]);
-      const int query = query0 + result_row(r) + 4 * h;
-      const bool counts = !kEdge || (query >= by && query < seg.q_len);
+      const bool counts = !kEdge || (result_row(r) >= by - query0 - 4 * h && result_row(r) < seg.q_len - query0 - 4 * h);
       s[r] = counts ? w : 0.0f;
       dp[r] = counts ? ds : 0.0f;
     }
@@ -264,61 +302,91 @@ __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
     }
     add_columns<T, WIDE, kEdge>(queries, col_at, b, dp, dk);
   };
-  int in_tile = begin, q_head = kv * p.group;
-  auto step = [&](lds_char *here, lds_char *next) {
-    landed<0>();
-    fetch(next);
+  Place used(F::kApart ? wave : 0, tiles);
+  auto use = [&](int, const lds_char *here) {
+    const int tile0 = (begin + used.tile) * QUERIES, q_head = kv * p.group + used.head;
 #pragma unroll
     for (int b = 0; b < QUERIES / 32; ++b) {
-      const int query0 = in_tile * QUERIES + b * 32;
+      const int query0 = tile0 + b * 32;
       if (first >= seg.k_len || query0 >= seg.q_len || query0 + 31 < by_any) continue;
       if (query0 >= by_all && query0 + 32 <= seg.q_len) block(here, here + Moves::kBytes, b, query0, q_head, std::false_type());
       else block(here, here + Moves::kBytes, b, query0, q_head, std::true_type());
     }
-    if (++in_tile == end) {
-      in_tile = begin;
-      ++q_head;
-    }
+    used.next(kTurn, tiles);
   };
-  lds_char *const L0 = (lds_char *)stage0, *const L1 = (lds_char *)stage1;
-  fetch(L0);
-  int t = 0;
-  for (; t + 2 <= all; t += 2) {
-    step(L0, L1);
-    step(L1, L0);
-  }
-  if (t < all) step(L0, L1);
+  const int region = F::kApart ? wave * kStage : 0;
+  through_tiles<F>(0, all, wave, (lds_char *)stage0 + region, (lds_char *)stage1 + (F::kStages == 2 ? region : 0), fetch, use);
   const int64_t to = (at * (p.heads / p.group) + kv) * p.dim;
-  store_row<T, R::kCols>((T *)p.gk + to, there, p.dim, dk, p.scale);
-  store_row<T, R::kCols>((T *)p.gv + to, there, p.dim, dv, 1.0f);
+  if constexpr (F::kApart) {
+    static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
+    Gathered<WIDE, F::kWaves> sums;
+    sums.leave((lds_char *)stage0 + region, dk, 1.0f);
+    __syncthreads();
+    sums.take((const lds_char *)stage0, kStage, wave);
+    sums.store((T *)p.gk + to, there, p.dim, wave, p.scale);
+    __syncthreads();
+    sums.leave((lds_char *)stage0 + region, dv, 1.0f);
+    __syncthreads();
+    sums.take((const lds_char *)stage0, kStage, wave);
+    sums.store((T *)p.gv + to, there, p.dim, wave, 1.0f);
+  } else {
+    store_row<T, R::kCols>((T *)p.gk + to, there, p.dim, dk, p.scale);
+    store_row<T, R::kCols>((T *)p.gv + to, there, p.dim, dv, 1.0f);
+  }
 }
-template <typename T, int WIDE, int WAVES, int QUERIES>
-__global__ __launch_bounds__(WAVES *kWave, 1) void segment_attn_dkv_kernel(Backward p) {
-  segment_attn_dkv<T, WIDE, WAVES, QUERIES>(p);
+// Two wavefronts a SIMD where their sums and operands (128 WIDE / 32 and 32 WIDE / 64 registers) leave room for it.
+template <typename T, int WIDE, typename F>
+__global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 && WIDE <= 64 ? 2 : 1) void segment_attn_dkv_kernel(Backward p) {
+  segment_attn_dkv<T, WIDE, F>(p);
 }
 
-template <typename T, int WIDE, int WAVES, int DEEP>
-int launch(Backward p, hipStream_t s) {
-  p.tiles = segment_tiles(p.nq, 1, p.segments, 32 * WAVES);
-  const int64_t dq_grid = p.tiles * p.heads;
-  const int64_t k_tiles = segment_tiles(p.nk, 1, p.segments, 32 * WAVES), dkv_grid = k_tiles * (p.heads / p.group);
-  if ((dq_grid > dkv_grid ? dq_grid : dkv_grid) > kMostLanes / (WAVES * kWave)) return GA_EUNSUPPORTED;
+enum Cutting { kShared, kSingle, kApart };
+// As cut_of() of the forward pass has it: by the rows of a segment on average and by how many workgroups of 128 rows there
+// are, `keys` being what a row goes through.
+Cutting cutting_of(int64_t segments, int64_t rows, int64_t keys, int64_t heads) {
+  const int64_t some = segments > 0 ? segments : 1, n = (rows + 127) / 128;
+  if (keys > 64 * some && (n > some ? n : some) * heads < 256) return kApart;
+  return rows <= 64 * some ? kSingle : kShared;
+}
+
+template <typename T, int WIDE, typename F>
+int launch_dq(Backward p, hipStream_t s) {
+  p.tiles = segment_tiles(p.nq, 1, p.segments, F::kRows);
+  const int64_t grid = p.tiles * p.heads;
+  if (grid > kMostLanes / (F::kWaves * kWave)) return GA_EUNSUPPORTED;
+  hipLaunchKernelGGL((segment_attn_dq_kernel<T, WIDE, F>), dim3((unsigned)grid), dim3(F::kWaves * kWave), 0, s, p);
+  return launch_status();
+}
+template <typename T, int WIDE, typename F>
+int launch_dkv(Backward p, hipStream_t s) {
+  p.tiles = segment_tiles(p.nk, 1, p.segments, F::kRows);
+  const int64_t grid = p.tiles * (p.heads / p.group);
+  if (grid > kMostLanes / (F::kWaves * kWave)) return GA_EUNSUPPORTED;
+  hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F>), dim3((unsigned)grid), dim3(F::kWaves * kWave), 0, s, p);
+  return launch_status();
+}
+template <typename T, int WIDE>
+int backward(const Backward &p, hipStream_t s) {
+  constexpr bool kDeepRows = WIDE * sizeof(T) > 256;         // 512 bytes: tiles of 32 of them, or one at a time
+  typedef Form<1, 64, 1, false> Single;
+  typedef Form<4, 32, kDeepRows ? 1 : 2, true> Apart;
+  typedef Form<4, kDeepRows ? 32 : 64, 2, false> Shared;
   if (p.nq > 0) {
-    hipLaunchKernelGGL((segment_attn_dq_kernel<T, WIDE, WAVES, DEEP>), dim3((unsigned)dq_grid), dim3(WAVES * kWave), 0, s, p);
-    if (int rc = launch_status()) return rc;
+    const Cutting c = cutting_of(p.segments, p.nq, p.nk, p.heads);
+    const int rc = c == kSingle ? launch_dq<T, WIDE, Single>(p, s) : c == kApart ? launch_dq<T, WIDE, Apart>(p, s)
+                                                                                 : launch_dq<T, WIDE, Shared>(p, s);
+    if (rc) return rc;
   }
-  p.tiles = k_tiles;
   if (p.nk > 0) {
-    hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, WAVES, DEEP>), dim3((unsigned)dkv_grid), dim3(WAVES * kWave), 0, s, p);
-    if (int rc = launch_status()) return rc;
+    const Cutting c = cutting_of(p.segments, p.nk, p.nq * p.group, p.heads / p.group);
+    return c == kSingle ? launch_dkv<T, WIDE, Single>(p, s) : c == kApart ? launch_dkv<T, WIDE, Apart>(p, s)
+                                                                          : launch_dkv<T, WIDE, Shared>(p, s);
   }
   return GA_OK;
 }
 template <typename T>
 int backward(const Backward &p, hipStream_t s) {
-  if (p.dim <= 32) return launch<T, 32, 4, 64>(p, s);
-  if (p.dim <= 64) return launch<T, 64, 4, 64>(p, s);
-  return launch<T, 128, 4, sizeof(T) == 2 ? 64 : 32>(p, s);
+  return p.dim <= 32 ? backward<T, 32>(p, s) : p.dim <= 64 ? backward<T, 64>(p, s) : backward<T, 128>(p, s);
 }
 
 }  // namespace
@@ -364,6 +432,7 @@ int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q
   p.grad = grad_out;
   p.out_head = p.grad_head = dim * e;
   p.out_row = p.grad_row = heads * dim * e;
+  p.out_whole = whole && aligned(out, 4);
   p.lse = lse;
   p.delta = (float *)workspace;
   p.gq = grad_q;

@@ -88,3 +88,13 @@ def test_scales(scale, dtype):
 def test_long(dtype):
     check([2500, 1000], None, 2, 1, 128, True, dtype)
     check([1700], None, 1, 1, 64, False, dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [24, 64, 128])
+def test_enough_workgroups_for_tiles_that_wavefronts_share(dim, causal, dtype):
+    """128 rows a workgroup and 256 workgroups at least, on both sides; single wavefronts where segments are short."""
+    check([200, 130, 70, 257], None, 64, 64, dim, causal, dtype)
+    check([100, 130, 70, 64], [300, 90, 129, 10], 128, 64, dim, causal, dtype, backward=dim < 128)
+    check([40, 64, 65, 3, 0, 33, 32] * 10, None, 4, 2, dim, causal, dtype)
