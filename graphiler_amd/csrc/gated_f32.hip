@@ -207,9 +207,10 @@ int gated_f32_launch(const void *x, const void *wg, const void *wu, void *h, int
   return f32_launch<true>(x, wg, wu, Gated4{(float *)h, act}, rows, K, F, s);
 }
 
-bool linear_f32_taken(int64_t rows, int64_t K, int64_t M) {
-  return M <= 128 || tiles_of(rows, M, kF32Rows, 2 * kF32Cols) <= (K <= 256 ? 2048 : 1280);
-}
+// One product: against x cut into pieces on the way (linear_split.hip), us with a bias and relu (instruction | pieces):
+// 1000 x 512 -> 512 13.7 | 22.1, 4096 x 500 -> 256 19.7 | 22.1, 30,000 x 64 -> 64 11.8 | 13.3, 100 x 4096 -> 4096 64 | 156; more tiles than run
+// at once: 19,717 x 500 -> 256 75 | 45.6, 65,536 x 256 -> 128 66 | 42, 2000 x 2000 -> 2000 183 | 111, 8192 x 1024 -> 512 96 | 60.
+bool linear_f32_taken(int64_t rows, int64_t M) { return tiles_of(rows, M, kF32Rows, 2 * kF32Cols) <= 512; }
 int linear_f32_launch(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, hipStream_t s) {
   return f32_launch<false>(x, w, nullptr, Ended4{end}, rows, K, M, s);
 }

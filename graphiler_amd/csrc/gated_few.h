@@ -38,9 +38,13 @@ struct Ended {
     f32_to_elem(z, y[row * M + col]);
   }
 };
+// fp32, x cut into pieces on the way (linear_split.hip); the workspace holds the weight's pieces.
+size_t linear_split_bytes(int64_t K, int64_t M);
+int linear_split_launch(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, void *workspace,
+                        hipStream_t s);
 int linear_few_launch(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, int dtype,
                       hipStream_t s);
-bool linear_f32_taken(int64_t rows, int64_t K, int64_t M);
+bool linear_f32_taken(int64_t rows, int64_t M);
 int linear_f32_launch(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, hipStream_t s);
 
 }  // namespace ga

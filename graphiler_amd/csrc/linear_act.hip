@@ -5,7 +5,9 @@
 // The forward product is one launch whose store adds the bias, applies the activation and adds the residual in
 // fp32, so neither z nor act(z) is ever in memory.  The gradients form z again where an activation's slope needs it (a third of
 // their operations) instead of keeping it; dz is rounded to bf16 once, as the operand of both products after, which
-// adds to a gradient as much as its own rounding.  fp32 operands are three bf16 pieces, as in gated.hip.
+// adds to a gradient as much as its own rounding.  fp32: the forward product of few tiles is the fp32 instruction's
+// (gated_f32.hip), of others that of pieces which x is cut into on the way (linear_split.hip); the gradients' operands are
+// pieces laid out in memory, as in gated.hip.
 #include "gated_few.h"
 #include "mm_parts.h"
 
@@ -21,38 +23,46 @@ __device__ __forceinline__ void by_act(const E &e, F f) {
   else f(e.template as<kReluGate>());
 }
 
-// act(z + b) + r
-template <typename T, int ACT = -2>
-struct LinearEpi : Stored<T> {
+// The bias of four columns, which their sums begin with.
+template <typename T>
+__device__ __forceinline__ floatx4 start_of(const T *bias, int64_t M, int64_t col, bool whole) {
+  return bias ? four_at(bias, M, 1, (int64_t)0, col, whole) : floatx4{0, 0, 0, 0};
+}
+
+// act(z) + r, bf16
+template <int ACT = -2>
+struct LinearEpi : Stored<bf16_t> {
   static constexpr int kOut = 1;
-  const T *bias, *residual;
-  T *y;
+  static constexpr bool kStarts = true;
+  const bf16_t *bias, *residual;
+  bf16_t *y;
   int64_t M;
   int act;
   bool whole, whole_bias;                // rows of the residual, the bias: whole groups of four
-  template <int A> __device__ __forceinline__ LinearEpi<T, A> as() const {
-    return LinearEpi<T, A>{{}, bias, residual, y, M, A, whole, whole_bias};
+  template <int A> __device__ __forceinline__ LinearEpi<A> as() const {
+    return LinearEpi<A>{{}, bias, residual, y, M, A, whole, whole_bias};
   }
   template <typename F> __device__ __forceinline__ void visit(F f) const { by_act<true>(*this, f); }
+  __device__ __forceinline__ floatx4 start(int64_t col) const { return start_of(bias, M, col, whole_bias); }
   __device__ __forceinline__ void make(const TileMm &p, int64_t row, int64_t col, const floatx4 &z, const floatx4 &,
-                                       typename Stored<T>::bits (&o)[1]) const {
+                                       uintx2 (&o)[1]) const {
     floatx4 t = z;
-    if (bias) t += four_at(bias, M, 1, (int64_t)0, col, whole_bias);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if constexpr (ACT != kNoGate) t[r] = gate_of(ACT, t[r]);
     if (residual) t += four_at(residual, M, p.rows, row, col, whole);
-    o[0] = Stored<T>::pack(t);
+    o[0] = pack(t);
   }
   __device__ __forceinline__ void store(const TileMm &, int, int64_t row, int64_t col, const uintx4 &w, int64_t n) const {
     store_chunk(y + row * M + col, w, n);
   }
 };
 
-// gy act'(z + b) as an operand: bf16 rows of `ld` values, of fp32 three planes of pieces.
+// gy act'(z) as an operand: bf16 rows of `ld` values, of fp32 three planes of pieces.
 template <typename T, int ACT = -2>
 struct SlopeEpi : Stored<bf16_t> {
   static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1, kOut = kPieces;
+  static constexpr bool kStarts = true;
   const T *gy, *bias;
   int64_t M;
   bf16_t *dz;
@@ -63,12 +73,12 @@ struct SlopeEpi : Stored<bf16_t> {
     return SlopeEpi<T, A>{{}, gy, bias, M, dz, ld, plane, A, whole, whole_bias};
   }
   template <typename F> __device__ __forceinline__ void visit(F f) const { by_act<false>(*this, f); }
+  __device__ __forceinline__ floatx4 start(int64_t col) const { return start_of(bias, M, col, whole_bias); }
   __device__ __forceinline__ void make(const TileMm &p, int64_t row, int64_t col, const floatx4 &z, const floatx4 &,
                                        uintx2 (&o)[kOut]) const {
-    floatx4 t = four_at(gy, M, p.rows, row, col, whole), s = z;
-    if (bias) s += four_at(bias, M, 1, (int64_t)0, col, whole_bias);
+    floatx4 t = four_at(gy, M, p.rows, row, col, whole);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) t[r] *= gate_slope(ACT, s[r]);
+    for (int r = 0; r < 4; ++r) t[r] *= gate_slope(ACT, z[r]);
     if constexpr (kPieces == 1) o[0] = pack(t);
     else cut_pieces(t, o[0], o[1], o[2]);
   }
@@ -78,8 +88,7 @@ struct SlopeEpi : Stored<bf16_t> {
 };
 
 // The parts of a forward product that was cut along k, and its end.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void linear_join_kernel(const float *__restrict__ parts, Ended<T> end, int64_t all,
+__global__ __launch_bounds__(kBlock) void linear_join_kernel(const float *__restrict__ parts, Ended<bf16_t> end, int64_t all,
                                                              int splits) {
   for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < all; i += (int64_t)gridDim.x * kBlock) {
     float s = 0.0f;
@@ -151,8 +160,8 @@ Plan plan_of(int64_t rows, int64_t K, int64_t M, int act, int dtype, bool grad) 
     if (p.splits > 1) p.parts = take(4 * p.splits * rows * M);
   } else {
     if (act != kNoGate || own_w) p.dz = take(2 * p.pieces * rows * p.Mp);
-    p.splits = parts_of(tiles_of(K, M, 64, 128), (rows + 63) / 64 * six);
-    p.x_splits = parts_of(tiles_of(rows, K, 64, 128), (M + 63) / 64 * six);
+    p.splits = parts_of(tiles_of(K, M, 128, 128), (rows + 63) / 64 * six);
+    p.x_splits = parts_of(tiles_of(rows, K, 128, 128), (M + 63) / 64 * six);
     int64_t most = 0;
     if (p.splits > 1) most = p.splits * K * M;
     if (p.x_splits > 1 && p.x_splits * rows * K > most) most = p.x_splits * rows * K;
@@ -211,20 +220,19 @@ TileMm product(const Plan &p, const bf16_t *x, const bf16_t *w, int64_t rows, in
 }
 bool fours(const void *p, int64_t cols, size_t e) { return cols % 4 == 0 && aligned(p, 4 * e); }
 
-template <typename T>
 int forward(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, const Plan &p, char *ws,
             hipStream_t s) {
   const bf16_t *xo, *wo, *none;
-  if (int rc = lay<T>(p, x, w, nullptr, rows, K, M, ws, xo, wo, none, s)) return rc;
+  if (int rc = lay<bf16_t>(p, x, w, nullptr, rows, K, M, ws, xo, wo, none, s)) return rc;
   const TileMm m = product(p, xo, wo, rows, K, M, p.splits);
   if (p.splits == 1) {
-    const LinearEpi<T> e{{}, (const T *)end.bias, (const T *)end.residual, (T *)end.y, M, end.act,
-                         fours(end.residual, M, sizeof(T)), fours(end.bias, M, sizeof(T))};
+    const LinearEpi<> e{{}, (const bf16_t *)end.bias, (const bf16_t *)end.residual, (bf16_t *)end.y, M, end.act,
+                        fours(end.residual, M, 2), fours(end.bias, M, 2)};
     return tile_mm_launch<false, false, true, false>(m, e, s);
   }
   float *parts = (float *)(ws + p.parts);
   if (int rc = tile_mm_launch<false, false, true, false, true>(m, StoreEpi<float>(parts, M, rows * M), s)) return rc;
-  hipLaunchKernelGGL((linear_join_kernel<T>), dim3(stream_grid(rows * M)), dim3(kBlock), 0, s, parts, Ended<T>(end), rows * M,
+  hipLaunchKernelGGL(linear_join_kernel, dim3(stream_grid(rows * M)), dim3(kBlock), 0, s, parts, Ended<bf16_t>(end), rows * M,
                      p.splits);
   return launch_status();
 }
@@ -314,8 +322,8 @@ int check_linear(int64_t rows, int64_t K, int64_t M, int act, int dtype) {
 bool operand_aligned(const void *p, int64_t row, int dtype) {
   return aligned(p, dtype == GA_F32 ? 4 : row % 8 == 0 ? 16 : 2);
 }
-bool by_instruction(int64_t rows, int64_t K, int64_t M, int dtype) {
-  return rows <= kGatedFewRows || (dtype == GA_F32 && linear_f32_taken(rows, K, M));
+bool by_instruction(int64_t rows, int64_t M, int dtype) {
+  return rows <= kGatedFewRows || (dtype == GA_F32 && linear_f32_taken(rows, M));
 }
 
 }  // namespace
@@ -324,7 +332,8 @@ bool by_instruction(int64_t rows, int64_t K, int64_t M, int dtype) {
 extern "C" {
 
 size_t ga_linear_act_workspace_bytes(int64_t rows, int64_t K, int64_t M, int dtype) {
-  if (ga::check_linear(rows, K, M, GA_GATE_NONE, dtype) != GA_OK || ga::by_instruction(rows, K, M, dtype)) return 0;
+  if (ga::check_linear(rows, K, M, GA_GATE_NONE, dtype) != GA_OK || ga::by_instruction(rows, M, dtype)) return 0;
+  if (dtype == GA_F32) return ga::linear_split_bytes(K, M);
   return ga::plan_of(rows, K, M, GA_GATE_NONE, dtype, false).bytes;
 }
 
@@ -340,12 +349,15 @@ int ga_linear_act(const void *x, const void *weight, const void *bias, const voi
   hipStream_t s = (hipStream_t)stream;
   const LinearEnd end{bias, residual, y, M, activation};
   if (rows <= kGatedFewRows) return linear_few_launch(x, weight, end, rows, K, M, dtype, s);     // takes any address
-  if (by_instruction(rows, K, M, dtype)) return linear_f32_launch(x, weight, end, rows, K, M, s);
+  if (by_instruction(rows, M, dtype)) return linear_f32_launch(x, weight, end, rows, K, M, s);
   if (!operand_aligned(x, K, dtype) || !operand_aligned(weight, M, dtype)) return GA_EALIGN;
+  if (dtype == GA_F32) {
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < linear_split_bytes(K, M)) return GA_EWORKSPACE;
+    return linear_split_launch(x, weight, end, rows, K, M, workspace, s);
+  }
   const Plan p = plan_of(rows, K, M, activation, dtype, false);
   if (p.bytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes)) return GA_EWORKSPACE;
-  return dtype == GA_F32 ? forward<float>(x, weight, end, rows, K, M, p, (char *)workspace, s)
-                         : forward<bf16_t>(x, weight, end, rows, K, M, p, (char *)workspace, s);
+  return forward(x, weight, end, rows, K, M, p, (char *)workspace, s);
 }
 
 size_t ga_linear_act_backward_workspace_bytes(int64_t rows, int64_t K, int64_t M, int activation, int dtype) {

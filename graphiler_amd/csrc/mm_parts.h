@@ -57,7 +57,7 @@ static __global__ __launch_bounds__(kBlock) void join_parts_kernel(const float *
                                                             int splits) {
   for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < all; i += (int64_t)gridDim.x * kBlock) {
     float s = 0.0f;
-#pragma unroll 4
+#pragma unroll 16
     for (int k = 0; k < splits; ++k) s += parts[k * all + i];
     f32_to_elem(s, i >= n ? out1[i - n] : out0[i]);
   }

@@ -257,12 +257,22 @@ __device__ __forceinline__ void tile_mm(const TileMm &p, const Epi &epi) {
   const int first = (int)blockIdx.y * share, last = min(all, first + share);
 
   typename M::result acc[TM][TN];
+  if constexpr (Epi::kStarts) {     // the sums begin with a value of their column: in the store it would be read for every row
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+    for (int j = 0; j < TN; ++j) {
+      const int64_t col = col0 + (j >= TC ? BC : 0) + wn * TC * kT + j % TC * kT + (threadIdx.x & (kWave - 1)) / kT * 4;
+      const floatx4 b = epi.start(col);
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+      for (int i = 0; i < TM; ++i) acc[i][j] = b;
+    }
+  } else {
 #pragma unroll
-      for (int r = 0; r < 4 * M::kQuads; ++r) acc[i][j][r] = 0.0f;
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4 * M::kQuads; ++r) acc[i][j][r] = 0.0f;
+  }
 
   // where the step to be fetched next begins; `to_fetch` steps are left
   int to_fetch = last - first;
@@ -531,14 +541,17 @@ __global__ __launch_bounds__(WM *WN *kWave, BLOCKS > 64 ? 1 : 2) void tile_mm_ke
   tile_mm<FP8, A_ACROSS, B_ACROSS, PAIR, WM, WN, TM, TN, BLOCKS>(p, epi);
 }
 
-// Results as they are stored: `bits` holds four adjacent values, a 16-byte chunk kChunk of them.
+// Results as they are stored: `bits` holds four adjacent values, a 16-byte chunk kChunk of them.  kStarts: the epilogue says
+// what the sums of a column begin with (of one product, in bf16).
 template <typename T> struct Stored;
 template <> struct Stored<float> {
+  static constexpr bool kStarts = false;
   typedef floatx4 bits;
   static constexpr int kSize = 4, kChunk = 4;
   static __device__ __forceinline__ bits pack(const floatx4 &v) { return v; }
 };
 template <> struct Stored<bf16_t> {
+  static constexpr bool kStarts = false;
   typedef uintx2 bits;
   static constexpr int kSize = 2, kChunk = 8;
   static __device__ __forceinline__ bits pack(const floatx4 &v) {
