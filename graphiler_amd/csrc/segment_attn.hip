@@ -235,33 +235,44 @@ __global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 ? 2 : 1) void segm
   segment_attn<T, WIDE, F>(p);
 }
 
-// The parts of a query's keys: a wavefront for each row.
+// The parts of a query's keys: a wavefront for each row, a lane for each part's maximum and sum (64 at most).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void segment_attn_join_kernel(Forward p) {
   const int64_t all = p.nq * p.heads, id = (int64_t)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
   if (id >= all) return;
   const int lane = threadIdx.x & (kWave - 1);
-  const float *ml = p.parts + (int64_t)p.splits * all * p.dim;
+  const float *ml = p.parts + (int64_t)p.splits * all * p.dim + id * 2;
   float most = -INFINITY, sum = 0.0f;
-  for (int z = 0; z < p.splits; ++z) most = fmaxf(most, ml[(z * all + id) * 2]);
-  const float from = most == -INFINITY ? 0.0f : most;
-  float o[2] = {0.0f, 0.0f};
-  for (int z = 0; z < p.splits; ++z) {
-    const float m = ml[(z * all + id) * 2], l = ml[(z * all + id) * 2 + 1];
-    const float f = __builtin_amdgcn_exp2f(m - from);
-    if (l == 0.0f) continue;
-    sum += l * f;
+  if (lane < p.splits) {
+    most = ml[lane * all * 2];
+    sum = ml[lane * all * 2 + 1];
+  }
+  float from = most;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (lane + j * kWave < p.dim) o[j] += f * p.parts[(z * all + id) * p.dim + lane + j * kWave];
+  for (int o = 32; o > 0; o >>= 1) from = fmaxf(from, __shfl_xor(from, o));
+  const float base = from == -INFINITY ? 0.0f : from;
+  const float f = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(most - base);
+  sum *= f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  float r[2] = {0.0f, 0.0f};
+  const float *parts = p.parts + id * p.dim;
+#pragma unroll 4
+  for (int z = 0; z < p.splits; ++z) {
+    const float w = __shfl(f, z);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int c = lane + j * kWave;
+      if (c < p.dim) r[j] += w == 0.0f ? 0.0f : w * parts[z * all * p.dim + c];
+    }
   }
   const int64_t query = id / p.heads;
   const int head = (int)(id % p.heads);
   T *out = (T *)p.out + query * p.out_row + head * p.out_head;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    if (lane + j * kWave < p.dim) f32_to_elem(sum == 0.0f ? 0.0f : o[j] / sum, out[lane + j * kWave]);
-  if (p.lse && lane == 0) p.lse[head * p.nq + query] = lse_of(most, sum);
+    if (lane + j * kWave < p.dim) f32_to_elem(sum == 0.0f ? 0.0f : r[j] / sum, out[lane + j * kWave]);
+  if (p.lse && lane == 0) p.lse[head * p.nq + query] = lse_of(from, sum);
 }
 
 enum Cutting { kShared, kSingle, kApart };

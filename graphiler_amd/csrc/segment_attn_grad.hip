@@ -20,6 +20,8 @@ struct Backward : SegAttn {
   float *delta;                          // (heads, nq)
   void *gq, *gk, *gv;                    // (rows, heads, dim), contiguous
   int64_t tiles;
+  int parts;                             // of the heads that share keys, each its own sums of dk and dv
+  float *part_sums;                      // (dk and dv, parts, nk, kv_heads, dim)
   int out_whole;                         // rows of out are whole pieces; the others always are, as they lie or laid out
 };
 
@@ -183,17 +185,19 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
   }
 }
 template <typename T, int WIDE, typename F>
-__global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 && WIDE <= 64 ? 2 : 1) void segment_attn_dq_kernel(Backward p) {
+__global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 ? 2 : 1) void segment_attn_dq_kernel(Backward p) {
   segment_attn_dq<T, WIDE, F>(p);
 }
 
-// A lane's share of 32 numbers, as it holds 16 of 32 rows of results; zeros behind the `left` that there are.
-__device__ __forceinline__ void load_numbers(const float *from, int64_t left, floatx4 (&f)[4]) {
+// 64 numbers from `from` on, of which `left` are there, into LDS (zeros for the others), and a lane's share of 32 of them: 4 of
+// the 16 rows of results that it holds.
+__device__ __forceinline__ void move_numbers(const float *from, int64_t left, lds_char *to) {
+  const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, (int)(min((int64_t)64, left) * 4), 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to, 4, (threadIdx.x & (kWave - 1)) * 4, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 numbers(const lds_char *at, int i) {
   const int h = (threadIdx.x >> 5) & 1;
-  const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, (int)(min((int64_t)32, left) * 4), 0x00020000);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    f[i] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, (i * 8 + h * 4) * 4, 0, 0));
+  return *reinterpret_cast<const __attribute__((address_space(3))) floatx4 *>(at + (i * 8 + h * 4) * 4);
 }
 
 // Which tile of which head of a group comes next.
@@ -211,12 +215,14 @@ struct Place {
 };
 
 // dk and dv: 32 keys of a head a wavefront.
-template <typename T, int WIDE, typename F>
+enum { kGradK = 1, kGradV = 2 };
+template <typename T, int WIDE, typename F, int WHICH>
 __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
+  constexpr bool kDk = WHICH & kGradK, kDv = WHICH & kGradV;
   typedef Rows<T, WIDE> R;
   constexpr int QUERIES = F::kDeep;
   typedef RowMoves<T, WIDE, QUERIES, F::kMovers> Moves;
-  constexpr int kStage = 2 * Moves::kBytes, kRegions = F::kApart ? F::kWaves : 1, kLds = kStage * kRegions;
+  constexpr int kNumbers = 2 * Moves::kBytes, kStage = kNumbers + 512, kRegions = F::kApart ? F::kWaves : 1, kLds = kStage * kRegions;
   __shared__ __attribute__((aligned(1024))) char stage0[kLds], stage1[F::kStages == 2 ? kLds : 16];
   int kv;
   int64_t tile;
@@ -232,7 +238,8 @@ __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
   uintx4 k[R::kSteps], v[R::kSteps];
   const int64_t row0 = seg.k0 + first;
   load_row<T, WIDE>((const char *)p.k + row0 * p.k_row + kv * p.k_head, (uint32_t)(n * p.k_row), there, p.dim, true, k);
-  load_row<T, WIDE>((const char *)p.v + row0 * p.v_row + kv * p.v_head, (uint32_t)(n * p.v_row), there, p.dim, true, v);
+  if constexpr (kDk)
+    load_row<T, WIDE>((const char *)p.v + row0 * p.v_row + kv * p.v_head, (uint32_t)(n * p.v_row), there, p.dim, true, v);
   const float c = p.scale * kLog2e;
 
   // the first query that sees the lane's key, the wavefront's first and last and the workgroup's first
@@ -241,15 +248,17 @@ __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
   const int by_any = p.causal ? first + less : 0, by_all = p.causal ? first + 31 + less : 0;
   const int begin = p.causal ? max(0, seg.tile * F::kRows + less) / QUERIES : 0;
   const int end = (seg.q_len + QUERIES - 1) / QUERIES;
-  const int tiles = max(0, end - begin), all = tiles * p.group;
+  const int tiles = max(0, end - begin);
+  // of the heads that share these keys, the workgroup's part
+  const int heads = (p.group + p.parts - 1) / p.parts, part = blockIdx.y, all = tiles * max(0, min(heads, p.group - part * heads));
 
   // tile t of all heads' is tile begin + t % tiles of head t / tiles
   constexpr int kTurn = F::kApart ? F::kWaves : 1;
   Moves mq, mg;
   mq.init(p.q_row, p.dim, F::kApart ? 0 : wave);
   mg.init(p.grad_row, p.dim, F::kApart ? 0 : wave);
-  const char *const q_first = (const char *)p.q + seg.q0 * p.q_row + kv * p.group * p.q_head;
-  const char *const g_first = (const char *)p.grad + seg.q0 * p.grad_row + kv * p.group * p.grad_head;
+  const char *const q_first = (const char *)p.q + seg.q0 * p.q_row + (kv * p.group + part * heads) * p.q_head;
+  const char *const g_first = (const char *)p.grad + seg.q0 * p.grad_row + (kv * p.group + part * heads) * p.grad_head;
   int to_fetch = F::kApart ? wave : 0;
   Place fetched(to_fetch, tiles);
   auto fetch = [&](lds_char *to) {
@@ -257,6 +266,10 @@ __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
     const int query0 = (begin + fetched.tile) * QUERIES;
     mq.move(q_first + query0 * p.q_row + fetched.head * p.q_head, seg.q_len - query0, to);
     mg.move(g_first + query0 * p.grad_row + fetched.head * p.grad_head, seg.q_len - query0, to + Moves::kBytes);
+    // the log-sum-exps and deltas of the tile's queries
+    const int64_t number = (int64_t)(part * heads + fetched.head + kv * p.group) * p.nq + seg.q0 + query0;
+    if (F::kMovers == 1 || wave == 0) move_numbers(p.lse + number, p.nq - seg.q0 - query0, to + kNumbers);
+    if (kDk && (F::kMovers == 1 || wave == 1)) move_numbers(p.delta + number, p.nq - seg.q0 - query0, to + kNumbers + 256);
     to_fetch += kTurn;
     fetched.next(kTurn, tiles);
   };
@@ -267,77 +280,83 @@ __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
 
-  auto block = [&](const lds_char *queries, const lds_char *grads, int b, int query0, int q_head, auto edge) {
+  auto block = [&](const lds_char *queries, const lds_char *grads, const lds_char *more, int b, int query0, auto edge) {
     constexpr bool kEdge = decltype(edge)::value;
-    // of the 32 queries, four adjacent ones a group; what lies behind the segment is not counted, behind the tensor zero
-    floatx4 lse[4], delta[4];
-    const int64_t row = q_head * p.nq + seg.q0 + query0, left = p.nq - seg.q0 - query0;
-    load_numbers(p.lse + row, left, lse);
-    load_numbers(p.delta + row, left, delta);
     floatx16 s, dp;
+    floatx4 lse, delta;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < R::kSteps; ++i) s = mma_piece<T>(R::row(queries, row_at, b, i), k[i], s);
     if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < R::kSteps; ++i) dp = mma_piece<T>(R::row(grads, row_at, b, i), v[i], dp);
+    for (int i = 0; i < R::kSteps; ++i)
+      if constexpr (kDk) dp = mma_piece<T>(R::row(grads, row_at, b, i), v[i], dp);
     if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float l = lse[r / 4][r % 4];
+      if (r % 4 == 0) {
+        lse = numbers(more + b * 128, r / 4);
+        if constexpr (kDk) delta = numbers(more + 256 + b * 128, r / 4);
+      }
+      const float l = lse[r % 4];
       const float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, l == -INFINITY ? -INFINITY : -kLog2e * l));
-      const float ds = w * (dp[r] - delta[r / 4][r % 4]);
       const bool counts = !kEdge || (result_row(r) >= by - query0 - 4 * h && result_row(r) < seg.q_len - query0 - 4 * h);
       s[r] = counts ? w : 0.0f;
-      dp[r] = counts ? ds : 0.0f;
+      if constexpr (kDk) dp[r] = counts ? w * (dp[r] - delta[r % 4]) : 0.0f;
     }
-    const bool found = add_columns<T, WIDE, kEdge>(grads, col_at, b, s, dv);
-    if constexpr (kEdge) {
+    bool found = false;
+    if constexpr (kDv) found = add_columns<T, WIDE, kEdge>(grads, col_at, b, s, dv);
+    if constexpr (kEdge && kDv) {
       if (__ballot(found)) {             // what is not finite counts for the keys that its query sees and for no other
 #pragma unroll 1
         for (int r = 0; r < 32; ++r)
           add_not_finite<T, WIDE>(grads, b * 32 + r, query0 + r >= by && query0 + r < seg.q_len, dv);
       }
     }
-    add_columns<T, WIDE, kEdge>(queries, col_at, b, dp, dk);
+    if constexpr (kDk) add_columns<T, WIDE, kEdge>(queries, col_at, b, dp, dk);
   };
   Place used(F::kApart ? wave : 0, tiles);
   auto use = [&](int, const lds_char *here) {
-    const int tile0 = (begin + used.tile) * QUERIES, q_head = kv * p.group + used.head;
+    const int tile0 = (begin + used.tile) * QUERIES;
 #pragma unroll
     for (int b = 0; b < QUERIES / 32; ++b) {
       const int query0 = tile0 + b * 32;
       if (first >= seg.k_len || query0 >= seg.q_len || query0 + 31 < by_any) continue;
-      if (query0 >= by_all && query0 + 32 <= seg.q_len) block(here, here + Moves::kBytes, b, query0, q_head, std::false_type());
-      else block(here, here + Moves::kBytes, b, query0, q_head, std::true_type());
+      if (query0 >= by_all && query0 + 32 <= seg.q_len) block(here, here + Moves::kBytes, here + kNumbers, b, query0, std::false_type());
+      else block(here, here + Moves::kBytes, here + kNumbers, b, query0, std::true_type());
     }
     used.next(kTurn, tiles);
   };
   const int region = F::kApart ? wave * kStage : 0;
   through_tiles<F>(0, all, wave, (lds_char *)stage0 + region, (lds_char *)stage1 + (F::kStages == 2 ? region : 0), fetch, use);
-  const int64_t to = (at * (p.heads / p.group) + kv) * p.dim;
-  if constexpr (F::kApart) {
-    static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
-    Gathered<WIDE, F::kWaves> sums;
-    sums.leave((lds_char *)stage0 + region, dk, 1.0f);
-    __syncthreads();
-    sums.take((const lds_char *)stage0, kStage, wave);
-    sums.store((T *)p.gk + to, there, p.dim, wave, p.scale);
-    __syncthreads();
-    sums.leave((lds_char *)stage0 + region, dv, 1.0f);
-    __syncthreads();
-    sums.take((const lds_char *)stage0, kStage, wave);
-    sums.store((T *)p.gv + to, there, p.dim, wave, 1.0f);
+  const int64_t to = (at * (p.heads / p.group) + kv) * p.dim, values = p.nk * (p.heads / p.group) * p.dim;
+  auto leave = [&](const floatx16 (&sum)[R::kCols], auto *grad, float by) {
+    if constexpr (F::kApart) {
+      static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
+      Gathered<WIDE, F::kWaves> sums;
+      __syncthreads();
+      sums.leave((lds_char *)stage0 + region, sum, 1.0f);
+      __syncthreads();
+      sums.take((const lds_char *)stage0, kStage, wave);
+      sums.store(grad + to, there, p.dim, wave, by);
+    } else {
+      store_row<std::remove_pointer_t<decltype(grad)>, R::kCols>(grad + to, there, p.dim, sum, by);
+    }
+  };
+  if (p.parts == 1) {
+    if constexpr (kDk) leave(dk, (T *)p.gk, p.scale);
+    if constexpr (kDv) leave(dv, (T *)p.gv, 1.0f);
   } else {
-    store_row<T, R::kCols>((T *)p.gk + to, there, p.dim, dk, p.scale);
-    store_row<T, R::kCols>((T *)p.gv + to, there, p.dim, dv, 1.0f);
+    if constexpr (kDk) leave(dk, p.part_sums + part * values, p.scale);
+    if constexpr (kDv) leave(dv, p.part_sums + (p.parts + part) * values, 1.0f);
   }
 }
-// Two wavefronts a SIMD where their sums and operands (128 WIDE / 32 and 32 WIDE / 64 registers) leave room for it.
-template <typename T, int WIDE, typename F>
-__global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 && WIDE <= 64 ? 2 : 1) void segment_attn_dkv_kernel(Backward p) {
-  segment_attn_dkv<T, WIDE, F>(p);
+// Two wavefronts a SIMD; not where dk of 128 columns, with k, v and both products in registers, would spill (8192 x 8192 x 8 heads
+// 1330 -> 1258 us in all, causal sequences of 16 heads that share four 1224 -> 1050).
+template <typename T, int WIDE, typename F, int WHICH>
+__global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 && (WIDE < 128 || WHICH != kGradK) ? 2 : 1) void segment_attn_dkv_kernel(Backward p) {
+  segment_attn_dkv<T, WIDE, F, WHICH>(p);
 }
 
 enum Cutting { kShared, kSingle, kApart };
@@ -357,12 +376,42 @@ int launch_dq(Backward p, hipStream_t s) {
   hipLaunchKernelGGL((segment_attn_dq_kernel<T, WIDE, F>), dim3((unsigned)grid), dim3(F::kWaves * kWave), 0, s, p);
   return launch_status();
 }
+// Sums of the parts, in their order.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void segment_attn_parts_kernel(Backward p, int64_t values) {
+  const float *from = p.part_sums + (int64_t)blockIdx.y * p.parts * values;
+  T *to = (T *)(blockIdx.y ? p.gv : p.gk);
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < values; i += (int64_t)gridDim.x * kBlock) {
+    float s = 0.0f;
+    for (int k = 0; k < p.parts; ++k) s += from[k * values + i];
+    f32_to_elem(s, to[i]);
+  }
+}
+
+// Into how many parts the heads that share keys are cut: until there are 1024 workgroups of 128 keys, which two a compute unit take
+// in two turns; those of a causal sequence's first keys have twice the work of the average.
+int parts_of_group(int64_t segments, int64_t nk, int64_t heads, int64_t kv_heads) {
+  const int64_t group = heads / kv_heads, tiles = (nk + 127) / 128 > segments ? (nk + 127) / 128 : segments;
+  const int64_t n = (1023 + tiles * kv_heads) / (tiles * kv_heads > 0 ? tiles * kv_heads : 1);
+  return (int)(n < 1 ? 1 : n > group ? group : n);
+}
+
 template <typename T, int WIDE, typename F>
 int launch_dkv(Backward p, hipStream_t s) {
   p.tiles = segment_tiles(p.nk, 1, p.segments, F::kRows);
   const int64_t grid = p.tiles * (p.heads / p.group);
   if (grid > kMostLanes / (F::kWaves * kWave)) return GA_EUNSUPPORTED;
-  hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F>), dim3((unsigned)grid), dim3(F::kWaves * kWave), 0, s, p);
+  const dim3 blocks((unsigned)grid, (unsigned)p.parts), threads(F::kWaves * kWave);
+  constexpr bool kTwice = WIDE > 64;
+  hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F, kTwice ? kGradK : kGradK | kGradV>), blocks, threads, 0, s, p);
+  if constexpr (kTwice) {
+    if (int rc = launch_status()) return rc;
+    hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F, kGradV>), blocks, threads, 0, s, p);
+  }
+  if (int rc = launch_status()) return rc;
+  if (p.parts == 1) return GA_OK;
+  const int64_t values = p.nk * (p.heads / p.group) * p.dim, n = (values + kBlock - 1) / kBlock;
+  hipLaunchKernelGGL((segment_attn_parts_kernel<T>), dim3((unsigned)(n > 4096 ? 4096 : n), 2), dim3(kBlock), 0, s, p, values);
   return launch_status();
 }
 template <typename T, int WIDE>
@@ -399,6 +448,8 @@ size_t ga_segment_attention_backward_workspace_bytes(int64_t n_segments, int64_t
   using namespace ga;
   if (segment_attn_sizes(n_segments, n_queries, n_keys, heads, kv_heads, dim, dtype)) return 0;
   int64_t n = (n_queries * heads * 4 + 255) / 256 * 256;
+  const int parts = parts_of_group(n_segments, n_keys, heads, kv_heads);
+  if (parts > 1) n += (2 * parts * n_keys * kv_heads * dim * 4 + 255) / 256 * 256;
   if (!whole_rows(dim, dtype))
     n += 2 * segment_attn_laid_bytes(n_queries, heads, dim, dtype) + 2 * segment_attn_laid_bytes(n_keys, kv_heads, dim, dtype);
   return (size_t)n;
@@ -435,11 +486,14 @@ int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q
   p.out_whole = whole && aligned(out, 4);
   p.lse = lse;
   p.delta = (float *)workspace;
+  char *at = (char *)workspace + (n_queries * heads * 4 + 255) / 256 * 256;
+  p.parts = parts_of_group(n_segments, n_keys, heads, kv_heads);
+  p.part_sums = (float *)at;
+  if (p.parts > 1) at += (2 * p.parts * n_keys * kv_heads * dim * 4 + 255) / 256 * 256;
   p.gq = grad_q;
   p.gk = grad_k;
   p.gv = grad_v;
   if (!whole) {
-    char *at = (char *)workspace + (n_queries * heads * 4 + 255) / 256 * 256;
     const int64_t of_q = segment_attn_laid_bytes(n_queries, heads, dim, dtype);
     const int64_t of_k = segment_attn_laid_bytes(n_keys, kv_heads, dim, dtype);
     const int64_t head = (dim * e + 15) / 16 * 16;

@@ -1746,54 +1746,56 @@ def gated_linear_backward(grad_h, x, w_gate, w_up, activation: str = "silu"):
 SEGMENT_ATTENTION_MAX_DIM = 128
 
 
-def _rows_heads(x, name: str, like=None) -> None:
+def _rows_heads(x, name: str, device: int, dtype) -> None:
     """(rows, heads, dim) whose dim values lie next to each other; rows and heads may lie anywhere."""
     if not x.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if x.dim() != 3 or x.shape[1] == 0 or not 0 < x.shape[2] <= SEGMENT_ATTENTION_MAX_DIM:
         raise RuntimeError(f"{name} must be (rows, heads, dim) with at most {SEGMENT_ATTENTION_MAX_DIM} dim")
-    if x.shape[2] > 1 and x.stride(2) != 1:
+    if x.stride(2) != 1 and x.shape[2] > 1:
         raise RuntimeError(f"the last dimension of {name} must be contiguous")
-    if like is not None and (x.dtype != like.dtype or x.get_device() != like.get_device()):
+    if x.dtype is not dtype or x.get_device() != device:
         raise RuntimeError(f"{name} must be of the dtype and on the device of q")
 
 
-def _check_pointer(pointer, name: str, device) -> None:
+def _check_pointer(pointer, name: str, device: int) -> None:
+    if pointer.dtype is torch.int64 and pointer.dim() == 1 and pointer.get_device() == device and pointer.numel() \
+            and pointer.is_contiguous():
+        return
     _check_input(pointer, name)
-    if pointer.dtype != torch.int64 or pointer.dim() != 1 or pointer.numel() == 0 or pointer.get_device() != device:
-        raise RuntimeError(f"{name} must be (segments + 1,) int64 on the device of q")
+    raise RuntimeError(f"{name} must be (segments + 1,) int64 on the device of q")
 
 
 def _in_pieces(x):
     """Heads whose rows are whole 16-byte pieces, as the kernels read them; a copy where they lie otherwise."""
     size = x.element_size()
-    if x.shape[2] * size % 16 == 0 and (x.data_ptr() % 16 or x.stride(0) * size % 16 or x.stride(1) * size % 16):
+    if x.shape[2] * size % 16 == 0 and (x.data_ptr() | x.stride(0) * size | x.stride(1) * size) % 16:
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
 
 def _attention_args(q, k, v, q_pointer, k_pointer, scale):
-    _rows_heads(q, "q")
+    device, dtype = q.get_device(), q.dtype
+    _rows_heads(q, "q", device, dtype)
     dt = _feat_dtype(q, "q")
-    _rows_heads(k, "k", q)
-    _rows_heads(v, "v", q)
-    if k.shape != v.shape or k.shape[2] != q.shape[2] or q.shape[1] % k.shape[1]:
+    _rows_heads(k, "k", device, dtype)
+    _rows_heads(v, "v", device, dtype)
+    (nq, heads, dim), (nk, kv_heads, kv_dim) = q.shape, k.shape
+    if k.shape != v.shape or kv_dim != dim or heads % kv_heads:
         raise RuntimeError("k and v must be (rows, kv_heads, dim) with q's dim and a divisor of its heads")
-    _check_pointer(q_pointer, "q_pointer", q.get_device())
+    _check_pointer(q_pointer, "q_pointer", device)
     if k_pointer is None:
         k_pointer = q_pointer
-    else:
-        _check_pointer(k_pointer, "k_pointer", q.get_device())
-    if k_pointer.numel() != q_pointer.numel():
-        raise RuntimeError("q_pointer and k_pointer must have one entry more than there are segments")
-    if k_pointer is q_pointer and k.shape[0] != q.shape[0]:
-        raise RuntimeError("k and v must have q's rows where there is no k_pointer")
-    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+        if nk != nq:
+            raise RuntimeError("k and v must have q's rows where there is no k_pointer")
+    elif k_pointer is not q_pointer:
+        _check_pointer(k_pointer, "k_pointer", device)
+        if k_pointer.numel() != q_pointer.numel():
+            raise RuntimeError("q_pointer and k_pointer must have one entry more than there are segments")
+    scale = dim ** -0.5 if scale is None else float(scale)
     if scale == 0 or not abs(scale) < float("inf"):
         raise RuntimeError("scale must be finite and not 0")
-    sizes = (int(q_pointer.numel()) - 1, int(q.shape[0]), int(k.shape[0]), int(q.shape[1]), int(k.shape[1]),
-             int(q.shape[2]))
-    return dt, k_pointer, scale, sizes
+    return dt, k_pointer, scale, (q_pointer.numel() - 1, nq, nk, heads, kv_heads, dim)
 
 
 def _placed(x):
@@ -1825,7 +1827,7 @@ class _SegmentAttention(torch.autograd.Function):
 def _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, return_lse):
     dt, k_pointer, scale, sizes = _attention_args(q, k, v, q_pointer, k_pointer, scale)
     k, v = _in_pieces(k), _in_pieces(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)      # contiguous, whatever q's strides
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if return_lse else None
     n = capi.load().ga_segment_attention_workspace_bytes(*sizes, dt)
     ws = _scratch(n, q.device)
@@ -1862,7 +1864,7 @@ def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer
     _check_input(lse, "lse")
     if lse.dtype != torch.float32 or lse.shape != (q.shape[1], q.shape[0]) or lse.get_device() != q.get_device():
         raise RuntimeError("lse must be the (heads, queries) float32 tensor that segment_attention returned")
-    _rows_heads(grad_out, "grad_out", q)
+    _rows_heads(grad_out, "grad_out", q.get_device(), q.dtype)
     if grad_out.shape != q.shape:
         raise RuntimeError("grad_out must have q's shape")
     grad_out = grad_out.contiguous()
