@@ -233,6 +233,7 @@ size_t linear_split_bytes(int64_t K, int64_t M) { return (size_t)(3 * 2 * padded
 
 int linear_split_launch(const void *x, const void *w, const LinearEnd &end, int64_t rows, int64_t K, int64_t M, void *workspace,
                         hipStream_t s) {
+  if (tiles_of(rows, M, 32, 128) > kMostLanes / (8 * kWave)) return GA_EUNSUPPORTED;       // of the smallest tiles
   Split p;
   p.x = (const float *)x;
   p.w = (const bf16_t *)workspace;

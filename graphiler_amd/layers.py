@@ -297,3 +297,34 @@ def hgt_block(g: DGLGraph, h, norm_attention, attention, norm_ff, ff, heads: int
         return t + _feed_forward_fp8((x8, scales), *ff, activation, h.dtype)
     x, t = ops.rms_norm(a, norm_ff, residual=h, eps=eps)
     return t + feed_forward(x, *ff, activation)
+
+
+def attention_block(h, pointer, norm_attention, attention, norm_ff, ff, heads: int, kv_heads: int | None = None,
+                    causal: bool = False, activation: str = "silu", eps: float = 1e-6):
+    """A transformer's layer over packed rows, every row attending inside its segment (the nodes of each graph of a
+    batch, sequences of nodes), with norms in front of both halves and a residual stream behind them:
+
+      q, k, v = rms_norm(h, norm_attention) @ w_qkv + b_qkv
+      t       = h + segment_attention(q, k, v, pointer) @ w_out + b_out
+      out     = t + feed_forward(rms_norm(t, norm_ff), *ff)
+
+    ``h`` (rows, hidden); ``attention``: w_qkv (hidden, (heads + 2 kv_heads) dim), its bias or None, w_out (heads dim,
+    hidden), its bias or None; ``pointer``: (segments + 1,) as :func:`graphiler_amd.ops.segment_attention` takes it.  q, k
+    and v are columns of one product and are read where they lie; both residuals are added in the store of a
+    product.  ``ff``: the three weights of :func:`feed_forward`, as tensors or in 8 bits; differentiable with tensors."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    w_qkv, b_qkv, w_out, b_out = attention
+    in_8_bits = _in_8_bits(*ff)
+    width = int(w_qkv.shape[1])
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or width % (heads + 2 * kv_heads):
+        raise RuntimeError("w_qkv must have a column for each value of heads + 2 kv_heads heads, heads a multiple of kv_heads")
+    dim = width // (heads + 2 * kv_heads)
+    x = ops.linear_act(ops.rms_norm(h, norm_attention, eps=eps), w_qkv, bias=b_qkv).view(-1, heads + 2 * kv_heads, dim)
+    q, k, v = x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]
+    a = ops.segment_attention(q, k, v, pointer, causal=causal)
+    t = ops.linear_act(a.reshape(-1, heads * dim), w_out, bias=b_out, residual=h)
+    if in_8_bits:
+        return t + _feed_forward_fp8(ops.rms_norm_fp8(t, norm_ff, eps=eps), *ff, activation, h.dtype)
+    w_gate, w_up, w_down = ff
+    hidden = ops.gated_linear(ops.rms_norm(t, norm_ff, eps=eps), w_gate, w_up, activation)
+    return ops.linear_act(hidden, w_down, residual=t)

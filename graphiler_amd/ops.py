@@ -1864,10 +1864,10 @@ def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer
     _check_input(lse, "lse")
     if lse.dtype != torch.float32 or lse.shape != (q.shape[1], q.shape[0]) or lse.get_device() != q.get_device():
         raise RuntimeError("lse must be the (heads, queries) float32 tensor that segment_attention returned")
+    grad_out = grad_out.contiguous()                     # a sum's gradient has no strides
     _rows_heads(grad_out, "grad_out", q.get_device(), q.dtype)
     if grad_out.shape != q.shape:
         raise RuntimeError("grad_out must have q's shape")
-    grad_out = grad_out.contiguous()
     q, k, v, grad_out = _in_pieces(q), _in_pieces(k), _in_pieces(v), _in_pieces(grad_out)
     gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     n = capi.load().ga_segment_attention_backward_workspace_bytes(*sizes, dt)
