@@ -196,6 +196,53 @@ __global__ __launch_bounds__(8 * kWave) void embedding_join_kernel(const float *
   }
 }
 
+// Few places: a workgroup for each row of the table looks through all of them, a quarter by each wavefront in its turn, 512
+// columns blockIdx.y.  One launch in the place of the sort's and the sums' eleven (us, 512 places of 64 columns, 300 rows 47 -> 9).
+constexpr int64_t kFewPlaces = 1024, kFewTable = 8192;
+template <typename T>
+__global__ __launch_bounds__(kBlock) void embedding_few_kernel(const T *__restrict__ gy, const void *__restrict__ ids, int bits,
+                                                               T *__restrict__ grad, int n_ids, int64_t cols, float scale) {
+  constexpr int kWaves = kBlock / kWave, kDeep = 4;
+  __shared__ float sums[kWaves][kWave * kVec];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t row = blockIdx.x, col = ((int64_t)blockIdx.y * kWave + lane) * kVec;
+  const int n = (int)max((int64_t)0, min((int64_t)kVec, cols - col));
+  const int share = (n_ids + kWaves * kWave - 1) / (kWaves * kWave) * kWave, end = min(n_ids, (wave + 1) * share);
+  float f[kVec] = {};
+  for (int i0 = wave * share; i0 < end; i0 += kWave) {
+    const int i = i0 + lane;
+    const bool named = i < end && (bits == 64 ? ((const int64_t *)ids)[i] : (int64_t)((const int32_t *)ids)[i]) == row;
+    uint64_t found = __ballot(named);
+    while (found) {
+      int place[kDeep];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        place[d] = found ? i0 + __ffsll((unsigned long long)found) - 1 : -1;
+        found &= found - 1;
+      }
+      float g[kDeep][kVec];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) load_group(gy + (int64_t)max(place[d], 0) * cols + col, place[d] < 0 ? 0 : n, g[d]);
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) f[j] += g[d][j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) sums[wave][j * kWave + lane] = f[j];
+  __syncthreads();
+  if (wave != 0 || n == 0) return;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    f[j] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) f[j] += sums[w][j * kWave + lane];
+    f[j] *= scale;
+  }
+  store_group(grad + row * cols + col, n, f);
+}
+
 template <typename W>
 __global__ __launch_bounds__(kBlock) void embedding_zero_kernel(W *__restrict__ out, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) out[i] = 0;
@@ -207,6 +254,7 @@ struct Plan {
   int64_t keys, pointer, places, status, parts, group;       // bytes from the workspace's start
   size_t group_bytes, bytes;
 };
+bool few(int64_t n_ids, int64_t n_table) { return n_ids <= kFewPlaces && n_table <= kFewTable; }
 Plan plan_of(int64_t n_ids, int64_t n_table, int64_t cols) {
   Plan p;
   int64_t at = 0;
@@ -292,7 +340,7 @@ int ga_embedding(const void *table, const void *ids, int idx_bits, void *y, int6
 
 size_t ga_embedding_backward_workspace_bytes(int64_t n_ids, int64_t n_table, int64_t cols) {
   if (n_ids <= 0 || n_table <= 0 || cols <= 0 || n_ids > 0x7ffffffe || n_table > 0x7ffffffd) return 0;
-  return ga::plan_of(n_ids, n_table, cols).bytes;
+  return ga::few(n_ids, n_table) ? 0 : ga::plan_of(n_ids, n_table, cols).bytes;
 }
 
 int ga_embedding_backward(const void *grad_y, const void *ids, int idx_bits, void *grad_table, int64_t n_ids, int64_t n_table,
@@ -311,6 +359,16 @@ int ga_embedding_backward(const void *grad_y, const void *ids, int idx_bits, voi
     } else {
       hipLaunchKernelGGL(embedding_zero_kernel<uint16_t>, dim3(4096), dim3(kBlock), 0, s, (uint16_t *)grad_table, n / 2);
     }
+    return launch_status();
+  }
+  if (few(n_ids, n_table)) {
+    const dim3 grid((unsigned)n_table, (unsigned)((cols + kWave * kVec - 1) / (kWave * kVec)));
+    if (dtype == GA_F32)
+      hipLaunchKernelGGL((embedding_few_kernel<float>), grid, dim3(kBlock), 0, s, (const float *)grad_y, ids, idx_bits,
+                         (float *)grad_table, (int)n_ids, cols, scale);
+    else
+      hipLaunchKernelGGL((embedding_few_kernel<bf16_t>), grid, dim3(kBlock), 0, s, (const bf16_t *)grad_y, ids, idx_bits,
+                         (bf16_t *)grad_table, (int)n_ids, cols, scale);
     return launch_status();
   }
   const Plan p = plan_of(n_ids, n_table, cols);

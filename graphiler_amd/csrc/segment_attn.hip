@@ -156,7 +156,7 @@ __device__ __forceinline__ void segment_attn(const Forward &p) {
   const int block_last = min(seg.tile * F::kRows + F::kRows, rows) - 1;
   const int wanted = p.causal ? max(0, min(seg.k_len, block_last / p.pack + 1 + more)) : seg.k_len;
   int begin = 0, end = (wanted + KEYS - 1) / KEYS;
-  if (p.splits > 1) {
+  if (F::kApart && p.splits > 1) {
     const int share = (end + p.splits - 1) / p.splits;
     begin = min(end, (int)blockIdx.y * share);
     end = min(end, begin + share);
@@ -213,20 +213,22 @@ __device__ __forceinline__ void segment_attn(const Forward &p) {
     all.take((const lds_char *)stage0, kStage, wave);
   }
   const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (p.splits > 1) {
-    const int64_t n_all = p.nq * p.heads, id = (int64_t)blockIdx.y * n_all + at * p.heads + q_head;
-    if constexpr (F::kApart) all.store(p.parts + id * p.dim, there, p.dim, wave, 1.0f);
-    else store_row<float, R::kCols>(p.parts + id * p.dim, there, p.dim, st.o, 1.0f);
-    if (there && h == 0 && (!F::kApart || wave == 0)) {
-      float *ml = p.parts + (int64_t)p.splits * n_all * p.dim + id * 2;
-      ml[0] = most;
-      ml[1] = sum;
-    }
-    return;
-  }
   T *out = (T *)p.out + at * p.out_row + q_head * p.out_head;
-  if constexpr (F::kApart) all.store(out, there, p.dim, wave, by);
-  else store_row<T, R::kCols>(out, there, p.dim, st.o, by);
+  if constexpr (F::kApart) {
+    if (p.splits > 1) {
+      const int64_t n_all = p.nq * p.heads, id = (int64_t)blockIdx.y * n_all + at * p.heads + q_head;
+      all.store(p.parts + id * p.dim, there, p.dim, wave, 1.0f);
+      if (there && h == 0 && wave == 0) {
+        float *ml = p.parts + (int64_t)p.splits * n_all * p.dim + id * 2;
+        ml[0] = most;
+        ml[1] = sum;
+      }
+      return;
+    }
+    all.store(out, there, p.dim, wave, by);
+  } else {
+    store_row<T, R::kCols>(out, there, p.dim, st.o, by);
+  }
   if (p.lse && there && h == 0 && (!F::kApart || wave == 0)) p.lse[q_head * p.nq + at] = lse_of(most, sum);
 }
 // bf16: two wavefronts a SIMD at least.
@@ -360,7 +362,7 @@ int segment_attn_check(SegAttn &p, const void *q, const void *k, const void *v, 
   if (!aligned(q, e) || !aligned(k, e) || !aligned(v, e) || !aligned(q_pointer, 8) || !aligned(k_pointer, 8)) return GA_EALIGN;
   // offsets inside a tile of 64 rows are 32-bit numbers
   const int64_t far = (int64_t)1 << 24;
-  if (q_row * e > far || k_row * e > far || v_row * e > far || q_head * (heads / kv_heads) * e > far * 32) return GA_EUNSUPPORTED;
+  if (q_row * e > far || k_row * e > far || v_row * e > far) return GA_EUNSUPPORTED;
   p.q = q;
   p.k = k;
   p.v = v;
@@ -459,7 +461,7 @@ int ga_segment_attention(const void *q, int64_t q_row, int64_t q_head, const voi
   p.lse = lse;
   p.out_head = dim;
   p.out_row = heads * dim;
-  p.pack = c.pack;
+  p.pack = p.q_head * p.group < (int64_t)1 << 29 ? c.pack : 1;          // 32-bit offsets inside a tile of packed heads
   p.cutting = c.cutting;
   p.splits = c.splits;
   p.parts = (float *)((char *)workspace + c.parts);

@@ -1966,6 +1966,7 @@ def linear_act_backward(grad_y, x, weight, bias=None, activation=None):
 
 
 _ID_BITS = {torch.int64: 64, torch.int32: 32}
+EMBEDDING_MOST_RECORDED = 16 << 20     # more ids are sorted by a library, whose launches are its own
 
 
 def _check_ids(ids, device) -> int:
@@ -2012,7 +2013,8 @@ def embedding(table, ids, scale: float = 1.0):
 
 def embedding_backward(grad_y, ids, rows: int, scale: float = 1.0):
     """Gradient of the (rows, cols) table of :func:`embedding`: scale times the sum of the rows of grad_y whose id is
-    the row's; zeros for rows that no id names.  Summed in fp32, rounded once; the result has no gradient of its own."""
+    the row's; zeros for rows that no id names.  Summed in fp32, rounded once; the result has no gradient of its own.
+    More than 16 M ids cannot be recorded into a HIP graph."""
     _check_seen("embedding_backward", grad_y)
     _check_input(grad_y, "grad_y")
     dt = _feat_dtype(grad_y, "grad_y")
@@ -2020,6 +2022,8 @@ def embedding_backward(grad_y, ids, rows: int, scale: float = 1.0):
     if grad_y.dim() != ids.dim() + 1 or grad_y.shape[:-1] != ids.shape or grad_y.shape[-1] == 0 or rows < 0:
         raise RuntimeError("grad_y must have a row for each id, and rows must not be negative")
     cols = int(grad_y.shape[-1])
+    if ids.numel() > EMBEDDING_MOST_RECORDED and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"the gradient of more than {EMBEDDING_MOST_RECORDED} rows cannot be recorded into a HIP graph")
     grad = torch.empty((int(rows), cols), dtype=grad_y.dtype, device=grad_y.device)
     if grad.numel():
         n = capi.load().ga_embedding_backward_workspace_bytes(ids.numel(), int(rows), cols)

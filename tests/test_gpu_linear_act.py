@@ -8,7 +8,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from graphiler_amd import ops
+from graphiler_amd import capi, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -124,6 +124,19 @@ def test_operands_at_any_address_and_a_result_over_the_residual(dtype):
         for a, b2 in zip(ops.linear_act_backward(gy, x, w, bias=b, activation="gelu"),
                          ops.linear_act_backward(far, apart[0], apart[1], bias=apart[2], activation="gelu")):
             assert torch.equal(a, b2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,k,m", [(5, 64, 96), (40, 2048, 70), (700, 64, 256), (9000, 64, 512)])
+def test_the_c_entry_writes_over_the_residual(rows, k, m, dtype):
+    x, w, b, r = operands(rows, k, m, dtype, True, True)
+    want = ops.linear_act(x, w, bias=b, activation="silu", residual=r)
+    lib, dt = capi.load(), ops._DTYPES[dtype]
+    n = lib.ga_linear_act_workspace_bytes(rows, k, m, dt)
+    ws = torch.empty(n + 16, dtype=torch.uint8, device=DEV)
+    assert lib.ga_linear_act(x.data_ptr(), w.data_ptr(), b.data_ptr(), r.data_ptr(), r.data_ptr(), rows, k, m, capi.GA_GATE_SILU, dt,
+                             ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(r, want)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -112,7 +112,8 @@ def test_embedding_codes():
         assert call(**bad) == EINVAL, bad
     assert call(dt=9) == EUNSUPPORTED and call(cols=(1 << 20) + 1) == EUNSUPPORTED and call(n=1 << 42) == EUNSUPPORTED
     assert call(t=PTR + 1) == EALIGN and call(ids=PTR + 4) == EALIGN and call(ids=PTR + 2, bits=32) == EALIGN
-    size = lib.ga_embedding_backward_workspace_bytes(5, 10, 8)
+    size = lib.ga_embedding_backward_workspace_bytes(5000, 10, 8)
+    assert lib.ga_embedding_backward_workspace_bytes(5, 10, 8) == 0        # few places need none
     assert size > 0 and lib.ga_embedding_backward_workspace_bytes(1 << 31, 10, 8) == 0
 
     def back(gy=PTR, ids=PTR, bits=64, g=PTR, n=5, rows=10, cols=8, dt=BF16, ws=PTR, size=size):
@@ -121,7 +122,8 @@ def test_embedding_codes():
     assert back(rows=0) == 0
     assert back(gy=None) == EINVAL and back(g=None) == EINVAL and back(ids=None) == EINVAL and back(bits=8) == EINVAL
     assert back(n=1 << 31) == EUNSUPPORTED and back(rows=1 << 31) == EUNSUPPORTED
-    assert back(ws=None) == EWORKSPACE and back(ws=PTR + 64) == EWORKSPACE and back(size=size - 1) == EWORKSPACE
+    assert back(n=5000, ws=None) == EWORKSPACE and back(n=5000, ws=PTR + 64) == EWORKSPACE
+    assert back(n=5000, size=size - 1) == EWORKSPACE
 
 
 def test_operators_refuse_host_tensors_and_names():
