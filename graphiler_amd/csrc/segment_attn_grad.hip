@@ -1,13 +1,19 @@
 // Gradients of attention inside segments, from the log-sum-exps that the forward pass left:
 //
-//   p_ij = exp(s_ij - lse_i), delta_i = <do_i, o_i>, ds_ij = p_ij (<do_i, v_j> - delta_i)
+//   p_ij = exp(s_ij - lse_i), delta_i = <do_i, o_i> = sum_j p_ij <do_i, v_j>, ds_ij = p_ij (<do_i, v_j> - delta_i)
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i
 //
-// Two passes, each over 32 x 32 tiles that never leave the registers: one with 32 queries a wavefront over the keys (dq, and
+// Two kernels, each over 32 x 32 tiles that never leave the registers: one with 32 queries a wavefront over the keys (dq, and
 // delta on the way), one with 32 keys a wavefront over the queries of all heads that share them (dk and dv).  Both form the
 // scores again, seven products instead of the five of a single pass, which would have to add up dq from many workgroups in
 // an order of its own; here every sum has one.  p and ds are rounded to bf16 as operands (bf16 tensors), once each: what that
 // adds to a gradient is as large as its own rounding.
+//
+// Measured: 8192 x 8192, 8 heads, width 64 670 us (0.51 PFLOP/s of the five products), width 128 1515 (0.45); four causal
+// sequences of up to 4096, 16 heads that share four, width 128 1135 (of it dk 430, dv 260, parts added up 47; one workgroup for
+// all heads of a group 1300); 2048 segments of 34 rows, 8 heads of 32 134.  Delta from out, in one pass over the keys, took 550,
+// 1280, 1048 and 137 and left bf16's grad_q up to 1.9 times as far off as its own rounding, for 1.5 with it from the weights.
+// Held by latency: two wavefronts a SIMD where registers allow it, one for dk of wide heads.
 #include "segment_attn.h"
 
 namespace ga {
@@ -26,8 +32,8 @@ struct Backward : SegAttn {
 };
 
 // Products of results w (operand over rows 32 b ... of `t`) and its columns onto acc.  CLEAN: values of t that are not finite
-// count as zero; whether there were any.
-template <typename T, int WIDE, bool CLEAN>
+// count as zero; whether there were any.  LEFT: what w's rounding leaves is multiplied too.
+template <typename T, int WIDE, bool CLEAN, bool LEFT = false>
 __device__ __forceinline__ bool add_columns(const lds_char *t, int col_at, int b, const floatx16 &w,
                                             floatx16 (&acc)[Rows<T, WIDE>::kCols]) {
   typedef Rows<T, WIDE> R;
@@ -35,11 +41,16 @@ __device__ __forceinline__ bool add_columns(const lds_char *t, int col_at, int b
 #pragma unroll
   for (int i = 0; i < R::kParts; ++i) {
     const uintx4 o = operand_of<T>(w, i);
+    uintx4 left;
+    if constexpr (LEFT)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) left[j] = pack_bf16(w[8 * i + 2 * j] - bf16_lo(o[j]), w[8 * i + 2 * j + 1] - bf16_hi(o[j]));
 #pragma unroll
     for (int d = 0; d < R::kCols; ++d) {
       uintx4 v = R::col(t, col_at, b, i, d);
       if constexpr (CLEAN) found |= cleaned<T>(v);
       acc[d] = mma_piece<T>(v, o, acc[d]);
+      if constexpr (LEFT) acc[d] = mma_piece<T>(v, left, acc[d]);
       if constexpr (CLEAN) __builtin_amdgcn_sched_barrier(0);          // the rare tiles are not to decide what registers it takes
     }
   }
@@ -124,12 +135,13 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
 
-  // What a wavefront's queries see in one tile alone gives delta from the weights themselves, sum_j p_ij <do_i, v_j>: with
-  // few keys the rounding of out would be what their gradients are off by.
-  const bool alone = !F::kApart && by_any <= KEYS;
+  // The rounding of out would be part of delta and, where a few keys have most of the weight, half as much again of what the gradients
+  // are off by.  So bf16 takes delta from the weights themselves, sum_j p_ij <do_i, v_j>, going through the keys once for it and
+  // once with it (a tile that is the only one stays where it is).
   float weighed = 0.0f;
-  auto block = [&](const lds_char *keys, const lds_char *values, int b, int key0, auto edge, bool weigh) {
-    constexpr bool kEdge = decltype(edge)::value;
+  // WEIGH: only onto that sum.
+  auto block = [&](const lds_char *keys, const lds_char *values, int b, int key0, auto edge, auto weigh) {
+    constexpr bool kEdge = decltype(edge)::value, kWeigh = decltype(weigh)::value;
     floatx16 s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
@@ -141,42 +153,54 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
     if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float ds = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+      const float ds = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (kWeigh ? dp[r] : dp[r] - delta);
       s[r] = !kEdge || result_row(r) < seen - key0 - 4 * h ? ds : 0.0f;
-      if constexpr (kEdge) weighed += s[r];
+      if constexpr (kWeigh) weighed += s[r];
     }
-    if (kEdge && weigh) return;
     // A key that is not finite has scores that are not, which is what reaches the queries that see it.
-    add_columns<T, WIDE, kEdge>(keys, col_at, b, s, dq);
+    // A query's ds add up to nothing, so what keys have in common cancels and the rounding of ds as operands, whose errors do not
+    // cancel, counts for more than its half step: most where heads are narrow or keys few, and there they keep 16 bits.
+    constexpr bool kLeft = sizeof(T) == 2 && (WIDE == 32 || F::kWaves == 1);
+    if constexpr (!kWeigh) add_columns<T, WIDE, kEdge, kLeft>(keys, col_at, b, s, dq);
   };
-  auto use = [&](int t, const lds_char *here) {
-    if (t * KEYS >= by_any) return;
-    // `alone`: once for delta, once with it
-    float known = delta;
-    if (alone) delta = weighed = 0.0f;
-#pragma unroll 1
-    for (int pass = alone ? 0 : 1; pass < 2; ++pass) {
+  auto tile_of = [&](int t, const lds_char *here, auto weigh) {
 #pragma unroll
-      for (int b = 0; b < KEYS / 32; ++b) {
-        const int key0 = t * KEYS + b * 32;
-        if (key0 >= by_any) continue;
-        if (!alone && key0 + 32 <= by_all) block(here, here + Moves::kBytes, b, key0, std::false_type(), false);
-        else block(here, here + Moves::kBytes, b, key0, std::true_type(), pass == 0);
-      }
-      if (pass == 0) {
-        delta = weighed + other_half(weighed);
-        if (!(fabsf(delta) < INFINITY)) delta = known;
-      }
+    for (int b = 0; b < KEYS / 32; ++b) {
+      const int key0 = t * KEYS + b * 32;
+      if (key0 >= by_any) continue;
+      if (key0 + 32 <= by_all) block(here, here + Moves::kBytes, b, key0, std::false_type(), weigh);
+      else block(here, here + Moves::kBytes, b, key0, std::true_type(), weigh);
     }
   };
   const int region = F::kApart ? wave * kStage : 0;
-  through_tiles<F>(0, end, wave, (lds_char *)stage0 + region, (lds_char *)stage1 + (F::kStages == 2 ? region : 0), fetch, use);
+  lds_char *const L0 = (lds_char *)stage0 + region, *const L1 = (lds_char *)stage1 + (F::kStages == 2 ? region : 0);
+  if constexpr (sizeof(T) == 2) {
+    through_tiles<F>(0, end, wave, L0, L1, fetch, [&](int t, const lds_char *here) { tile_of(t, here, std::true_type()); });
+    weighed += other_half(weighed);
+    if constexpr (F::kApart) {
+      __shared__ float sums[F::kWaves][32];
+      if (h == 0) sums[wave][n] = weighed;
+      __syncthreads();
+      weighed = 0.0f;
+#pragma unroll
+      for (int w = 0; w < F::kWaves; ++w) weighed += sums[w][n];
+    } else {
+      __syncthreads();
+    }
+    if (fabsf(weighed) < INFINITY) delta = weighed;          // what is not finite has results that are not either
+    if (end > kTurn) {
+      to_fetch = F::kApart ? wave : 0;
+      k_at = (const char *)p.k + (seg.k0 + (int64_t)to_fetch * KEYS) * p.k_row + kv * p.k_head;
+      v_at = (const char *)p.v + (seg.k0 + (int64_t)to_fetch * KEYS) * p.v_row + kv * p.v_head;
+    }
+  }
+  through_tiles<F>(0, end, wave, L0, L1, fetch, [&](int t, const lds_char *here) { tile_of(t, here, std::false_type()); });
   if (there && h == 0 && (!F::kApart || wave == 0)) p.delta[head * p.nq + at] = delta;
   T *out = (T *)p.gq + (at * p.heads + head) * p.dim;
   if constexpr (F::kApart) {
     static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
     Gathered<WIDE, F::kWaves> all;
-    all.leave((lds_char *)stage0 + region, dq, 1.0f);
+    all.leave(L0, dq, 1.0f);
     __syncthreads();
     all.take((const lds_char *)stage0, kStage, wave);
     all.store(out, there, p.dim, wave, p.scale);

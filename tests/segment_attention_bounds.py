@@ -59,8 +59,12 @@ def reference(q, k, v, q_len, k_len, causal, scale=None, grad=None, q_first=0, k
             gi = g[a:a + n, h]
             dp, delta = gi @ z.t(), (gi * o).sum(dim=1, keepdim=True)
             ds = p * (dp - delta)
+            if dtype == torch.bfloat16:          # delta is the sum of the weighed dp, whose products are off as the scores' are
+                delta_off = ((e + (m + 8) * U) * p * dp.abs() + (d + 8) * U * p * (gi.abs() @ z.abs().t())).sum(dim=1, keepdim=True)
+            else:                                # ... of the products with out
+                delta_off = (gi.abs() * out_tol[a:a + n, h]).sum(dim=1, keepdim=True)
             off = p * (e * (dp.abs() + delta.abs()) + (d + 8) * U * (gi.abs() @ z.abs().t()) + (d + 8) * U * (gi.abs() * o.abs()).sum(1, keepdim=True)
-                       + (gi.abs() * out_tol[a:a + n, h]).sum(dim=1, keepdim=True)) + 4 * U * ds.abs()
+                       + delta_off) + 4 * U * ds.abs()
             off = off + operand * (ds.abs() + off)
             terms = abs(scale) * (ds.abs() @ y.abs())
             grads[0][a:a + n, h] += scale * (ds @ y)
