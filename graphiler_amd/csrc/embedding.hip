@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kBlock) void embedding_runs_kernel(const T *__restr
   }
 }
 
-// The runs of long rows added up: 512 rows of the table a workgroup, gridDim.x apart (ids named often tend to lie side by side),
+// The runs of long rows added up: up to 512 rows of the table a workgroup, gridDim.x apart (ids named often tend to lie side by side),
 // 64 columns blockIdx.y; eight wavefronts take equal shares of a row's runs.
 template <typename T>
 __global__ __launch_bounds__(8 * kWave) void embedding_join_kernel(const float *__restrict__ parts,
@@ -302,8 +302,11 @@ int sum_rows(const void *gy, const Plan &p, char *ws, void *grad, int64_t n_ids,
   hipLaunchKernelGGL((embedding_runs_kernel<T, LANES>), dim3((unsigned)runs, (unsigned)wide), dim3(kBlock), 0, s, (const T *)gy,
                      (const int64_t *)(ws + p.keys), pointer, places, parts, n_ids, n_table, cols);
   if (int rc = launch_status()) return rc;
-  hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)((n_table + 8 * kWave - 1) / (8 * kWave)), (unsigned)((cols + kWave - 1) / kWave)),
-                     dim3(8 * kWave), 0, s, parts, pointer, (T *)grad, n_table, cols, scale);
+  // a small table's long rows in as many workgroups as there are (435 rows, nearly all long, 311 -> 8 us)
+  const int64_t across = (cols + kWave - 1) / kWave, some = n_table < 2048 / across ? n_table : 2048 / across;
+  const int64_t least = (n_table + 8 * kWave - 1) / (8 * kWave);
+  hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)(some > least ? some : least), (unsigned)across), dim3(8 * kWave), 0, s,
+                     parts, pointer, (T *)grad, n_table, cols, scale);
   return launch_status();
 }
 
