@@ -201,8 +201,9 @@ __global__ __launch_bounds__(8 * kWave) void embedding_join_kernel(const float *
 }
 
 // Few places: a workgroup for each row of the table looks through all of them, a quarter by each wavefront in its turn, 512
-// columns blockIdx.y.  One launch in the place of the sort's and the sums' eleven (us, 512 places of 64 columns, 300 rows 47 -> 9).
-constexpr int64_t kFewPlaces = 1024, kFewTable = 8192;
+// columns blockIdx.y.  One launch in the place of the sort's and the sums' eleven (us, 512 places of 64 columns, 300 rows 47 -> 9;
+// 88 of 417, 26,498 rows 41 -> 14; 1024 of 512, 16,000 39 -> 16, 60,000 50 -> 49).
+constexpr int64_t kFewPlaces = 1024, kFewTable = 65536;
 template <typename T>
 __global__ __launch_bounds__(kBlock) void embedding_few_kernel(const T *__restrict__ gy, const void *__restrict__ ids, int bits,
                                                                T *__restrict__ grad, int n_ids, int64_t cols, float scale) {

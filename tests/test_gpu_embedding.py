@@ -54,7 +54,7 @@ def test_widths(cols, dtype):
 
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("bits", [64, 32])
-@pytest.mark.parametrize("n,rows", [(1, 1), (1, 1000), (127, 1), (128, 1), (129, 1), (1000, 1), (1024, 8192), (1025, 300), (1024, 8193), (600, 40), (5000, 2), (257, 65), (20000, 7),
+@pytest.mark.parametrize("n,rows", [(1, 1), (1, 1000), (127, 1), (128, 1), (129, 1), (1000, 1), (1024, 8192), (1000, 65536), (1024, 65537), (1025, 300), (1024, 8193), (600, 40), (5000, 2), (257, 65), (20000, 7),
                                     (30000, 3000), (3000, 30000), (100000, 64)])
 def test_counts(n, rows, bits, dtype):
     check(n, rows, 48, dtype, bits)
