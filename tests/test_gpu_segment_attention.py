@@ -98,3 +98,19 @@ def test_enough_workgroups_for_tiles_that_wavefronts_share(dim, causal, dtype):
     check([200, 130, 70, 257], None, 64, 64, dim, causal, dtype)
     check([100, 130, 70, 64], [300, 90, 129, 10], 128, 64, dim, causal, dtype, backward=dim < 128)
     check([40, 64, 65, 3, 0, 33, 32] * 10, None, 4, 2, dim, causal, dtype)
+
+
+@pytest.mark.parametrize("q_len,k_len,causal", [([182, 61, 40, 7], None, True), ([116, 20], None, False), ([3, 2, 3], [179, 64, 20], False),
+                                                ([300, 500], None, True)])
+@pytest.mark.parametrize("dim", [16, 32])
+def test_grad_q_of_narrow_heads_is_off_by_its_own_rounding(q_len, k_len, causal, dim):
+    # With few keys that count, a delta from the rounded result or ds of 8 bits would add to it: here delta is a sum in 32 bits and ds
+    # has 16, 2^-8 of what the result's rounding is off by.  A tenth is for the 32-bit sums and the weights' exponentials.
+    keys = k_len or q_len
+    q, k, v = made(sum(q_len), 4, dim, torch.bfloat16, 5, 1.8), made(sum(keys), 2, dim, torch.bfloat16, 6), made(sum(keys), 2, dim, torch.bfloat16, 7)
+    grad = made(sum(q_len), 4, dim, torch.bfloat16, 8)
+    qp, kp = pointer(q_len), pointer(k_len) if k_len else None
+    want = reference(q, k, v, q_len, keys, causal, None, grad)[3][0]
+    out, lse = ops.segment_attention(q, k, v, qp, kp, causal=causal, return_lse=True)
+    got = ops.segment_attention_backward(grad, q, k, v, out, lse, qp, kp, causal=causal)[0]
+    assert (got.double() - want).norm() <= 1.1 * (want.bfloat16().double() - want).norm()
