@@ -80,6 +80,11 @@ struct SlopeEpi : Stored<bf16_t> {
     floatx4 t = four_at(gy, M, p.rows, row, col, whole);
 #pragma unroll
     for (int r = 0; r < 4; ++r) t[r] *= gate_slope(ACT, z[r]);
+    // Columns behind the last are operands too: 0 whatever the slope there, which is NaN where x has an infinity.
+    if (col + 4 > M) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[r] = col + r < M ? t[r] : 0.0f;
+    }
     if constexpr (kPieces == 1) o[0] = pack(t);
     else cut_pieces(t, o[0], o[1], o[2]);
   }
