@@ -390,6 +390,34 @@ __device__ __forceinline__ void add_not_finite(const lds_char *t, int r, bool co
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// NaN in the results of columns 32 b ... of `t` that are not finite in a row with a 1 in `rows` (0 in the others): what such a value
+// weighed with 0, or with what is not finite either, adds.  Counted by the products themselves, a tile of columns at a time.
+template <typename T, int WIDE>
+__device__ __forceinline__ void spoil_columns(const lds_char *t, int col_at, int b, const floatx16 &rows,
+                                              floatx16 (&acc)[Rows<T, WIDE>::kCols]) {
+  typedef Rows<T, WIDE> R;
+#pragma unroll
+  for (int d = 0; d < R::kCols; ++d) {
+    floatx16 n;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) n[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R::kParts; ++i) {
+      uintx4 v = R::col(t, col_at, b, i, d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t hi = (v[j] & 0x7f800000u) == 0x7f800000u ? 0x3f800000u : 0u;
+        v[j] = sizeof(T) == 4 ? hi : hi | ((v[j] & 0x7f80u) == 0x7f80u ? 0x3f80u : 0u);
+      }
+      n = mma_piece<T>(v, operand_of<T>(rows, i), n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = n[r] > 0.0f ? NAN : acc[d][r];
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // The other half's value.
 __device__ __forceinline__ float other_half(float v) {
   return __shfl_xor(v, 32);

@@ -157,11 +157,20 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
       s[r] = !kEdge || result_row(r) < seen - key0 - 4 * h ? ds : 0.0f;
       if constexpr (kWeigh) weighed += s[r];
     }
-    // A key that is not finite has scores that are not, which is what reaches the queries that see it.
     // A query's ds add up to nothing, so what keys have in common cancels and the rounding of ds as operands, whose errors do not
     // cancel, counts for more than its half step: most where heads are narrow or keys few, and there they keep 16 bits.
     constexpr bool kLeft = sizeof(T) == 2 && (WIDE == 32 || F::kWaves == 1);
-    if constexpr (!kWeigh) add_columns<T, WIDE, kEdge, kLeft>(keys, col_at, b, s, dq);
+    bool found = false;
+    if constexpr (!kWeigh) found = add_columns<T, WIDE, kEdge, kLeft>(keys, col_at, b, s, dq);
+    if constexpr (kEdge && !kWeigh) {
+      // Such a key's ds is 0 (of a score of -inf) or not finite: its columns that are not finite become NaN for the queries that see it,
+      // as they do by themselves in a tile that all see.
+      if (__ballot(found)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = result_row(r) < seen - key0 - 4 * h ? 1.0f : 0.0f;
+        spoil_columns<T, WIDE>(keys, col_at, b, s, dq);
+      }
+    }
   };
   auto tile_of = [&](int t, const lds_char *here, auto weigh) {
 #pragma unroll
@@ -338,7 +347,15 @@ __device__ __forceinline__ void segment_attn_dkv(const Backward &p) {
           add_not_finite<T, WIDE>(grads, b * 32 + r, query0 + r >= by && query0 + r < seg.q_len, dv);
       }
     }
-    if constexpr (kDk) add_columns<T, WIDE, kEdge>(queries, col_at, b, dp, dk);
+    if constexpr (kDk) found = add_columns<T, WIDE, kEdge>(queries, col_at, b, dp, dk);
+    if constexpr (kEdge && kDk) {
+      if (__ballot(found)) {             // as for dq: the ds of a query that is not finite is 0 or not finite
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          dp[r] = result_row(r) >= by - query0 - 4 * h && result_row(r) < seg.q_len - query0 - 4 * h ? 1.0f : 0.0f;
+        spoil_columns<T, WIDE>(queries, col_at, b, dp, dk);
+      }
+    }
   };
   Place used(F::kApart ? wave : 0, tiles);
   auto use = [&](int, const lds_char *here) {
