@@ -52,6 +52,8 @@ struct Running {
   __device__ __forceinline__ void tile(const lds_char *keys, const lds_char *values, int row_at, int col_at,
                                        const uintx4 (&q)[R::kSteps], float c, int seen) {
     constexpr int kB = KEYS / 32;
+    // 128 columns: or the 16 addresses that these give are kept over all tiles, which single wavefronts have no registers for
+    if constexpr (WIDE > 64 && KEYS == 32) asm volatile("" : "+v"(row_at), "+v"(col_at));
     const int h = (threadIdx.x >> 5) & 1;
     floatx16 s[kB];
     __builtin_amdgcn_s_setprio(1);       // products first: the other wavefront of the SIMD has its exponentials meanwhile
@@ -298,7 +300,7 @@ int launch(Forward p, hipStream_t s) {
 template <typename T, int WIDE>
 int forward(const Forward &p, hipStream_t s) {
   constexpr bool kDeepRows = WIDE * sizeof(T) > 256;         // 512 bytes: tiles of 32 of them, or one at a time
-  if (p.cutting == kSingle) return launch<T, WIDE, Form<1, 64, 1, false>>(p, s);
+  if (p.cutting == kSingle) return launch<T, WIDE, Form<1, single_deep(WIDE), 1, false>>(p, s);
   if (p.cutting == kApart) return launch<T, WIDE, Form<4, 32, kDeepRows ? 1 : 2, true>>(p, s);
   return launch<T, WIDE, Form<4, 64, 2, false>>(p, s);
 }

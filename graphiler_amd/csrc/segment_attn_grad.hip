@@ -38,22 +38,25 @@ __device__ __forceinline__ bool add_columns(const lds_char *t, int col_at, int b
                                             floatx16 (&acc)[Rows<T, WIDE>::kCols]) {
   typedef Rows<T, WIDE> R;
   bool found = false;
+  uintx4 o[R::kParts], left[R::kParts];
 #pragma unroll
   for (int i = 0; i < R::kParts; ++i) {
-    const uintx4 o = operand_of<T>(w, i);
-    uintx4 left;
+    o[i] = operand_of<T>(w, i);
     if constexpr (LEFT)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) left[j] = pack_bf16(w[8 * i + 2 * j] - bf16_lo(o[j]), w[8 * i + 2 * j + 1] - bf16_hi(o[j]));
+      for (int j = 0; j < 4; ++j) left[i][j] = pack_bf16(w[8 * i + 2 * j] - bf16_lo(o[i][j]), w[8 * i + 2 * j + 1] - bf16_hi(o[i][j]));
+  }
+  if constexpr (LEFT && WIDE > 64) __builtin_amdgcn_sched_barrier(0);        // and its registers are free
+#pragma unroll
+  for (int i = 0; i < R::kParts; ++i)
 #pragma unroll
     for (int d = 0; d < R::kCols; ++d) {
       uintx4 v = R::col(t, col_at, b, i, d);
       if constexpr (CLEAN) found |= cleaned<T>(v);
-      acc[d] = mma_piece<T>(v, o, acc[d]);
-      if constexpr (LEFT) acc[d] = mma_piece<T>(v, left, acc[d]);
+      acc[d] = mma_piece<T>(v, o[i], acc[d]);
+      if constexpr (LEFT) acc[d] = mma_piece<T>(v, left[i], acc[d]);
       if constexpr (CLEAN) __builtin_amdgcn_sched_barrier(0);          // the rare tiles are not to decide what registers it takes
     }
-  }
   return found;
 }
 
@@ -76,7 +79,6 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
   const int kv = head / p.group;
   const int first = seg.tile * F::kRows + (F::kApart ? 0 : wave * 32), query = first + n;
   const bool there = query < seg.q_len;
-  const int64_t at = seg.q0 + query;
 
   uintx4 q[R::kSteps], g[R::kSteps];
   const int64_t row0 = seg.q0 + first;
@@ -100,7 +102,7 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
       }
     delta += other_half(delta);
   }
-  float lse = there ? p.lse[head * p.nq + at] * kLog2e : 0.0f;
+  float lse = there ? p.lse[head * p.nq + seg.q0 + query] * kLog2e : 0.0f;
   if (lse == -INFINITY) lse = INFINITY;                      // a query that sees nothing: p = 0
   const float c = p.scale * kLog2e;
 
@@ -142,14 +144,17 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
   // WEIGH: only onto that sum.
   auto block = [&](const lds_char *keys, const lds_char *values, int b, int key0, auto edge, auto weigh) {
     constexpr bool kEdge = decltype(edge)::value, kWeigh = decltype(weigh)::value;
+    // 128 columns: the 16 addresses that these two give are reckoned in every block, where registers for them are
+    int at_row = row_at, at_col = col_at;
+    if constexpr (WIDE > 64) asm volatile("" : "+v"(at_row), "+v"(at_col));
     floatx16 s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < R::kSteps; ++i) s = mma_piece<T>(R::row(keys, row_at, b, i), q[i], s);
+    for (int i = 0; i < R::kSteps; ++i) s = mma_piece<T>(R::row(keys, at_row, b, i), q[i], s);
     if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < R::kSteps; ++i) dp = mma_piece<T>(R::row(values, row_at, b, i), g[i], dp);
+    for (int i = 0; i < R::kSteps; ++i) dp = mma_piece<T>(R::row(values, at_row, b, i), g[i], dp);
     if constexpr (kEdge) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -161,14 +166,14 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
     // cancel, counts for more than its half step: most where heads are narrow or keys few, and there they keep 16 bits.
     constexpr bool kLeft = sizeof(T) == 2 && (WIDE == 32 || F::kWaves == 1);
     bool found = false;
-    if constexpr (!kWeigh) found = add_columns<T, WIDE, kEdge, kLeft>(keys, col_at, b, s, dq);
+    if constexpr (!kWeigh) found = add_columns<T, WIDE, kEdge, kLeft>(keys, at_col, b, s, dq);
     if constexpr (kEdge && !kWeigh) {
       // Such a key's ds is 0 (of a score of -inf) or not finite: its columns that are not finite become NaN for the queries that see it,
       // as they do by themselves in a tile that all see.
       if (__ballot(found)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = result_row(r) < seen - key0 - 4 * h ? 1.0f : 0.0f;
-        spoil_columns<T, WIDE>(keys, col_at, b, s, dq);
+        spoil_columns<T, WIDE>(keys, at_col, b, s, dq);
       }
     }
   };
@@ -204,7 +209,13 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
     }
   }
   through_tiles<F>(0, end, wave, L0, L1, fetch, [&](int t, const lds_char *here) { tile_of(t, here, std::false_type()); });
-  if (there && h == 0 && (!F::kApart || wave == 0)) p.delta[head * p.nq + at] = delta;
+  // Whose row this is, reckoned again: over the loops it would take registers that 128 columns have not.
+  int lane_again = 0;
+  asm volatile("" : "+v"(lane_again));
+  lane_again = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, lane_again));
+  const int64_t at = seg.q0 + first + (lane_again & 31);
+  const bool own = first + (lane_again & 31) < seg.q_len;
+  if (own && lane_again < 32 && (!F::kApart || wave == 0)) p.delta[head * p.nq + at] = delta;
   T *out = (T *)p.gq + (at * p.heads + head) * p.dim;
   if constexpr (F::kApart) {
     static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
@@ -212,9 +223,9 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
     all.leave(L0, dq, 1.0f);
     __syncthreads();
     all.take((const lds_char *)stage0, kStage, wave);
-    all.store(out, there, p.dim, wave, p.scale);
+    all.store(out, own, p.dim, wave, p.scale);
   } else {
-    store_row<T, R::kCols>(out, there, p.dim, dq, p.scale);
+    store_row<T, R::kCols>(out, own, p.dim, dq, p.scale);
   }
 }
 template <typename T, int WIDE, typename F>
@@ -458,7 +469,7 @@ int launch_dkv(Backward p, hipStream_t s) {
 template <typename T, int WIDE>
 int backward(const Backward &p, hipStream_t s) {
   constexpr bool kDeepRows = WIDE * sizeof(T) > 256;         // 512 bytes: tiles of 32 of them, or one at a time
-  typedef Form<1, 64, 1, false> Single;
+  typedef Form<1, single_deep(WIDE), 1, false> Single;
   typedef Form<4, 32, kDeepRows ? 1 : 2, true> Apart;
   typedef Form<4, kDeepRows ? 32 : 64, 2, false> Shared;
   if (p.nq > 0) {
