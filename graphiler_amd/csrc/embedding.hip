@@ -324,11 +324,18 @@ int check_embedding(const void *a, const void *ids, int idx_bits, const void *ou
 }
 
 // Lanes a row: as many as its columns need, a wavefront's at most.
-#define GA_BY_COLS(call, T, ...)                                     \
-  (cols <= 8 * kVec    ? call<T, 8>(__VA_ARGS__)                     \
-   : cols <= 16 * kVec ? call<T, 16>(__VA_ARGS__)                    \
-   : cols <= 32 * kVec ? call<T, 32>(__VA_ARGS__)                    \
-                       : call<T, 64>(__VA_ARGS__))
+int lanes_of(int64_t cols) { return cols <= 8 * kVec ? 8 : cols <= 16 * kVec ? 16 : cols <= 32 * kVec ? 32 : 64; }
+#define GA_BY_COLS(call, T, ...)                          \
+  (lanes_of(cols) == 8    ? call<T, 8>(__VA_ARGS__)       \
+   : lanes_of(cols) == 16 ? call<T, 16>(__VA_ARGS__)      \
+   : lanes_of(cols) == 32 ? call<T, 32>(__VA_ARGS__)      \
+                          : call<T, 64>(__VA_ARGS__))
+
+// What the launches of a gradient hold: a workgroup for every run of the ids, and for as many rows of the table as it has groups of lanes.
+bool holds(int64_t n_ids, int64_t n_table, int64_t cols) {
+  constexpr int64_t blocks = kMostLanes / kBlock;
+  return n_ids <= blocks * kRun && n_table <= blocks * (kBlock / lanes_of(cols));
+}
 
 }  // namespace
 }  // namespace ga
@@ -347,7 +354,7 @@ int ga_embedding(const void *table, const void *ids, int idx_bits, void *y, int6
 }
 
 size_t ga_embedding_backward_workspace_bytes(int64_t n_ids, int64_t n_table, int64_t cols) {
-  if (n_ids <= 0 || n_table <= 0 || cols <= 0 || n_ids > 0x7ffffffe || n_table > 0x7ffffffd) return 0;
+  if (n_ids <= 0 || n_table <= 0 || cols <= 0 || !ga::holds(n_ids, n_table, cols)) return 0;
   return ga::few(n_ids, n_table) ? 0 : ga::plan_of(n_ids, n_table, cols).bytes;
 }
 
@@ -355,10 +362,9 @@ int ga_embedding_backward(const void *grad_y, const void *ids, int idx_bits, voi
                           int64_t cols, float scale, int dtype, void *workspace, size_t workspace_bytes, ga_stream_t stream) {
   using namespace ga;
   if (int rc = check_embedding(grad_y, ids, idx_bits, grad_table, n_ids, n_table, cols, dtype, n_table > 0)) return rc;
-  if (n_ids > 0x7ffffffe || n_table > 0x7ffffffd) return GA_EUNSUPPORTED;
+  if (!holds(n_ids, n_table, cols)) return GA_EUNSUPPORTED;
   if (n_table == 0) return GA_OK;
   if (n_ids > 0 && !grad_y) return GA_EINVAL;
-  if (n_table > kMostLanes / kBlock * 4 || (cols + 63) / 64 > 65535) return GA_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
   if (n_ids == 0) {
     const int64_t n = n_table * cols * (dtype == GA_F32 ? 4 : 2);

@@ -917,7 +917,8 @@ int ga_linear_act_backward(const void *grad_y, const void *x, const void *weight
 
 /*
  * Embedding rows: y[i] = scale * table[ids[i]], zeros for an id outside [0, n_table).  table (n_table, cols) and y (n_ids, cols)
- * of `dtype`, ids int64 (idx_bits 64) or int32 (idx_bits 32); the product is rounded once.
+ * of `dtype`, ids int64 (idx_bits 64) or int32 (idx_bits 32); the product is rounded once.  GA_EUNSUPPORTED when n_ids exceeds
+ * 2^31 - 128 (up to 64 columns), 2^30 - 64 (up to 128), 2^29 - 32 (up to 256) or 2^28 - 16, or cols 2^20.
  */
 int ga_embedding(const void *table, const void *ids, int idx_bits, void *y, int64_t n_ids, int64_t n_table, int64_t cols,
                  float scale, int dtype, ga_stream_t stream);
@@ -925,7 +926,8 @@ int ga_embedding(const void *table, const void *ids, int idx_bits, void *y, int6
 /*
  * The table's gradient: grad_table[v] = scale * sum of grad_y[i] over the i with ids[i] = v, in fp32 in the order of the i
  * (inside runs whose bounds depend on the ids alone), rounded once; zeros for rows that no id names.  Ids outside the table
- * give nothing.  workspace: 256-byte aligned.  GA_EUNSUPPORTED when n_ids or n_table exceeds 2^31 - 2.
+ * give nothing.  workspace: 256-byte aligned.  GA_EUNSUPPORTED when n_ids exceeds 2^30 - 64 or n_table 2^29 - 32 (up to 64
+ * columns), 2^28 - 16 (up to 128), 2^27 - 8 (up to 256) or 2^26 - 4, or cols 2^20.
  */
 size_t ga_embedding_backward_workspace_bytes(int64_t n_ids, int64_t n_table, int64_t cols);
 int ga_embedding_backward(const void *grad_y, const void *ids, int idx_bits, void *grad_table, int64_t n_ids, int64_t n_table,
