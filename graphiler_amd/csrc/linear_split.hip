@@ -217,18 +217,25 @@ int launch(const Split &p, hipStream_t s) {
 }
 template <int WAVES>
 int launch(const Split &p, hipStream_t s) {
-  // a step of a workgroup takes TM parts and one more, whatever its rows
+  // A step of a workgroup takes TM parts and one more, whatever its rows.  By the LDS that they take 256 workgroups of eight wavefronts run
+  // at once; of four, 512 of up to two parts but 256 of three or four, which have 2 / 3 or 1 / 2 of the tiles of two in half of the places and
+  // take 4 / 3 or 5 / 3 of their time: never the least.
+  constexpr int kMost = WAVES == 8 ? 4 : 2;
+  constexpr int64_t kAtOnce = WAVES == 8 ? 256 : 512;
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int tm = 1; tm <= 4; ++tm) {
-    const int64_t at_once = 256 * (WAVES == 8 ? 1 : tm <= 2 ? 2 : 1);      // by the LDS that they take
-    const int64_t t = (tiles_of(p.rows, p.M, 32 * tm, 32 * WAVES) + at_once - 1) / at_once * (tm + 1);
+  for (int tm = 1; tm <= kMost; ++tm) {
+    const int64_t t = (tiles_of(p.rows, p.M, 32 * tm, 32 * WAVES) + kAtOnce - 1) / kAtOnce * (tm + 1);
     if (t <= least) {
       least = t;
       best = tm;
     }
   }
-  return best == 1 ? launch<1, WAVES>(p, s) : best == 2 ? launch<2, WAVES>(p, s) : best == 3 ? launch<3, WAVES>(p, s) : launch<4, WAVES>(p, s);
+  if constexpr (WAVES == 8) {
+    if (best == 3) return launch<3, WAVES>(p, s);
+    if (best == 4) return launch<4, WAVES>(p, s);
+  }
+  return best == 1 ? launch<1, WAVES>(p, s) : launch<2, WAVES>(p, s);
 }
 
 }  // namespace
