@@ -21,6 +21,7 @@ GA_CLASSES_MIN_DEGREE = 16
 GA_ACT_NONE, GA_ACT_RELU, GA_ACT_ELU = 0, 1, 2
 GA_GATE_NONE, GA_GATE_SILU, GA_GATE_GELU, GA_GATE_RELU = -1, 0, 1, 2
 GA_F32, GA_BF16 = 0, 1
+GA_GRAD_Q, GA_GRAD_K, GA_GRAD_V = 1, 2, 4
 GA_COPY_U, GA_COPY_E, GA_U_MUL_E, GA_U_ADD_E, GA_U_SUB_E, GA_U_DIV_E = 0, 1, 2, 3, 4, 5
 GA_SDDMM_ADD, GA_SDDMM_SUB, GA_SDDMM_MUL, GA_SDDMM_DIV = 0, 1, 2, 3
 GA_SUM, GA_MAX, GA_MIN = 0, 1, 2
@@ -159,6 +160,9 @@ SIGNATURES = {
     "ga_segment_attention_backward": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
                                              _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int,
                                              ctypes.c_float, _int, _vp, _sz, _vp]),
+    "ga_segment_attention_gradients": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+                                              _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int,
+                                              ctypes.c_float, _int, _int, _vp, _sz, _vp]),
     "ga_linear_act_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
     "ga_linear_act": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _sz, _vp]),
     "ga_linear_act_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),

@@ -24,7 +24,7 @@ struct Backward : SegAttn {
   int64_t out_row, out_head, grad_row, grad_head;
   const float *lse;                      // (heads, nq)
   float *delta;                          // (heads, nq)
-  void *gq, *gk, *gv;                    // (rows, heads, dim), contiguous
+  void *gq, *gk, *gv;                    // (rows, heads, dim), contiguous; NULL: not wanted
   int64_t tiles;
   int parts;                             // of the heads that share keys, each its own sums of dk and dv
   float *part_sums;                      // (dk and dv, parts, nk, kv_heads, dim)
@@ -202,13 +202,13 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
       __syncthreads();
     }
     if (fabsf(weighed) < INFINITY) delta = weighed;          // what is not finite has results that are not either
-    if (end > kTurn) {
+    if (p.gq && end > kTurn) {
       to_fetch = F::kApart ? wave : 0;
       k_at = (const char *)p.k + (seg.k0 + (int64_t)to_fetch * KEYS) * p.k_row + kv * p.k_head;
       v_at = (const char *)p.v + (seg.k0 + (int64_t)to_fetch * KEYS) * p.v_row + kv * p.v_head;
     }
   }
-  through_tiles<F>(0, end, wave, L0, L1, fetch, [&](int t, const lds_char *here) { tile_of(t, here, std::false_type()); });
+  if (p.gq) through_tiles<F>(0, end, wave, L0, L1, fetch, [&](int t, const lds_char *here) { tile_of(t, here, std::false_type()); });
   // Whose row this is, reckoned again: over the loops it would take registers that 128 columns have not.
   int lane_again = 0;
   asm volatile("" : "+v"(lane_again));
@@ -216,6 +216,7 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
   const int64_t at = seg.q0 + first + (lane_again & 31);
   const bool own = first + (lane_again & 31) < seg.q_len;
   if (own && lane_again < 32 && (!F::kApart || wave == 0)) p.delta[head * p.nq + at] = delta;
+  if (!p.gq) return;                     // delta alone, for dk
   T *out = (T *)p.gq + (at * p.heads + head) * p.dim;
   if constexpr (F::kApart) {
     static_assert(kStage >= 32 * WIDE * 4, "a wavefront's results lie where its tiles were");
@@ -433,6 +434,7 @@ template <typename T>
 __global__ __launch_bounds__(kBlock) void segment_attn_parts_kernel(Backward p, int64_t values) {
   const float *from = p.part_sums + (int64_t)blockIdx.y * p.parts * values;
   T *to = (T *)(blockIdx.y ? p.gv : p.gk);
+  if (!to) return;
   for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < values; i += (int64_t)gridDim.x * kBlock) {
     float s = 0.0f;
     for (int k = 0; k < p.parts; ++k) s += from[k * values + i];
@@ -455,10 +457,12 @@ int launch_dkv(Backward p, hipStream_t s) {
   if (grid > kMostLanes / (F::kWaves * kWave)) return GA_EUNSUPPORTED;
   const dim3 blocks((unsigned)grid, (unsigned)p.parts), threads(F::kWaves * kWave);
   constexpr bool kTwice = WIDE > 64;
-  hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F, kTwice ? kGradK : kGradK | kGradV>), blocks, threads, 0, s, p);
-  if constexpr (kTwice) {
+  if (!kTwice && p.gk && p.gv) {
+    if constexpr (!kTwice) hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F, kGradK | kGradV>), blocks, threads, 0, s, p);
+  } else {
+    if (p.gk) hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F, kGradK>), blocks, threads, 0, s, p);
     if (int rc = launch_status()) return rc;
-    hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F, kGradV>), blocks, threads, 0, s, p);
+    if (p.gv) hipLaunchKernelGGL((segment_attn_dkv_kernel<T, WIDE, F, kGradV>), blocks, threads, 0, s, p);
   }
   if (int rc = launch_status()) return rc;
   if (p.parts == 1) return GA_OK;
@@ -472,13 +476,13 @@ int backward(const Backward &p, hipStream_t s) {
   typedef Form<1, single_deep(WIDE), 1, false> Single;
   typedef Form<4, 32, kDeepRows ? 1 : 2, true> Apart;
   typedef Form<4, kDeepRows ? 32 : 64, 2, false> Shared;
-  if (p.nq > 0) {
+  if (p.nq > 0 && (p.gq || p.gk)) {      // dk takes delta of it
     const Cutting c = cutting_of(p.segments, p.nq, p.nk, p.heads);
     const int rc = c == kSingle ? launch_dq<T, WIDE, Single>(p, s) : c == kApart ? launch_dq<T, WIDE, Apart>(p, s)
                                                                                  : launch_dq<T, WIDE, Shared>(p, s);
     if (rc) return rc;
   }
-  if (p.nk > 0) {
+  if (p.nk > 0 && (p.gk || p.gv)) {
     const Cutting c = cutting_of(p.segments, p.nk, p.nq * p.group, p.heads / p.group);
     return c == kSingle ? launch_dkv<T, WIDE, Single>(p, s) : c == kApart ? launch_dkv<T, WIDE, Apart>(p, s)
                                                                           : launch_dkv<T, WIDE, Shared>(p, s);
@@ -507,18 +511,23 @@ size_t ga_segment_attention_backward_workspace_bytes(int64_t n_segments, int64_t
   return (size_t)n;
 }
 
-int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q_row, int64_t q_head, const void *k,
-                                  int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
-                                  const float *lse, const int64_t *q_pointer, const int64_t *k_pointer, int64_t n_segments,
-                                  void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
-                                  int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
-                                  size_t workspace_bytes, ga_stream_t stream) {
+int ga_segment_attention_gradients(const void *grad_out, const void *q, int64_t q_row, int64_t q_head, const void *k,
+                                   int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
+                                   const float *lse, const int64_t *q_pointer, const int64_t *k_pointer, int64_t n_segments,
+                                   void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
+                                   int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, int wanted,
+                                   void *workspace, size_t workspace_bytes, ga_stream_t stream) {
   using namespace ga;
   Backward p{};
   if (int rc = segment_attn_check(p, q, k, v, q_row, q_head, k_row, k_head, v_row, v_head, q_pointer, k_pointer, n_segments,
                                   n_queries, n_keys, heads, kv_heads, dim, causal, scale, dtype))
     return rc;
-  if ((n_queries > 0 && (!grad_out || !out || !lse || !grad_q)) || (n_keys > 0 && (!grad_k || !grad_v))) return GA_EINVAL;
+  if (!wanted || (wanted & ~(GA_GRAD_Q | GA_GRAD_K | GA_GRAD_V))) return GA_EINVAL;
+  if (!(wanted & GA_GRAD_Q)) grad_q = nullptr;
+  if (!(wanted & GA_GRAD_K)) grad_k = nullptr;
+  if (!(wanted & GA_GRAD_V)) grad_v = nullptr;
+  if (n_queries > 0 && (!grad_out || !out || !lse || ((wanted & GA_GRAD_Q) && !grad_q))) return GA_EINVAL;
+  if (n_keys > 0 && (((wanted & GA_GRAD_K) && !grad_k) || ((wanted & GA_GRAD_V) && !grad_v))) return GA_EINVAL;
   const int64_t e = dtype == GA_F32 ? 4 : 2;
   if (!aligned(grad_out, e) || !aligned(out, e) || !aligned(lse, 4) || !aligned(grad_q, e) || !aligned(grad_k, e) ||
       !aligned(grad_v, e))
@@ -566,6 +575,17 @@ int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q
     p.k_row = p.v_row = head * kv_heads;
   }
   return dtype == GA_F32 ? backward<float>(p, s) : backward<bf16_t>(p, s);
+}
+
+int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q_row, int64_t q_head, const void *k,
+                                  int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
+                                  const float *lse, const int64_t *q_pointer, const int64_t *k_pointer, int64_t n_segments,
+                                  void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
+                                  int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
+                                  size_t workspace_bytes, ga_stream_t stream) {
+  return ga_segment_attention_gradients(grad_out, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, out, lse, q_pointer, k_pointer,
+                                        n_segments, grad_q, grad_k, grad_v, n_queries, n_keys, heads, kv_heads, dim, causal, scale,
+                                        dtype, GA_GRAD_Q | GA_GRAD_K | GA_GRAD_V, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -1817,10 +1817,11 @@ class _SegmentAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out, grad_lse=None):
         _not_recorded("segment_attention")
-        if grad_out is None:
+        wanted = ctx.needs_input_grad[:3]
+        if grad_out is None or not any(wanted):
             return (None,) * 7
         q, k, v, out, lse, q_pointer, k_pointer = ctx.saved_tensors
-        return (*segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, ctx.causal, ctx.scale),
+        return (*_segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, ctx.causal, ctx.scale, wanted),
                 None, None, None, None)
 
 
@@ -1854,11 +1855,7 @@ def segment_attention(q, k, v, q_pointer, k_pointer=None, causal: bool = False, 
     return _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, return_lse)
 
 
-def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer=None, causal: bool = False,
-                               scale=None):
-    """Gradients of :func:`segment_attention`: (of q, of k, of v), contiguous, from what it returned with
-    ``return_lse``.  Rows in no segment get zeros.  The results have no gradients of their own."""
-    _check_seen("segment_attention_backward", grad_out, q, k, v, out)
+def _segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, causal, scale, wanted):
     dt, k_pointer, scale, sizes = _attention_args(q, k, v, q_pointer, k_pointer, scale)
     _check_like(out, "out", q.shape, q)
     _check_input(lse, "lse")
@@ -1869,13 +1866,23 @@ def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer
     if grad_out.shape != q.shape:
         raise RuntimeError("grad_out must have q's shape")
     q, k, v, grad_out = _in_pieces(q), _in_pieces(k), _in_pieces(v), _in_pieces(grad_out)
-    gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((q, k, v), wanted)]
+    which = sum(bit for bit, w in zip((capi.GA_GRAD_Q, capi.GA_GRAD_K, capi.GA_GRAD_V), wanted) if w)
     n = capi.load().ga_segment_attention_backward_workspace_bytes(*sizes, dt)
     ws = _scratch(n, q.device)
-    _launch("ga_segment_attention_backward", q.get_device(), grad_out.data_ptr(), *_placed(q), *_placed(k), *_placed(v),
-            out.data_ptr(), lse.data_ptr(), q_pointer.data_ptr(), k_pointer.data_ptr(), sizes[0], gq.data_ptr(),
-            gk.data_ptr(), gv.data_ptr(), *sizes[1:], bool(causal), scale, dt, _ptr(ws), n)
-    return gq, gk, gv
+    _launch("ga_segment_attention_gradients", q.get_device(), grad_out.data_ptr(), *_placed(q), *_placed(k), *_placed(v),
+            out.data_ptr(), lse.data_ptr(), q_pointer.data_ptr(), k_pointer.data_ptr(), sizes[0], *(_ptr(g) for g in grads),
+            *sizes[1:], bool(causal), scale, dt, which, _ptr(ws), n)
+    return tuple(grads)
+
+
+def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer=None, causal: bool = False,
+                               scale=None):
+    """Gradients of :func:`segment_attention`: (of q, of k, of v), contiguous, from what it returned with
+    ``return_lse``.  Rows in no segment get zeros.  The results have no gradients of their own.  (Through autograd only
+    those are formed that a tensor wants.)"""
+    _check_seen("segment_attention_backward", grad_out, q, k, v, out)
+    return _segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, causal, scale, (True, True, True))
 
 
 # ------------------------------- what is around that attention: projections and embedding rows ----
