@@ -160,7 +160,7 @@ SIGNATURES = {
     "ga_segment_attention_backward": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
                                              _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int,
                                              ctypes.c_float, _int, _vp, _sz, _vp]),
-    "ga_segment_attention_gradients": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+    "ga_segment_attention_gradients": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
                                               _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int,
                                               ctypes.c_float, _int, _int, _vp, _sz, _vp]),
     "ga_linear_act_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),

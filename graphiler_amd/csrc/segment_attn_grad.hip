@@ -3,6 +3,8 @@
 //   p_ij = exp(s_ij - lse_i), delta_i = <do_i, o_i> = sum_j p_ij <do_i, v_j>, ds_ij = p_ij (<do_i, v_j> - delta_i)
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i
 //
+// and, where the log-sum-exps have gradients dlse_i of their own, delta_i - dlse_i in delta_i's place: d lse_i / d s_ij = p_ij.
+//
 // Two kernels, each over 32 x 32 tiles that never leave the registers: one with 32 queries a wavefront over the keys (dq, and
 // delta on the way), one with 32 keys a wavefront over the queries of all heads that share them (dk and dv).  Both form the
 // scores again, seven products instead of the five of a single pass, which would have to add up dq from many workgroups in
@@ -23,6 +25,7 @@ struct Backward : SegAttn {
   const void *out, *grad;                // (nq, heads, dim), rows and heads as far apart as these say (bytes)
   int64_t out_row, out_head, grad_row, grad_head;
   const float *lse;                      // (heads, nq)
+  const float *grad_lse;                 // (heads, nq) or NULL: taken from delta, as d lse_i / d s_ij = p_ij
   float *delta;                          // (heads, nq)
   void *gq, *gk, *gv;                    // (rows, heads, dim), contiguous; NULL: not wanted
   int64_t tiles;
@@ -208,6 +211,7 @@ __device__ __forceinline__ void segment_attn_dq(const Backward &p) {
       v_at = (const char *)p.v + (seg.k0 + (int64_t)to_fetch * KEYS) * p.v_row + kv * p.v_head;
     }
   }
+  if (p.grad_lse) delta -= there ? p.grad_lse[head * p.nq + seg.q0 + query] : 0.0f;
   if (p.gq) through_tiles<F>(0, end, wave, L0, L1, fetch, [&](int t, const lds_char *here) { tile_of(t, here, std::false_type()); });
   // Whose row this is, reckoned again: over the loops it would take registers that 128 columns have not.
   int lane_again = 0;
@@ -511,8 +515,8 @@ size_t ga_segment_attention_backward_workspace_bytes(int64_t n_segments, int64_t
   return (size_t)n;
 }
 
-int ga_segment_attention_gradients(const void *grad_out, const void *q, int64_t q_row, int64_t q_head, const void *k,
-                                   int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
+int ga_segment_attention_gradients(const void *grad_out, const float *grad_lse, const void *q, int64_t q_row, int64_t q_head,
+                                   const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
                                    const float *lse, const int64_t *q_pointer, const int64_t *k_pointer, int64_t n_segments,
                                    void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
                                    int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, int wanted,
@@ -529,7 +533,7 @@ int ga_segment_attention_gradients(const void *grad_out, const void *q, int64_t 
   if (n_queries > 0 && (!grad_out || !out || !lse || ((wanted & GA_GRAD_Q) && !grad_q))) return GA_EINVAL;
   if (n_keys > 0 && (((wanted & GA_GRAD_K) && !grad_k) || ((wanted & GA_GRAD_V) && !grad_v))) return GA_EINVAL;
   const int64_t e = dtype == GA_F32 ? 4 : 2;
-  if (!aligned(grad_out, e) || !aligned(out, e) || !aligned(lse, 4) || !aligned(grad_q, e) || !aligned(grad_k, e) ||
+  if (!aligned(grad_out, e) || !aligned(grad_lse, 4) || !aligned(out, e) || !aligned(lse, 4) || !aligned(grad_q, e) || !aligned(grad_k, e) ||
       !aligned(grad_v, e))
     return GA_EALIGN;
   const bool whole = whole_rows(dim, dtype);
@@ -546,6 +550,7 @@ int ga_segment_attention_gradients(const void *grad_out, const void *q, int64_t 
   p.out_row = p.grad_row = heads * dim * e;
   p.out_whole = whole && aligned(out, 4);
   p.lse = lse;
+  p.grad_lse = grad_lse;
   p.delta = (float *)workspace;
   char *at = (char *)workspace + (n_queries * heads * 4 + 255) / 256 * 256;
   p.parts = parts_of_group(n_segments, n_keys, heads, kv_heads);
@@ -583,7 +588,7 @@ int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q
                                   void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
                                   int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
                                   size_t workspace_bytes, ga_stream_t stream) {
-  return ga_segment_attention_gradients(grad_out, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, out, lse, q_pointer, k_pointer,
+  return ga_segment_attention_gradients(grad_out, nullptr, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, out, lse, q_pointer, k_pointer,
                                         n_segments, grad_q, grad_k, grad_v, n_queries, n_keys, heads, kv_heads, dim, causal, scale,
                                         dtype, GA_GRAD_Q | GA_GRAD_K | GA_GRAD_V, workspace, workspace_bytes, stream);
 }

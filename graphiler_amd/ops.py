@@ -1809,7 +1809,6 @@ class _SegmentAttention(torch.autograd.Function):
         out, lse = _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, True)
         ctx.causal, ctx.scale = causal, scale
         ctx.save_for_backward(q, k, v, out, lse, q_pointer, k_pointer)
-        ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
 
@@ -1818,10 +1817,11 @@ class _SegmentAttention(torch.autograd.Function):
     def backward(ctx, grad_out, grad_lse=None):
         _not_recorded("segment_attention")
         wanted = ctx.needs_input_grad[:3]
-        if grad_out is None or not any(wanted):
+        if (grad_out is None and grad_lse is None) or not any(wanted):
             return (None,) * 7
         q, k, v, out, lse, q_pointer, k_pointer = ctx.saved_tensors
-        return (*_segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, ctx.causal, ctx.scale, wanted),
+        grad_out = torch.zeros_like(out) if grad_out is None else grad_out
+        return (*_segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, ctx.causal, ctx.scale, grad_lse, wanted),
                 None, None, None, None)
 
 
@@ -1847,20 +1847,27 @@ def segment_attention(q, k, v, q_pointer, k_pointer=None, causal: bool = False, 
     ``scale`` (1 / sqrt(dim)) multiplies the scores.  Returns (queries, heads, dim); with ``return_lse`` also the
     (heads, queries) fp32 logarithms of the sums of exponentials.  A query that sees no key gives zeros and
     -inf, as do rows in no segment.  float32 or bfloat16, dim up to 128; rows and heads may be strided (columns of one
-    projection), dim not.  Scores and sums are fp32; bf16 weights are rounded once as operands.  Differentiable in q, k
-    and v (backward mode)."""
+    projection), dim not.  Scores and sums are fp32; bf16 weights are rounded once as operands.  Both results are differentiable
+    in q, k and v (backward mode)."""
     if _wants_grad("segment_attention", q, k, v):
         got = _SegmentAttention.apply(q, k, v, q_pointer, q_pointer if k_pointer is None else k_pointer, bool(causal), scale)
         return got if return_lse else got[0]
     return _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, return_lse)
 
 
-def _segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, causal, scale, wanted):
+def _check_of_queries(t, name: str, q) -> None:
+    _check_input(t, name)
+    if t.dtype != torch.float32 or t.shape != (q.shape[1], q.shape[0]) or t.get_device() != q.get_device():
+        raise RuntimeError(f"{name} must be a (heads, queries) float32 tensor, as segment_attention returns lse")
+
+
+def _segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, causal, scale, grad_lse, wanted):
     dt, k_pointer, scale, sizes = _attention_args(q, k, v, q_pointer, k_pointer, scale)
     _check_like(out, "out", q.shape, q)
-    _check_input(lse, "lse")
-    if lse.dtype != torch.float32 or lse.shape != (q.shape[1], q.shape[0]) or lse.get_device() != q.get_device():
-        raise RuntimeError("lse must be the (heads, queries) float32 tensor that segment_attention returned")
+    _check_of_queries(lse, "lse", q)
+    if grad_lse is not None:
+        grad_lse = grad_lse.contiguous()
+        _check_of_queries(grad_lse, "grad_lse", q)
     grad_out = grad_out.contiguous()                     # a sum's gradient has no strides
     _rows_heads(grad_out, "grad_out", q.get_device(), q.dtype)
     if grad_out.shape != q.shape:
@@ -1870,19 +1877,19 @@ def _segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointe
     which = sum(bit for bit, w in zip((capi.GA_GRAD_Q, capi.GA_GRAD_K, capi.GA_GRAD_V), wanted) if w)
     n = capi.load().ga_segment_attention_backward_workspace_bytes(*sizes, dt)
     ws = _scratch(n, q.device)
-    _launch("ga_segment_attention_gradients", q.get_device(), grad_out.data_ptr(), *_placed(q), *_placed(k), *_placed(v),
+    _launch("ga_segment_attention_gradients", q.get_device(), grad_out.data_ptr(), _ptr(grad_lse), *_placed(q), *_placed(k), *_placed(v),
             out.data_ptr(), lse.data_ptr(), q_pointer.data_ptr(), k_pointer.data_ptr(), sizes[0], *(_ptr(g) for g in grads),
             *sizes[1:], bool(causal), scale, dt, which, _ptr(ws), n)
     return tuple(grads)
 
 
 def segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer=None, causal: bool = False,
-                               scale=None):
+                               scale=None, grad_lse=None):
     """Gradients of :func:`segment_attention`: (of q, of k, of v), contiguous, from what it returned with
-    ``return_lse``.  Rows in no segment get zeros.  The results have no gradients of their own.  (Through autograd only
+    ``return_lse``, and from the gradient of lse where it has one.  Rows in no segment get zeros.  The results have no gradients of their own.  (Through autograd only
     those are formed that a tensor wants.)"""
-    _check_seen("segment_attention_backward", grad_out, q, k, v, out)
-    return _segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, causal, scale, (True, True, True))
+    _check_seen("segment_attention_backward", grad_out, q, k, v, out, grad_lse)
+    return _segment_attention_backward(grad_out, q, k, v, out, lse, q_pointer, k_pointer, causal, scale, grad_lse, (True, True, True))
 
 
 # ------------------------------- what is around that attention: projections and embedding rows ----

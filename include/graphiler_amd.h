@@ -893,10 +893,11 @@ int ga_segment_attention_backward(const void *grad_out, const void *q, int64_t q
                                   int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, void *workspace,
                                   size_t workspace_bytes, ga_stream_t stream);
 /* The same with those of the gradients that `wanted` (an or of ga_grad) names; the others' pointers are not looked at.  That of v alone
- * takes no pass over the queries, those of k and v none for that of q. */
+ * takes no pass over the queries, those of k and v none for that of q.  grad_lse: (heads, n_queries) fp32, the gradients of the
+ * log-sum-exps, whose part in ds is p grad_lse[h, i]; or NULL for none. */
 enum ga_grad { GA_GRAD_Q = 1, GA_GRAD_K = 2, GA_GRAD_V = 4 };
-int ga_segment_attention_gradients(const void *grad_out, const void *q, int64_t q_row, int64_t q_head, const void *k,
-                                   int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
+int ga_segment_attention_gradients(const void *grad_out, const float *grad_lse, const void *q, int64_t q_row, int64_t q_head,
+                                   const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, const void *out,
                                    const float *lse, const int64_t *q_pointer, const int64_t *k_pointer, int64_t n_segments,
                                    void *grad_q, void *grad_k, void *grad_v, int64_t n_queries, int64_t n_keys, int64_t heads,
                                    int64_t kv_heads, int64_t dim, int causal, float scale, int dtype, int wanted,
