@@ -105,6 +105,9 @@ struct Form {
   static constexpr int kMovers = APART_ ? 1 : WAVES_;        // wavefronts that fetch a tile
 };
 
+// Shared, by one wavefront (short segments), or apart; which of them a call takes goes by what the host knows (cut_of, cutting_of).
+enum Cutting { kShared, kSingle, kApart };
+
 // Tiles of single wavefronts: 64 rows or, of 128 columns, 32, with which two wavefronts a SIMD keep what they have in registers (1024
 // segments of 34 rows, 8 heads, bf16, 64 -> 32: forward 131 -> 80 us, gradients 431 -> 339; fp32, 4 heads, 235 -> 117 and 752 -> 446).
 constexpr int single_deep(int wide) { return wide > 64 ? 32 : 64; }

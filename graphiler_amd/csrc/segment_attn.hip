@@ -27,7 +27,7 @@ struct Forward : SegAttn {
   int64_t out_row, out_head;             // values
   int64_t tiles;                         // per head
   int pack;                              // heads of a group whose rows are one tile's: 1 or group
-  int cutting;
+  Cutting cutting;
   int splits;                            // parts of the keys, each its own partial result
   float *parts;                          // (splits, nq, heads, dim) sums, then (splits, nq, heads, 2) maxima and sums
 };
@@ -287,8 +287,6 @@ __global__ __launch_bounds__(kBlock) void segment_attn_join_kernel(Forward p) {
   if (p.lse && lane == 0) p.lse[head * p.nq + query] = lse_of(from, sum);
 }
 
-enum Cutting { kShared, kSingle, kApart };
-
 template <typename T, int WIDE, typename F>
 int launch(Forward p, hipStream_t s) {
   p.tiles = segment_tiles(p.nq, p.pack, p.segments, F::kRows);
@@ -403,7 +401,7 @@ static bool pieces_aligned(const void *p, int64_t row, int64_t head) {
 
 namespace {
 // How a call is cut up, from what the host knows: how many rows and segments there are, not how long which segment is.
-struct Cut { int pack, cutting, splits; int64_t laid, parts; size_t bytes; };
+struct Cut { int pack; Cutting cutting; int splits; int64_t laid, parts; size_t bytes; };
 Cut cut_of(int64_t segments, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim, int dtype) {
   Cut c;
   const int64_t group = heads / kv_heads, some = segments > 0 ? segments : 1;

@@ -416,7 +416,6 @@ __global__ __launch_bounds__(F::kWaves *kWave, sizeof(T) == 2 && (WIDE < 128 || 
   segment_attn_dkv<T, WIDE, F, WHICH>(p);
 }
 
-enum Cutting { kShared, kSingle, kApart };
 // As cut_of() of the forward pass has it: by the rows of a segment on average and by how many workgroups of 128 rows there
 // are, `keys` being what a row goes through (bf16, all gradients, us, apart | not, heads of 64: four segments of up to 1000 rows 64 | 65 at
 // 256 tiles, eight 99 | 84, 32 of 100 rows 57 | 31, 64 of 200 98 | 48; heads of 128 311 | 176 and 289 | 110).
