@@ -1766,12 +1766,19 @@ def _check_pointer(pointer, name: str, device: int) -> None:
     raise RuntimeError(f"{name} must be (segments + 1,) int64 on the device of q")
 
 
+def _near(x):
+    """Rows that lie at most 16 MB apart, as the kernels read them; a copy where they lie otherwise."""
+    if x.stride(0) * x.element_size() > 1 << 24:         # contiguous() keeps the stride of a single row
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
 def _in_pieces(x):
-    """Heads whose rows are whole 16-byte pieces, as the kernels read them; a copy where they lie otherwise."""
+    """Heads whose rows are whole 16-byte pieces too; a copy where they lie otherwise."""
     size = x.element_size()
     if x.shape[2] * size % 16 == 0 and (x.data_ptr() | x.stride(0) * size | x.stride(1) * size) % 16:
         return x.clone(memory_format=torch.contiguous_format)
-    return x
+    return _near(x)
 
 
 def _attention_args(q, k, v, q_pointer, k_pointer, scale):
@@ -1827,7 +1834,7 @@ class _SegmentAttention(torch.autograd.Function):
 
 def _segment_attention(q, k, v, q_pointer, k_pointer, causal, scale, return_lse):
     dt, k_pointer, scale, sizes = _attention_args(q, k, v, q_pointer, k_pointer, scale)
-    k, v = _in_pieces(k), _in_pieces(v)
+    q, k, v = _near(q), _in_pieces(k), _in_pieces(v)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)      # contiguous, whatever q's strides
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if return_lse else None
     n = capi.load().ga_segment_attention_workspace_bytes(*sizes, dt)
