@@ -312,8 +312,9 @@ int sum_rows(const void *gy, const Plan &p, char *ws, void *grad, int64_t n_ids,
 }
 
 int check_embedding(const void *a, const void *ids, int idx_bits, const void *out, int64_t n_ids, int64_t n_table, int64_t cols,
-                    int dtype, bool any_out) {
+                    float scale, int dtype, bool any_out) {
   if (n_ids < 0 || n_table < 0 || cols <= 0 || (idx_bits != 32 && idx_bits != 64)) return GA_EINVAL;
+  if (!(scale - scale == 0.0f)) return GA_EINVAL;            // times the zeros of ids outside it would be NaN
   if (dtype != GA_F32 && dtype != GA_BF16) return GA_EUNSUPPORTED;
   if (cols > (1 << 20)) return GA_EUNSUPPORTED;
   if (n_ids > 0 && !ids) return GA_EINVAL;
@@ -345,7 +346,7 @@ extern "C" {
 int ga_embedding(const void *table, const void *ids, int idx_bits, void *y, int64_t n_ids, int64_t n_table, int64_t cols,
                  float scale, int dtype, ga_stream_t stream) {
   using namespace ga;
-  if (int rc = check_embedding(table, ids, idx_bits, y, n_ids, n_table, cols, dtype, n_ids > 0)) return rc;
+  if (int rc = check_embedding(table, ids, idx_bits, y, n_ids, n_table, cols, scale, dtype, n_ids > 0)) return rc;
   if (n_ids == 0) return GA_OK;
   if (n_table > 0 && !table) return GA_EINVAL;
   hipStream_t s = (hipStream_t)stream;
@@ -361,7 +362,7 @@ size_t ga_embedding_backward_workspace_bytes(int64_t n_ids, int64_t n_table, int
 int ga_embedding_backward(const void *grad_y, const void *ids, int idx_bits, void *grad_table, int64_t n_ids, int64_t n_table,
                           int64_t cols, float scale, int dtype, void *workspace, size_t workspace_bytes, ga_stream_t stream) {
   using namespace ga;
-  if (int rc = check_embedding(grad_y, ids, idx_bits, grad_table, n_ids, n_table, cols, dtype, n_table > 0)) return rc;
+  if (int rc = check_embedding(grad_y, ids, idx_bits, grad_table, n_ids, n_table, cols, scale, dtype, n_table > 0)) return rc;
   if (!holds(n_ids, n_table, cols)) return GA_EUNSUPPORTED;
   if (n_table == 0) return GA_OK;
   if (n_ids > 0 && !grad_y) return GA_EINVAL;

@@ -1990,6 +1990,13 @@ _ID_BITS = {torch.int64: 64, torch.int32: 32}
 EMBEDDING_MOST_RECORDED = 16 << 20     # more ids are sorted by a library, whose launches are its own
 
 
+def _finite(scale) -> float:
+    scale = float(scale)
+    if not abs(scale) < float("inf"):
+        raise RuntimeError("scale must be finite")
+    return scale
+
+
 def _check_ids(ids, device) -> int:
     _check_input(ids, "ids")
     if ids.dtype not in _ID_BITS or ids.get_device() != device:
@@ -2015,11 +2022,11 @@ class _Embedding(torch.autograd.Function):
 def _embedding(table, ids, scale):
     dt = _check_rows(table, "table")
     bits = _check_ids(ids, table.get_device())
-    cols = int(table.shape[1])
+    cols, scale = int(table.shape[1]), _finite(scale)
     y = torch.empty((*ids.shape, cols), dtype=table.dtype, device=table.device)
     if y.numel():
         _launch("ga_embedding", table.get_device(), table.data_ptr(), ids.data_ptr(), bits, y.data_ptr(), ids.numel(),
-                int(table.shape[0]), cols, float(scale), dt)
+                int(table.shape[0]), cols, scale, dt)
     return y
 
 
@@ -2042,7 +2049,7 @@ def embedding_backward(grad_y, ids, rows: int, scale: float = 1.0):
     bits = _check_ids(ids, grad_y.get_device())
     if grad_y.dim() != ids.dim() + 1 or grad_y.shape[:-1] != ids.shape or grad_y.shape[-1] == 0 or rows < 0:
         raise RuntimeError("grad_y must have a row for each id, and rows must not be negative")
-    cols = int(grad_y.shape[-1])
+    cols, scale = int(grad_y.shape[-1]), _finite(scale)
     if ids.numel() > EMBEDDING_MOST_RECORDED and torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"the gradient of more than {EMBEDDING_MOST_RECORDED} rows cannot be recorded into a HIP graph")
     grad = torch.empty((int(rows), cols), dtype=grad_y.dtype, device=grad_y.device)
@@ -2050,5 +2057,5 @@ def embedding_backward(grad_y, ids, rows: int, scale: float = 1.0):
         n = capi.load().ga_embedding_backward_workspace_bytes(ids.numel(), int(rows), cols)
         ws = _scratch(n, grad.device)
         _launch("ga_embedding_backward", grad_y.get_device(), grad_y.data_ptr(), ids.data_ptr(), bits, grad.data_ptr(),
-                ids.numel(), int(rows), cols, float(scale), dt, _ptr(ws), n)
+                ids.numel(), int(rows), cols, scale, dt, _ptr(ws), n)
     return grad

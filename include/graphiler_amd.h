@@ -927,7 +927,8 @@ int ga_linear_act_backward(const void *grad_y, const void *x, const void *weight
 
 /*
  * Embedding rows: y[i] = scale * table[ids[i]], zeros for an id outside [0, n_table).  table (n_table, cols) and y (n_ids, cols)
- * of `dtype`, ids int64 (idx_bits 64) or int32 (idx_bits 32); the product is rounded once.  GA_EUNSUPPORTED when n_ids exceeds
+ * of `dtype`, ids int64 (idx_bits 64) or int32 (idx_bits 32); the product is rounded once.  GA_EINVAL for a scale that is
+ * not finite, here and below.  GA_EUNSUPPORTED when n_ids exceeds
  * 2^31 - 128 (up to 64 columns), 2^30 - 64 (up to 128), 2^29 - 32 (up to 256) or 2^28 - 16, or cols 2^20.
  */
 int ga_embedding(const void *table, const void *ids, int idx_bits, void *y, int64_t n_ids, int64_t n_table, int64_t cols,

@@ -1,11 +1,12 @@
 """How large embedding rows and their gradient may be, without a GPU: what a launch does not hold is refused before the first one, and
-what it holds is not."""
+what it holds is not.  So is a scale that would make NaN of the zeros of ids outside the table."""
 import pytest
+import torch
 
-from graphiler_amd import capi
+from graphiler_amd import capi, ops
 
 PTR = 1 << 20            # a pointer that is aligned and never followed
-EUNSUPPORTED, EWORKSPACE = -2, -3
+EINVAL, EUNSUPPORTED, EWORKSPACE = -1, -2, -3
 LANES = [(1, 8), (64, 8), (65, 16), (128, 16), (129, 32), (256, 32), (257, 64), (4096, 64)]
 
 
@@ -34,3 +35,13 @@ def test_the_lookup(cols, lanes):
     most = 0xffffffff // 256 * (256 // lanes * 4)
     assert most == (1 << 34) // lanes - 1024 // lanes
     assert lib.ga_embedding(PTR, PTR, 64, PTR, most + 1, 10, cols, 1.0, capi.GA_BF16, None) == EUNSUPPORTED
+
+
+@pytest.mark.parametrize("scale", [float("inf"), -float("inf"), float("nan")])
+def test_a_scale_that_is_not_finite(scale):
+    lib = capi.load()
+    assert lib.ga_embedding(PTR, PTR, 64, PTR, 1 << 40, 10, 8, scale, capi.GA_F32, None) == EINVAL
+    assert lib.ga_embedding_backward(PTR, PTR, 64, PTR, 5000, 10, 8, scale, capi.GA_F32, PTR, 0, None) == EINVAL
+    with pytest.raises(RuntimeError, match="scale must be finite"):
+        ops._finite(scale)
+    assert ops._finite(torch.tensor(2.0)) == 2.0

@@ -122,3 +122,11 @@ def test_rows_at_any_address(dtype):
         gy = made((n, cols), dtype, 6)
         odd = torch.empty(n * cols + 1, dtype=dtype, device=DEV)[1:].view(n, cols).copy_(gy)
         assert torch.equal(ops.embedding_backward(gy, ids, rows), ops.embedding_backward(odd, ids, rows))
+
+
+def test_a_scale_that_is_not_finite_is_refused():
+    table, ids = made((5, 8), torch.float32, 0), torch.tensor([0, -1], device=DEV)
+    for scale in (float("inf"), float("nan")):
+        for call in (lambda: ops.embedding(table, ids, scale=scale), lambda: ops.embedding_backward(table[:2], ids, 5, scale=scale)):
+            with pytest.raises(RuntimeError, match="scale must be finite"):
+                call()
