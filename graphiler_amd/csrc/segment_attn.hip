@@ -414,10 +414,11 @@ Cut cut_of(int64_t segments, int64_t nq, int64_t nk, int64_t heads, int64_t kv_h
   c.splits = 1;
   // Wavefronts apart where workgroups of 128 rows would leave compute units without one (bf16, us, apart | shared or single, heads of 64:
   // four segments of up to 1000 rows, 8 heads, 20.5 | 20.5 at 256 tiles, eight of them 32 | 24, 32 of up to 100 rows 19.7 | 14.7; of 128 83 | 35),
-  // and where a segment's rows are one wavefront's but its keys many, which it would go through alone (one query each, 32 heads of which 8
-  // share keys, of 128: 64 segments of up to 8192 keys 138 | 360, of 1024 21 | 42; 128 of 8192 254 | 384, of 1024 37 | 46, of 256 22 | 17; 256 of
-  // 4096 253 | 281, of 512 50 | 33).  By averages, as only the device knows the lengths: one long segment among short ones is cut as they are.
-  const bool one = nq * c.pack <= 32 * some && keys >= 512;
+  // and where a segment's rows are one wavefront's but its keys many, which it would go through alone, until single wavefronts fill the chip
+  // (one query each, heads that share keys, of 128; 64 segments of up to 8192 keys, 4 key heads, 138 | 360, of 1024 21 | 42; 128 of 8192
+  // 254 | 384, of 1024 37 | 46, of 256 22 | 17; 256 of 4096 253 | 281, of 512 50 | 33; with 8 key heads 256 of 4096 450 | 481, of 1024 154 | 134,
+  // 2048 of 1024 1089 | 828).  By averages, as only the device knows the lengths: one long segment among short ones is cut as they are.
+  const bool one = nq * c.pack <= 32 * some && keys >= 512 && tiles(32) <= 1024;
   if (keys > 64 && (one || tiles(128) < 256)) {
     c.cutting = kApart;
     int64_t n = 512 / tiles(32);

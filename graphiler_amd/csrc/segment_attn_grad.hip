@@ -7,9 +7,10 @@
 //
 // Two kernels, each over 32 x 32 tiles that never leave the registers: one with 32 queries a wavefront over the keys (dq, and
 // delta on the way), one with 32 keys a wavefront over the queries of all heads that share them (dk and dv).  Both form the
-// scores again, seven products instead of the five of a single pass, which would have to add up dq from many workgroups in
-// an order of its own; here every sum has one.  p and ds are rounded to bf16 as operands (bf16 tensors), once each: what that
-// adds to a gradient is as large as its own rounding.
+// scores and <do, v> again, seven products instead of the five of a single pass, which would have to add up dq from many workgroups
+// in an order of its own; here every sum has one.  bf16 takes delta from the weights, which forms both once more (not where one
+// tile holds all keys): nine.  dk and dv of more than 64 columns are a launch each, which forms the scores once more: ten.  p and
+// ds are rounded to bf16 as operands (bf16 tensors), once each: what that adds to a gradient is as large as its own rounding.
 //
 // Measured: 8192 x 8192, 8 heads, width 64 670 us (0.51 PFLOP/s of the five products), width 128 1515 (0.45); four causal
 // sequences of up to 4096, 16 heads that share four, width 128 1135 (of it dk 430, dv 260, parts added up 47; one workgroup for

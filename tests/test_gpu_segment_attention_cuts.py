@@ -15,6 +15,7 @@ def test_keys_are_cut_for_as_many_segments_as_there_are_compute_units():
         assert small(64, 64, 64 * 8192, 32, 4, 128, dt) == 2 * 64 * 32 * 130 * 4           # two parts: sums, a maximum and a sum each
         assert small(256, 256, 256 * 4096, 32, 4, 128, dt) == 0                            # one, by four wavefronts
         assert small(256, 256, 256 * 512, 32, 4, 128, dt) == 0
+        assert small(2048, 2048, 2048 * 8192, 32, 4, 128, dt) == 0
 
 
 @pytest.mark.gpu
