@@ -5,7 +5,7 @@
 // The forward product is one launch whose store adds the bias, applies the activation and adds the residual in
 // fp32, so neither z nor act(z) is ever in memory.  The gradients form z again where an activation's slope needs it (a third of
 // their operations) instead of keeping it; dz is rounded to bf16 once, as the operand of both products after, which
-// adds to a gradient as much as its own rounding.  8192 x 1024 -> 4096 bf16: forward with relu 81 us (0.85 PFLOP/s); gradients with gelu
+// adds to a gradient as much as its own rounding.  8192 x 1024 -> 4096 bf16: forward with relu 74-81 us (0.85-0.93 PFLOP/s); gradients with gelu
 // 105 for dz (a third of it the slope), 63 for grad_x, 66 + 7 for grad_W in two parts, 12 + 4 for grad_b.  fp32: the forward product of few tiles is the fp32 instruction's
 // (gated_f32.hip), of others that of pieces which x is cut into on the way (linear_split.hip); the gradients' operands are
 // pieces laid out in memory, as in gated.hip.

@@ -7,13 +7,14 @@
 // by far, and the quotient does not depend on it), so the results are hardly ever rescaled and the halves of a
 // wavefront, which hold half of a query's keys each, speak to each other only then and at the end.
 //
-// Bound by the vector instructions at widths up to 64 (19,717 x 19,717, 8 heads of 64, 925-985 us, 0.81-0.86 PFLOP/s: an exponential, 16
+// Bound by the vector instructions at widths up to 64 (19,717 x 19,717, 8 heads of 64, 918-985 us, 0.81-0.87 PFLOP/s: an exponential, 16
 // cycles, and 15 cycles of others a score, busy .83 of the time, the matrix instructions .36) and by both together at 128
-// (8192 x 8192, 16 heads 550-575 us, 0.96-1.0 PFLOP/s; the vendor's product of 8192^3 1.14).  No LDS bank conflicts.  Two
+// (8192 x 8192, 16 heads 535-575 us, 0.96-1.03 PFLOP/s; the vendor's product of 8192^3 1.14); causal sequences of unequal length leave
+// SIMDs idle, 1.2 of two wavefronts each on average.  No LDS bank conflicts.  Two
 // workgroups a compute unit (1 -> 2 wavefronts a SIMD 850 -> 565 us) need 255 of 256 registers at 128; products at raised priority
 // 3-15 %; tiles of 32 keys 611, eight wavefronts a workgroup level on long segments and 40 % slower on short ones.  One query
 // each over 16 x 9400 keys, 32 heads of which 8 share keys: 76 + 6 us for 331 MB (4.4 TB/s).  2048 segments of 34 rows, 8 heads of 32:
-// 49 us (128 rows a workgroup 113).  fp32: 120 TFLOP/s of the instruction's 152.
+// 49 us (128 rows a workgroup 113).  fp32: 4096 x 4096, 8 heads of 64 280 us, of 128 550, 123-125 TFLOP/s of the instruction's 152.
 #include "segment_attn.h"
 
 namespace ga {

@@ -12,11 +12,11 @@
 // tile holds all keys): nine.  dk and dv of more than 64 columns are a launch each, which forms the scores once more: ten.  p and
 // ds are rounded to bf16 as operands (bf16 tensors), once each: what that adds to a gradient is as large as its own rounding.
 //
-// Measured: 8192 x 8192, 8 heads, width 64 670 us (0.51 PFLOP/s of the five products), width 128 1515 (0.45); four causal
-// sequences of up to 4096, 16 heads that share four, width 128 1135 (of it dk 430, dv 260, parts added up 47; one workgroup for
-// all heads of a group 1300); 2048 segments of 34 rows, 8 heads of 32 134.  Delta from out, in one pass over the keys, took 550,
+// Measured: 8192 x 8192, 8 heads, width 64 665-700 us (0.5 PFLOP/s of the five products), width 128 1460-1520 (0.46); four causal
+// sequences of up to 4096, 16 heads that share four, width 128 1105 (of it dq 449, dk 451, dv 266, parts added up 47; one workgroup for
+// all heads of a group 1300); 2048 segments of 34 rows, 8 heads of 32 136.  Delta from out, in one pass over the keys, took 550,
 // 1280, 1048 and 137 and left bf16's grad_q up to 1.9 times as far off as its own rounding, for 1.5 with it from the weights.
-// Held by latency: two wavefronts a SIMD where registers allow it, one for dk of wide heads.
+// Held by latency: two wavefronts a SIMD where registers allow it, one for dk of wide heads.  fp32: 4096 x 4096, 4 heads of 64, 785 us.
 #include "segment_attn.h"
 
 namespace ga {

@@ -1852,8 +1852,8 @@ def segment_attention(q, k, v, q_pointer, k_pointer=None, causal: bool = False, 
     keys k_pointer[s] to k_pointer[s + 1] (int64, ascending; without k_pointer those of the queries).  With
     ``causal`` the query at place i of its segment sees the keys at places up to i + (keys - queries).
     ``scale`` (1 / sqrt(dim)) multiplies the scores.  Returns (queries, heads, dim); with ``return_lse`` also the
-    (heads, queries) fp32 logarithms of the sums of exponentials.  A query that sees no key gives zeros and
-    -inf, as do rows in no segment.  float32 or bfloat16, dim up to 128; rows and heads may be strided (columns of one
+    (heads, queries) fp32 logarithms of the sums of exponentials.  A query that sees no key, or whose scores are all
+    -inf, gives zeros and -inf, as do rows in no segment.  float32 or bfloat16, dim up to 128; rows and heads may be strided (columns of one
     projection), dim not.  Scores and sums are fp32; bf16 weights are rounded once as operands.  Both results are differentiable
     in q, k and v (backward mode)."""
     if _wants_grad("segment_attention", q, k, v):

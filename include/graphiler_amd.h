@@ -857,7 +857,8 @@ int ga_gated_linear_fp8(const void *x8, const void *x_scales, const void *wg8, c
  *   out[i, h] = sum over j of exp(s - lse) v[j, g],  s = scale <q[i, h], k[j, g]>,  lse = log of the sum of exp(s)
  * over the keys j of query i's segment; with `causal` those whose place in the segment is at most i's plus (keys - queries).
  * Segment s has the queries q_pointer[s] ... q_pointer[s + 1] - 1 and the keys k_pointer[s] ... k_pointer[s + 1] - 1.
- * A query that sees no key, and rows in front of the first and behind the last segment, give zeros (lse -inf).
+ * A query that sees no key or whose scores are all -inf, and rows in front of the first and behind the last segment, give zeros
+ * (lse -inf).
  *   q, out   (n_queries, heads, dim), k, v (n_keys, kv_heads, dim), all of `dtype`; heads is a multiple of kv_heads, and
  *            g = h / (heads / kv_heads).  q_row ... v_head: values from row to row and from head to head of q, k and v,
  *            whose dim values lie next to each other; out is contiguous
@@ -878,9 +879,11 @@ int ga_segment_attention(const void *q, int64_t q_row, int64_t q_head, const voi
                          size_t workspace_bytes, ga_stream_t stream);
 
 /*
- * Its gradients, from out and lse: with p = exp(s - lse), ds = p (<grad_out[i], v[j]> - <grad_out[i], out[i]>),
+ * Its gradients, from out and lse: with p = exp(s - lse), ds = p (<grad_out[i], v[j]> - delta), delta = <grad_out[i], out[i]>,
  *   grad_q[i] = scale sum_j ds k[j], grad_k[j] = scale sum_i ds q[i], grad_v[j] = sum_i p grad_out[i],
- * those of k and v over all heads that share them; rows outside the segments get zeros.  grad_out, out and the gradients are
+ * those of k and v over all heads that share them; rows outside the segments get zeros.  Where the tensors are bf16, delta is
+ * sum_j p <grad_out[i], v[j]>, free of out's rounding, and out is read only for where that is not finite.  A key (or query) that is
+ * not finite, whose ds is 0 or not finite, makes its columns NaN in the gradients of the queries (keys) that see it and no others.  grad_out, out and the gradients are
  * contiguous; p and ds are rounded to bf16 as operands where the tensors are bf16.  No sum's order depends on anything but the
  * sizes.  Where dim values are whole 16-byte pieces, q and grad_out have to be 16-byte aligned as k and v are.
  */
